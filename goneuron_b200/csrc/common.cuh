@@ -314,3 +314,5 @@ __device__ __forceinline__ float block_max(float v, float* red) {
 }
 
 }  // namespace gn
+
+struct gn_ctx { gn::Ctx c; bool alive = true; };

@@ -152,8 +152,6 @@ struct LayerRT {
 
 }  // namespace gn
 
-struct gn_ctx { gn::Ctx c; bool alive = true; };
-
 namespace gn { struct StepGraph; }
 struct gn_model {
   ~gn_model();

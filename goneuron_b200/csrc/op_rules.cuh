@@ -1,0 +1,139 @@
+// op_rules.cuh -- operators on device memory: what a call's arguments must be, and how its work is cut.  Plain C++ (tested on the CPU).
+// The checks return null, or what is wrong.
+#pragma once
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+
+#include "../../include/goneuron_cuda.h"
+
+namespace gn {
+
+constexpr int64_t OP_MAX_ROWS = 0x7fffffff;                          // tokens, rows, vocabulary
+inline int dtype_size(int dtype) { return dtype == GN_F32 ? 4 : dtype == GN_F16 || dtype == GN_BF16 ? 2 : 0; }
+inline bool aligned_to(const void* p, int64_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+inline int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
+inline const char* check_dtype(int dtype, const void* p) {
+  if (!dtype_size(dtype)) return "dtype is none of GN_F32, GN_F16, GN_BF16";
+  return aligned_to(p, dtype_size(dtype)) ? nullptr : "a pointer is not aligned to its type";
+}
+inline const char* check_index(int index_type, const void* p) {
+  if (index_type != GN_I32 && index_type != GN_I64) return "index_type is neither GN_I32 nor GN_I64";
+  return aligned_to(p, index_type == GN_I64 ? 8 : 4) ? nullptr : "an index pointer is not aligned to its type";
+}
+
+// ------------------------------------------------------------------ norm of queries and keys with the rotation
+struct QkArgs {
+  int dtype; int64_t tokens; int head_size, rotated; float eps; const gn_heads *q, *k; const float *gain_q, *gain_k;
+  const void* positions; int index_type; const double* frequencies;
+};
+inline const char* check_heads(const QkArgs& a, const gn_heads* h, int heads, bool written) {
+  if (!h || h->heads != heads) return "tensors of the same heads are needed for every input and output";
+  if (a.tokens && heads && !h->data) return "a data pointer is null";
+  if (const char* e = check_dtype(a.dtype, h->data)) return e;
+  if (h->token_stride < 0 || h->head_stride < 0) return "a stride is negative";
+  if (written && ((a.tokens > 1 && h->token_stride < a.head_size) || (heads > 1 && h->head_stride < a.head_size))) return "an output's rows overlap";
+  return nullptr;
+}
+inline const char* check_qk(const QkArgs& a) {
+  if (!dtype_size(a.dtype)) return "dtype is none of GN_F32, GN_F16, GN_BF16";
+  if (a.tokens < 0 || a.tokens > OP_MAX_ROWS) return "tokens out of range";
+  if (a.head_size < 1 || a.head_size > 1024) return "head_size is not in [1, 1024]";
+  if (a.rotated < 0 || a.rotated > a.head_size || a.rotated % 2) return "rotated is not an even number of at most head_size elements";
+  if (!(a.eps >= 0.f) || std::isinf(a.eps)) return "eps is negative or not finite";
+  if (!a.q) return "q is null";
+  if (a.q->heads < 0 || a.q->heads > 65536 || (a.k && (a.k->heads < 0 || a.k->heads > 65536))) return "the number of heads is not in [0, 65536]";
+  if (!aligned_to(a.gain_q, 4) || !aligned_to(a.gain_k, 4) || !aligned_to(a.frequencies, 8)) return "a pointer is not aligned to its type";
+  if (a.rotated && a.tokens && (!a.positions || !a.frequencies)) return "positions and frequencies are needed for a rotation";
+  if (a.rotated) if (const char* e = check_index(a.index_type, a.positions)) return e;
+  if (const char* e = check_heads(a, a.q, a.q->heads, false)) return e;
+  return a.k ? check_heads(a, a.k, a.k->heads, false) : nullptr;
+}
+// Groups of lanes: a lane has two 16-byte pieces of a row, and a row's lanes are neighbours, 2 to 32 of them.  0: the row goes element by element
+// (sizes, strides or pointers that 16-byte pieces do not fit, pairs that end inside one, rows of more than 64 pieces).
+inline int qk_group(int dtype, int head_size, int rotated, bool interleaved, const gn_heads* const* t, int n) {
+  const int vec = 16 / dtype_size(dtype), pieces = head_size / vec;
+  if (head_size % vec || pieces > 64 || (!interleaved && rotated % (2 * vec))) return 0;
+  for (int i = 0; i < n; i++)
+    if (t[i] && (!aligned_to(t[i]->data, 16) || t[i]->token_stride % vec || t[i]->head_stride % vec)) return 0;
+  int g = 2;
+  while (2 * g < pieces) g *= 2;
+  return g;
+}
+// Tokens of a block at a time: four share their block's cosines' latency once there is work for every multiprocessor, one each before that.
+inline int qk_tokens(int64_t tokens, int sms) { return tokens >= 8L * sms ? 4 : 1; }
+// Blocks: all resident at once, so that a gradient's blocks leave no more partial sums than those.
+inline int64_t qk_blocks(int64_t tokens, int sms, int per_sm) { return std::max<int64_t>(1, std::min<int64_t>(ceil_div(tokens, qk_tokens(tokens, sms)), (int64_t)sms * per_sm)); }
+constexpr int QK_PER_SM = 3;                                      // (of the gradient: 85 registers a thread; with four blocks of 64 it spilled)
+inline int64_t qk_workspace(int64_t tokens, int head_size, int sms) { return qk_blocks(tokens, sms, QK_PER_SM) * 2 * head_size * 4; }
+
+// ------------------------------------------------------------------ distillation
+inline const char* check_distill(int dtype, int64_t rows, int64_t vocab, int top, float temperature, const void* logits, int64_t row_stride, const void* top_ids, int index_type,
+                                 const float* top_logits, const float* weight, const float* loss, const void* dlogits, int64_t drow_stride) {
+  if (rows < 0 || rows > OP_MAX_ROWS) return "rows out of range";
+  if (vocab < 1 || vocab > OP_MAX_ROWS) return "vocab out of range";
+  if (top < 0 || top > 1024) return "top is not in [0, 1024]";
+  if (!(temperature > 0.f) || std::isinf(temperature)) return "temperature is not positive and finite";
+  if (rows && (!logits || !loss || (top && (!top_ids || !top_logits)))) return "a data pointer is null";
+  if (const char* e = check_dtype(dtype, logits)) return e;
+  if (const char* e = check_dtype(dtype, dlogits)) return e;
+  if (const char* e = check_index(index_type, top_ids)) return e;
+  if (!aligned_to(top_logits, 4) || !aligned_to(weight, 4) || !aligned_to(loss, 4)) return "a pointer is not aligned to its type";
+  if (row_stride < 0 || (rows > 1 && dlogits && drow_stride < vocab)) return "rows overlap, or a stride is negative";
+  if (dlogits && dlogits == logits && rows > 1 && row_stride != drow_stride) return "in place, both strides have to be the same";
+  return nullptr;
+}
+// A row is kept on chip: `threads` threads of each of `cluster` blocks hold DISTILL_ITEMS elements each in registers.  cluster 0: the row does not fit, and is
+// read again instead.  Few rows are cut further, so that they fill the multiprocessors, down to a thousand elements per block.
+constexpr int DISTILL_ITEMS = 32;
+struct DistillPlan { int cluster, threads; };
+inline DistillPlan distill_plan(int64_t rows, int64_t vocab, int sms) {
+  const int64_t slack = 16;                                          // a row may begin inside a 16-byte piece
+  int c = 1;
+  while (c < 8 && vocab + slack * c > (int64_t)c * 1024 * DISTILL_ITEMS) c *= 2;
+  if (vocab + slack * c > (int64_t)c * 1024 * DISTILL_ITEMS) return {0, 1024};
+  while (c < 8 && rows * c * 2 <= sms && vocab >= 2048L * c) c *= 2;
+  int threads = 1024;                                                // the fewest of 64, 256, 512, 1024 that hold a block's part: blocks of one multiprocessor overlap each other's barriers
+  for (int t : {512, 256, 64}) if (ceil_div(vocab, c) + slack <= (int64_t)t * DISTILL_ITEMS) threads = t;
+  return {c, threads};
+}
+
+// ------------------------------------------------------------------ embedding
+inline const char* check_embedding(int dtype, int64_t tokens, int64_t vocab, int dim, float scale, const void* rows_in, int64_t in_stride, int64_t in_rows, const void* ids, int index_type,
+                                   const void* out, int64_t out_stride, int64_t out_rows) {
+  if (tokens < 0 || tokens > OP_MAX_ROWS) return "tokens out of range";
+  if (vocab < 1 || vocab >= OP_MAX_ROWS) return "vocab out of range";
+  if (dim < 1) return "dim out of range";
+  if (!(std::fabs(scale) <= 3.4028235e38f)) return "scale is not finite";
+  if ((in_rows && !rows_in) || (tokens && !ids) || (out_rows && !out)) return "a data pointer is null";
+  if (const char* e = check_dtype(dtype, rows_in)) return e;
+  if (const char* e = check_index(index_type, ids)) return e;
+  if (in_stride < 0 || (out_rows > 1 && out_stride < dim)) return "rows overlap, or a stride is negative";
+  return nullptr;
+}
+// The tokens' order by id, then sums of it in pieces of `chunk` neighbouring places.  Up to SORT_SMALL tokens one block sorts them in shared memory; above, passes of
+// 8 bits over tiles of SORT_TILE tokens.
+constexpr int SORT_SMALL = 8192, SORT_TILE = 2048, SORT_BITS = 8;
+struct EmbeddingPlan {
+  bool small; int bits, passes, chunk; int64_t tiles, chunks;
+  int64_t keys, order, keys2, order2, hist, partial, bytes;          // places in the workspace, in bytes
+};
+inline EmbeddingPlan embedding_plan(int64_t tokens, int64_t vocab, int dim, int sms) {
+  EmbeddingPlan p{};
+  p.small = tokens <= SORT_SMALL;
+  p.bits = 1;
+  while (((int64_t)1 << p.bits) <= vocab) p.bits++;                  // keys 0 .. vocab (padding)
+  p.passes = (int)ceil_div(p.bits, SORT_BITS);
+  p.chunk = 4;                                                       // places of a piece: some eight pieces for each multiprocessor, 64 at most
+  while (p.chunk < 64 && tokens > (int64_t)p.chunk * 8 * sms) p.chunk *= 2;
+  p.tiles = ceil_div(tokens, SORT_TILE); p.chunks = ceil_div(tokens, p.chunk);
+  int64_t at = 0; auto take = [&](int64_t bytes) { const int64_t a = at; at += round_up(bytes, 256); return a; };
+  p.keys = take(4 * tokens); p.order = take(4 * tokens);
+  p.keys2 = take(p.small ? 0 : 4 * tokens); p.order2 = take(p.small ? 0 : 4 * tokens);
+  p.hist = take(p.small ? 0 : 4 * (p.tiles << SORT_BITS));
+  p.partial = take(p.chunks * 2 * (int64_t)dim * 4);                 // a piece's first and last sum may go on in its neighbours
+  p.bytes = at; return p;
+}
+
+}  // namespace gn

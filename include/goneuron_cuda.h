@@ -281,6 +281,76 @@ int gn_op_lstm(gn_ctx* ctx, int engine, int B, int T, int in_size, int H, const 
 int gn_op_gemm_nt_static(gn_ctx* ctx, int M, int N, int K, const float* A_dev, const float* B_dev,
                          const float* bias_dev, float* C_dev);
 
+/* ---- operators on device memory ------------------------------------------
+ * Operators of language models for callers that keep their tensors on the GPU (a cgo host with its own device buffers,
+ * torch tensors through goneuron_b200/operators.py).  They have no counterpart in the reference, whose layers are
+ * float32 on host slices: 16-bit types, true gradients where the layer keeps the reference's literal ones, forms for
+ * one token at a time.
+ *   - Data pointers are DEVICE memory of the context's GPU; strides count elements; the last dimension is contiguous.
+ *   - `stream` is a cudaStream_t of that GPU (0: CUDA's default stream).  A call enqueues its kernels there and returns:
+ *     it allocates nothing, waits for nothing, changes neither the calling thread's current device nor any state of the
+ *     context, and can be captured into a graph.  Calls on several streams or threads may overlap.
+ *   - `workspace` is device memory of at least the bytes that the operator's _workspace function gives (16-byte aligned;
+ *     may be null where that is 0).  Its contents mean nothing before and after the call; calls that may run at the same
+ *     time, replayed graphs among them, need one each.
+ *   - Outputs must not overlap inputs or each other except where an operator says so.
+ *   - What a kernel finds wrong while it runs (an index out of range, a bounded wait that gave up) is kept in one word of
+ *     the GPU until gn_op_status reads it. */
+typedef enum gn_dtype { GN_F32 = 0, GN_F16 = 1, GN_BF16 = 2 } gn_dtype;
+typedef enum gn_index_type { GN_I32 = 0, GN_I64 = 1 } gn_index_type;
+
+/* Waits for `stream` and returns what the operators found wrong on this GPU since the last call that reported it:
+ * GN_ERR_INVALID_ARG (a token id or teacher index out of range), GN_ERR_TIMEOUT (a bounded wait gave up), else GN_OK. */
+int gn_op_status(gn_ctx* ctx, void* stream);
+
+/* heads of a tensor [tokens, heads, head_size] */
+typedef struct gn_heads {
+  void* data;
+  int64_t token_stride, head_stride;   /* in elements */
+  int32_t heads, reserved;
+} gn_heads;
+
+/* Norm of queries and keys per head with the position rotation in the same pass:
+ *   y = R(position) (gain * x / sqrt(mean(x^2) + eps)),
+ * R turning the pair (x[i], x[i + rotated/2]) -- interleaved: (x[2i], x[2i + 1]) -- of the first `rotated` elements by
+ * position * frequencies[i]; the others stay.  The angle is formed and reduced in 64 bits.  q, k -> q_out, k_out of the same
+ * heads (in place where pointer and strides are the same); k and k_out may both be null.  gain_q, gain_k: float32 [head_size],
+ * null for 1.  positions: [tokens] of index_type; frequencies: float64 [rotated / 2]; both may be null where rotated is 0.
+ * head_size <= 1024; rotated even, <= head_size.  The rotation is that of TransformerBlock with useRoPE (transformer.go:212-236). */
+int gn_op_qk_norm_rope(gn_ctx* ctx, int dtype, int64_t tokens, int head_size, int rotated, int interleaved, float eps,
+                       const gn_heads* q, const gn_heads* k, const float* gain_q, const float* gain_k,
+                       const void* positions, int index_type, const double* frequencies,
+                       const gn_heads* q_out, const gn_heads* k_out, void* stream);
+/* Its gradient: dy of the outputs (dq_out, dk_out) -> dq, dk (may be dq_out, dk_out in place) and, float32 [head_size] and null
+ * where not wanted, dgain_q, dgain_k (sums over tokens and heads in an order that only the sizes fix). */
+int gn_op_qk_norm_rope_workspace(gn_ctx* ctx, int64_t tokens, int q_heads, int k_heads, int head_size, int64_t* bytes);
+int gn_op_qk_norm_rope_backward(gn_ctx* ctx, int dtype, int64_t tokens, int head_size, int rotated, int interleaved, float eps,
+                                const gn_heads* q, const gn_heads* k, const float* gain_q, const float* gain_k,
+                                const void* positions, int index_type, const double* frequencies,
+                                const gn_heads* dq_out, const gn_heads* dk_out, const gn_heads* dq, const gn_heads* dk,
+                                float* dgain_q, float* dgain_k, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Distillation from a teacher's top logits.  With p = softmax(top_logits / temperature) over the entries of a row whose index is
+ * not -1 and q = softmax(logits / temperature) over the vocabulary,
+ *   loss[r] = weight[r] temperature^2 sum_k p_k (log p_k - log q_{index k}),   dlogits[r] = weight[r] temperature (q - p)
+ * (the derivative of loss[r] by logits[r]; an index that occurs twice counts twice).  A row whose weight is 0, or that has no entry of
+ * positive probability, has loss 0 and gradient 0 whatever its logits hold.  logits [rows, vocab] and dlogits (null: loss only; may be
+ * logits in place) of `dtype`, rows row_stride / drow_stride elements apart; top_ids [rows, top] of index_type, top_logits float32 [rows, top],
+ * dense; weight float32 [rows] (null: 1); loss float32 [rows].  top <= 1024.  An index outside [-1, vocab) counts as -1 and sets the status. */
+int gn_op_distill(gn_ctx* ctx, int dtype, int64_t rows, int64_t vocab, int top, float temperature,
+                  const void* logits, int64_t row_stride, const void* top_ids, int index_type, const float* top_logits,
+                  const float* weight, float* loss, void* dlogits, int64_t drow_stride, void* stream);
+
+/* Embedding lookup: out[i] = scale * table[ids[i]], rows of zeros where ids[i] is -1.  table [vocab, dim] and out [tokens, dim] of
+ * `dtype`, rows table_stride / out_stride elements apart.  An id outside [-1, vocab) counts as -1 and sets the status. */
+int gn_op_embedding(gn_ctx* ctx, int dtype, int64_t tokens, int64_t vocab, int dim, float scale, const void* table, int64_t table_stride,
+                    const void* ids, int index_type, void* out, int64_t out_stride, void* stream);
+/* Its gradient, every row of it: dtable[v] = scale * sum of dout[i] over the tokens i with ids[i] = v, float32, dense [vocab, dim].  The
+ * tokens are sorted by id first (stable), and the order of a row's sum depends on the sizes alone: the same call gives the same bits. */
+int gn_op_embedding_workspace(gn_ctx* ctx, int64_t tokens, int64_t vocab, int dim, int64_t* bytes);
+int gn_op_embedding_backward(gn_ctx* ctx, int dtype, int64_t tokens, int64_t vocab, int dim, float scale, const void* dout, int64_t dout_stride,
+                             const void* ids, int index_type, float* dtable, void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

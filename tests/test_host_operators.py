@@ -1,0 +1,163 @@
+"""Operators on device memory, without a GPU: the argument checks and the plans of op_rules.cuh (plain C++), and the refusals of the Python functions."""
+import os
+import subprocess
+import tempfile
+
+import pytest
+import torch
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+SRC = r'''
+#include <cstdio>
+#include "goneuron_b200/csrc/op_rules.cuh"
+using namespace gn;
+static int bad = 0;
+#define OK(x) do { if (const char* e_ = (x)) { bad++; std::printf("line %d: refused: %s\n", __LINE__, e_); } } while (0)
+#define NO(x) do { if (!(x)) { bad++; std::printf("line %d: not refused\n", __LINE__); } } while (0)
+#define IS(x) do { if (!(x)) { bad++; std::printf("line %d: %s\n", __LINE__, #x); } } while (0)
+static void* at(uintptr_t a) { return reinterpret_cast<void*>(a); }
+
+static void qk() {
+  gn_heads q{at(4096), 512, 64, 8, 0}, k{at(8192), 512, 64, 2, 0};
+  const float* g = (const float*)at(256); const double* f = (const double*)at(512); const void* pos = at(1024);
+  const QkArgs a{GN_F16, 10, 64, 64, 1e-5f, &q, &k, g, g, pos, GN_I64, f};
+  OK(check_qk(a));
+  QkArgs b = a; b.dtype = 3; NO(check_qk(b));
+  b = a; b.tokens = -1; NO(check_qk(b));
+  b = a; b.tokens = 1LL << 31; NO(check_qk(b));
+  for (int size : {0, -1, 1025}) { b = a; b.head_size = size; b.rotated = 0; NO(check_qk(b)); }
+  for (int rot : {-2, 63, 66}) { b = a; b.rotated = rot; NO(check_qk(b)); }
+  b = a; b.eps = -1.f; NO(check_qk(b)); b.eps = NAN; NO(check_qk(b)); b.eps = INFINITY; NO(check_qk(b));
+  b = a; b.q = nullptr; NO(check_qk(b));
+  b = a; b.k = nullptr; OK(check_qk(b));
+  b = a; b.positions = nullptr; NO(check_qk(b)); b.rotated = 0; OK(check_qk(b));
+  b = a; b.frequencies = nullptr; NO(check_qk(b));
+  b = a; b.frequencies = (const double*)at(516); NO(check_qk(b));
+  b = a; b.index_type = 2; NO(check_qk(b));
+  b = a; b.positions = at(1028); NO(check_qk(b)); b.index_type = GN_I32; OK(check_qk(b));
+  gn_heads r = q; r.data = at(4097); b = a; b.q = &r; NO(check_qk(b));
+  r = q; r.data = nullptr; NO(check_qk(b)); b.tokens = 0; OK(check_qk(b));
+  r = q; r.heads = -1; b = a; b.q = &r; NO(check_qk(b));
+  r = q; r.token_stride = -512; NO(check_qk(b));
+  r = q; r.token_stride = 0; OK(check_qk(b)); NO(check_heads(b, &r, 8, true));      // one row for all: as an input only
+  r = q; r.head_stride = 63; NO(check_heads(b, &r, 8, true));
+  NO(check_heads(a, &k, 8, true)); NO(check_heads(a, nullptr, 8, true));
+  const gn_heads* all[] = {&q, &k, nullptr};
+  IS(qk_group(GN_F16, 64, 64, false, all, 3) == 4); IS(qk_group(GN_F32, 64, 64, false, all, 3) == 8); IS(qk_group(GN_F16, 512, 512, false, all, 3) == 32);
+  IS(qk_group(GN_F16, 65, 64, false, all, 3) == 0); IS(qk_group(GN_F16, 64, 24, false, all, 3) == 0); IS(qk_group(GN_F16, 64, 24, true, all, 3) == 4); IS(qk_group(GN_F16, 1024, 0, false, all, 3) == 0);
+  gn_heads odd = q; odd.token_stride = 513; all[0] = &odd; IS(qk_group(GN_F16, 64, 64, false, all, 3) == 0);
+  odd = q; odd.data = at(4098); IS(qk_group(GN_F16, 64, 64, false, all, 3) == 0);
+  for (long n : {1L, 7L, 1184L, 65536L, 2000000000L}) for (int sms : {1, 148}) {
+    const long blocks = qk_blocks(n, sms, QK_PER_SM);
+    IS(blocks >= 1 && blocks <= (long)sms * QK_PER_SM && blocks <= n); IS(qk_workspace(n, 128, sms) == blocks * 1024);
+  }
+}
+static void distill() {
+  const float *t = (const float*)at(256), *w = (const float*)at(512), *l = (const float*)at(1024); void *x = at(4096), *d = at(1 << 20), *ids = at(2048);
+  OK(check_distill(GN_BF16, 4, 100, 8, 1.f, x, 100, ids, GN_I64, t, w, l, d, 100)); OK(check_distill(GN_BF16, 4, 100, 8, 1.f, x, 100, ids, GN_I64, t, nullptr, l, nullptr, 0));
+  OK(check_distill(GN_BF16, 4, 100, 0, 1.f, x, 0, nullptr, GN_I64, nullptr, w, l, d, 100)); OK(check_distill(GN_F32, 0, 100, 8, 1.f, nullptr, 100, nullptr, GN_I32, nullptr, nullptr, nullptr, nullptr, 0));
+  NO(check_distill(9, 4, 100, 8, 1.f, x, 100, ids, GN_I64, t, w, l, d, 100)); NO(check_distill(GN_BF16, -4, 100, 8, 1.f, x, 100, ids, GN_I64, t, w, l, d, 100));
+  NO(check_distill(GN_BF16, 4, 0, 8, 1.f, x, 100, ids, GN_I64, t, w, l, d, 100)); NO(check_distill(GN_BF16, 4, 100, 1025, 1.f, x, 100, ids, GN_I64, t, w, l, d, 100));
+  for (float tau : {0.f, -1.f, NAN, INFINITY}) NO(check_distill(GN_BF16, 4, 100, 8, tau, x, 100, ids, GN_I64, t, w, l, d, 100));
+  NO(check_distill(GN_BF16, 4, 100, 8, 1.f, nullptr, 100, ids, GN_I64, t, w, l, d, 100)); NO(check_distill(GN_BF16, 4, 100, 8, 1.f, x, 100, nullptr, GN_I64, t, w, l, d, 100));
+  NO(check_distill(GN_BF16, 4, 100, 8, 1.f, x, 100, ids, GN_I64, nullptr, w, l, d, 100)); NO(check_distill(GN_BF16, 4, 100, 8, 1.f, x, 100, ids, GN_I64, t, w, nullptr, d, 100));
+  NO(check_distill(GN_BF16, 4, 100, 8, 1.f, at(4097), 100, ids, GN_I64, t, w, l, d, 100)); NO(check_distill(GN_F32, 4, 100, 8, 1.f, x, 100, ids, GN_I64, t, w, l, at(4098), 100));
+  NO(check_distill(GN_BF16, 4, 100, 8, 1.f, x, 100, at(2052), GN_I64, t, w, l, d, 100)); NO(check_distill(GN_BF16, 4, 100, 8, 1.f, x, 100, ids, 2, t, w, l, d, 100));
+  NO(check_distill(GN_BF16, 4, 100, 8, 1.f, x, 100, ids, GN_I64, (const float*)at(258), w, l, d, 100)); NO(check_distill(GN_BF16, 4, 100, 8, 1.f, x, -1, ids, GN_I64, t, w, l, d, 100));
+  NO(check_distill(GN_BF16, 4, 100, 8, 1.f, x, 100, ids, GN_I64, t, w, l, d, 99)); OK(check_distill(GN_BF16, 1, 100, 8, 1.f, x, 100, ids, GN_I64, t, w, l, d, 0));
+  NO(check_distill(GN_BF16, 4, 100, 8, 1.f, x, 104, ids, GN_I64, t, w, l, x, 100)); OK(check_distill(GN_BF16, 4, 100, 8, 1.f, x, 104, ids, GN_I64, t, w, l, x, 104));
+  // a block's part of a row, wherever it begins within 16 bytes, fits its threads' registers
+  for (long rows : {1L, 24L, 149L, 100000L}) for (int v = 0; v < 40; v++) for (long vocab = std::max(1L, (1L << v / 2) - 17); vocab < (1L << v / 2) + 17 && vocab < 2000000; vocab++)
+    for (int size : {2, 4}) {
+      const DistillPlan p = distill_plan(rows, vocab, 148);
+      if (p.cluster == 0) { IS(vocab > 8 * 32768 - 200); continue; }
+      const int V = 16 / size;
+      for (int lead = 0; lead < V; lead++) { const long pieces = ceil_div(lead + vocab, V); if (ceil_div(pieces, p.cluster) > (long)p.threads * DISTILL_ITEMS / V) { bad++; std::printf("vocab %ld rows %ld\n", vocab, rows); } }
+    }
+}
+static void embedding() {
+  void *x = at(4096), *ids = at(2048), *out = at(1 << 20);
+  OK(check_embedding(GN_F16, 5, 100, 33, 1.f, x, 33, 100, ids, GN_I32, out, 33, 5)); OK(check_embedding(GN_F16, 0, 100, 33, 1.f, x, 33, 100, nullptr, GN_I32, nullptr, 33, 0));
+  NO(check_embedding(GN_F16, -1, 100, 33, 1.f, x, 33, 100, ids, GN_I32, out, 33, 5)); NO(check_embedding(GN_F16, 5, 0, 33, 1.f, x, 33, 100, ids, GN_I32, out, 33, 5));
+  NO(check_embedding(GN_F16, 5, 0x7fffffff, 33, 1.f, x, 33, 100, ids, GN_I32, out, 33, 5)); NO(check_embedding(GN_F16, 5, 100, 0, 1.f, x, 33, 100, ids, GN_I32, out, 33, 5));
+  NO(check_embedding(GN_F16, 5, 100, 33, NAN, x, 33, 100, ids, GN_I32, out, 33, 5)); NO(check_embedding(GN_F16, 5, 100, 33, INFINITY, x, 33, 100, ids, GN_I32, out, 33, 5));
+  NO(check_embedding(GN_F16, 5, 100, 33, 1.f, nullptr, 33, 100, ids, GN_I32, out, 33, 5)); NO(check_embedding(GN_F16, 5, 100, 33, 1.f, x, 33, 100, nullptr, GN_I32, out, 33, 5));
+  NO(check_embedding(GN_F16, 5, 100, 33, 1.f, x, 33, 100, ids, GN_I32, nullptr, 33, 5)); NO(check_embedding(GN_F16, 5, 100, 33, 1.f, x, 33, 100, ids, GN_I32, out, 32, 5));
+  NO(check_embedding(7, 5, 100, 33, 1.f, x, 33, 100, ids, GN_I32, out, 33, 5)); NO(check_embedding(GN_F16, 5, 100, 33, 1.f, x, 33, 100, at(2049), GN_I32, out, 33, 5));
+  NO(check_embedding(GN_F16, 5, 100, 33, 1.f, x, -33, 100, ids, GN_I32, out, 33, 5));
+  for (long n : {1L, 8192L, 8193L, 131072L, 2147483647L}) for (long vocab : {1L, 255L, 256L, 65535L, 65536L, 2147483646L}) for (int dim : {1, 1024}) {
+    const EmbeddingPlan p = embedding_plan(n, vocab, dim, 148);
+    IS((1LL << p.bits) > vocab && p.passes * SORT_BITS >= p.bits && p.passes <= 4); IS(p.chunk >= 4 && p.chunk <= 64); IS(p.chunks * p.chunk >= n && (p.chunks - 1) * p.chunk < n);
+    IS(p.small || p.tiles * SORT_TILE >= n); IS(p.keys % 256 == 0 && p.order >= p.keys + 4 * n && p.partial + p.chunks * 2 * dim * 4 <= p.bytes);
+    if (!p.small) IS(p.keys2 >= p.order + 4 * n && p.order2 >= p.keys2 + 4 * n && p.hist >= p.order2 + 4 * n && p.partial >= p.hist + 4 * (p.tiles << SORT_BITS));
+  }
+}
+int main() { qk(); distill(); embedding(); std::printf("%d bad\n", bad); return bad != 0; }
+'''
+
+
+def test_checks_and_plans():
+    with tempfile.TemporaryDirectory() as d:
+        src, exe = os.path.join(d, "t.cpp"), os.path.join(d, "t")
+        open(src, "w").write(SRC)
+        subprocess.check_call(["g++", "-std=c++17", "-O1", "-I", ROOT, "-x", "c++", src, "-o", exe])
+        r = subprocess.run([exe], capture_output=True, text=True, timeout=120)
+        assert r.returncode == 0, r.stdout
+
+
+class _NoDevice:
+    """Stands in for a Device where a call must not get as far as the library."""
+    device, handle = 0, None
+
+
+class _OnGpu(torch.Tensor):
+    """A tensor that says it is on the GPU, for the checks behind the one of the device."""
+    is_cuda = True
+    device = torch.device("cuda", 0)
+
+
+def _gpu(*shape, dtype=torch.float32):
+    return torch.zeros(*shape, dtype=dtype).as_subclass(_OnGpu)
+
+
+def test_python_refusals_need_no_gpu():
+    from goneuron_b200 import operators as ops
+    dev, q, ids = _NoDevice(), _gpu(6, 2, 8), _gpu(6, dtype=torch.int64)
+    freq = _gpu(4, dtype=torch.float64)
+    refused = [
+        lambda: ops.qk_norm_rope(dev, torch.zeros(6, 2, 8), None),                                           # not on the GPU
+        lambda: ops.qk_norm_rope(dev, "q", None), lambda: ops.qk_norm_rope(dev, _gpu(6, 8), None), lambda: ops.qk_norm_rope(dev, q.double(), None),
+        lambda: ops.qk_norm_rope(dev, q.transpose(1, 2), None), lambda: ops.qk_norm_rope(dev, q, _gpu(5, 2, 8)), lambda: ops.qk_norm_rope(dev, q, _gpu(6, 2, 8, dtype=torch.float16)),
+        lambda: ops.qk_norm_rope(dev, q, None, _gpu(7)), lambda: ops.qk_norm_rope(dev, q, None, _gpu(8, dtype=torch.float16)),
+        lambda: ops.qk_norm_rope(dev, q, None, None, None, None, freq), lambda: ops.qk_norm_rope(dev, q, None, None, None, ids[:5], freq),
+        lambda: ops.qk_norm_rope(dev, q, None, None, None, ids.float(), freq), lambda: ops.qk_norm_rope(dev, q, None, None, None, ids, freq.float()),
+        lambda: ops.qk_norm_rope(dev, _gpu(3, 2, 2, 8).transpose(0, 1), None), lambda: ops.qk_norm_rope(dev, q, None, out=(_gpu(6, 2, 7), None)),
+        lambda: ops.qk_norm_rope_backward(dev, _gpu(6, 1, 8), None, q, None),
+        lambda: ops.distill_loss(dev, _gpu(4, 10), _gpu(4, 3, dtype=torch.int64), _gpu(4, 2)), lambda: ops.distill_loss(dev, _gpu(4, 10), _gpu(5, 3, dtype=torch.int64), _gpu(5, 3)),
+        lambda: ops.distill_loss(dev, _gpu(4, 10), _gpu(4, 3), _gpu(4, 3)), lambda: ops.distill_loss(dev, _gpu(4, 10), _gpu(4, 3, dtype=torch.int32), _gpu(4, 3, dtype=torch.float16)),
+        lambda: ops.distill_loss(dev, _gpu(10, 4).t(), _gpu(4, 3, dtype=torch.int32), _gpu(4, 3)), lambda: ops.distill_loss(dev, _gpu(4, 10), _gpu(4, 3, dtype=torch.int32), _gpu(4, 3), 1.0, _gpu(3)),
+        lambda: ops.distill_loss_grad(dev, _gpu(4, 10), _gpu(4, 3, dtype=torch.int32), _gpu(4, 3), out=_gpu(4, 9)),
+        lambda: ops.embedding(dev, _gpu(10), ids), lambda: ops.embedding(dev, _gpu(10, 4), ids.float()), lambda: ops.embedding(dev, _gpu(10, 4).t(), ids), lambda: ops.embedding(dev, _gpu(10, 4), ids[::2]),
+        lambda: ops.embedding_backward(dev, _gpu(5, 4), ids, 10), lambda: ops.embedding_backward(dev, _gpu(6, 4, dtype=torch.int32), ids, 10),
+    ]
+    for i, call in enumerate(refused):
+        with pytest.raises(ValueError):
+            call()
+            print("not refused:", i)
+
+
+def test_a_closed_device_is_a_status_code():
+    """Every entry point refuses a null context before anything else."""
+    from goneuron_b200 import _lib, build
+    build.build()
+    lib = _lib.load()
+    for name in (n for n in _lib.EXPORTS if n.startswith("gn_op_") and n in lib_device_operators()):
+        f = getattr(lib, name)
+        assert f(*[t() if t is not None else None for t in f.argtypes]) == -1, name
+        assert b"context is null" in lib.gn_last_error() or b"bad argument" in lib.gn_last_error()
+
+
+def lib_device_operators():
+    header = open(os.path.join(ROOT, "include", "goneuron_cuda.h")).read()
+    return header[header.index("operators on device memory"):]
