@@ -7,19 +7,24 @@
 // another before it sums; (m, sum) pairs then meet in shuffles, in shared memory and between the blocks of a cluster, and q_j = e_j 2^((m - M) c) / S.  Differences
 // come before the factor: logits at the type's lowest value stay finite.
 //
-// Bound by memory: a row is read once and its gradient written once.  A row stays on chip, 32 elements a thread in registers as float32 exponentials (one exponential an element:
-// with two the special-function units bound it, 2 x 11 an SM and cycle at full bandwidth against the 16 they give).  While a row is in registers the same
+// Bound by memory: a row is read once and its gradient written once.  One launch forms what the teacher's few entries come to, a warp a row, so that no long
+// row waits for their chain of dependent loads; the second streams the rows.  A row stays on chip there, 32 elements a thread in registers as float32 exponentials (one exponential
+// an element: with two the special-function units bound it, 2 x 11 an SM and cycle at full bandwidth against the 16 they give).  While a row is in registers the same
 // thread's asynchronous copies fetch its elements of the next one, into slots of shared memory that no other thread touches, so that the only barrier
-// of a row is the one at which the sums meet.  A row that is too long for one block is spread over a cluster of up to eight.
-// Each block writes q for all of its elements; where the teacher has entries q - p is written over it, behind the next row's barrier.
+// of a row is the one at which the sums meet.  A row that is too long for 512 threads is spread over a cluster of blocks, two of which share an SM and overlap each
+// other's barriers.  Each block writes q for all of its elements; where the teacher has entries q - p is written over it, behind the next row's barrier.
 #pragma once
 #include "device_ops.cuh"
 
 namespace gn {
 
+// What the teacher's entries of a row come to: l as in Norm below, r the student's largest value where the teacher has probability (0 if it has none), d = sum of
+// p ((t - max t) - (s - r)); w: the row's weight, 0 where it has no entry of positive probability.
+struct alignas(16) Teacher { float l, d, r, w; };
 struct DistillParams {
   const void* logits; long stride; const void* ids; int index_type; const float* top_logits; const float* weight; float* loss; void* dlogits; long dstride;
   long rows, vocab; int top; float temperature;
+  Teacher* teach; int* id; float* prob; float* stud;                 // workspace: [rows], and [rows][top] each (the gradient's)
 };
 
 struct MaxSum { float m, s; };                                       // of values v: m >= all v (or -inf: none), s = sum of 2^((v - m) c)
@@ -37,9 +42,6 @@ __device__ __forceinline__ MaxSum warp_join(MaxSum v, float c) {
 struct Norm { float m, l; };
 __device__ __forceinline__ Norm norm_of(MaxSum v) { return Norm{v.m, log2f(v.s)}; }
 
-// What the teacher's entries of a row come to, formed by one warp: l as above, r the student's largest value where the teacher has probability (0 if it has none),
-// d = sum of p ((t - max t) - (s - r)).
-struct Teacher { float l, d, r; bool some; };
 constexpr int DISTILL_TOP = 1024;
 // id (-1: none) and logit of entry k
 __device__ __forceinline__ int teacher_entry(const DistillParams& p, long row, int k, float& t) {
@@ -49,114 +51,128 @@ __device__ __forceinline__ int teacher_entry(const DistillParams& p, long row, i
   t = there ? __ldg(p.top_logits + row * p.top + k) : -INFINITY;
   return there ? (int)id : -1;
 }
-// ids / probabilities / student values of the row's entries to `ids`, `prob`, `stud` (`keep`), and the loss's part (`loss`); one warp.
-template <class T>
-__device__ __forceinline__ Teacher teacher_row(const DistillParams& p, long row, const T* logits, float c, int lane, bool keep, int* ids, float* prob, float* stud, bool loss) {
-  MaxSum v{-INFINITY, 0.f};
-  for (int k = lane; k < p.top; k += 32) { float t; teacher_entry(p, row, k, t); v = join(v, MaxSum{t, t == -INFINITY ? 0.f : 1.f}, c); }
-  v = warp_join(v, c);
-  Teacher out{0.f, 0.f, 0.f, !(v.m == -INFINITY && v.s == 0.f)};
-  const Norm n = norm_of(v);
-  out.l = n.l;
-  float d = 0.f, r = -INFINITY;                                      // d: relative to this lane's r so far
-  float weight = 0.f;                                                // probability that it holds
-  for (int k = lane; k < p.top; k += 32) {
-    float t; const int id = teacher_entry(p, row, k, t);
-    const float pk = !out.some || t == -INFINITY ? 0.f : exp2f((t - n.m) * c - n.l);
-    const float s = id >= 0 && (loss || keep) ? to_f32(logits[id]) : 0.f;
-    if (pk != 0.f) {                                                 // (an entry without weight says nothing, whatever the student has there)
-      if (s > r) { if (weight != 0.f) d += weight * (s - r); r = s; }      // sum of p (r - s) moves with r
-      d += pk * ((t - n.m) - (s - (r == -INFINITY ? 0.f : r))); weight += pk;
+// A warp a row.  With a gradient the entries' ids, probabilities and student values are kept for the second launch; of entries with the same id the first keeps all of their
+// probability and the others become -1.  Such entries are rare and found by a table: every entry writes its number at its id's place, and whoever finds another's number there, or is found by
+// another of the same id, looks through the row.
+constexpr int TEACHER_WARPS = 4, TEACHER_TABLE = 2048;
+inline int teacher_smem(int top) { return TEACHER_WARPS * (TEACHER_TABLE * 2 + (top + 3) / 4 * 4 * 9); }      // table, ids, probabilities, flags
+template <class T, bool GRAD>
+__global__ void __launch_bounds__(32 * TEACHER_WARPS) distill_teacher_kernel(const __grid_constant__ DistillParams p) {
+  extern __shared__ uint4 teacher_smem_raw[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, top4 = (p.top + 3) & ~3; const float c = 1.4426950408889634f / p.temperature;
+  uint8_t* own = reinterpret_cast<uint8_t*>(teacher_smem_raw) + warp * (TEACHER_TABLE * 2 + top4 * 9);
+  int* id_of = reinterpret_cast<int*>(own); float* prob_of = reinterpret_cast<float*>(id_of + top4);
+  unsigned short* table = reinterpret_cast<unsigned short*>(prob_of + top4); uint8_t* look = reinterpret_cast<uint8_t*>(table + TEACHER_TABLE);
+  const long row = (long)blockIdx.x * TEACHER_WARPS + warp;
+  if (row >= p.rows) return;
+  const float w = p.weight ? __ldg(p.weight + row) : 1.f;
+  Teacher out{0.f, 0.f, 0.f, 0.f};
+  if (w != 0.f) {
+    const T* logits = static_cast<const T*>(p.logits) + row * p.stride;
+    MaxSum v{-INFINITY, 0.f};
+    for (int k = lane; k < p.top; k += 32) { float t; teacher_entry(p, row, k, t); v = join(v, MaxSum{t, t == -INFINITY ? 0.f : 1.f}, c); }
+    v = warp_join(v, c);
+    const bool some = !(v.m == -INFINITY && v.s == 0.f); const Norm n = norm_of(v);
+    float d = 0.f, r = -INFINITY, weight = 0.f;                      // d: relative to this lane's r so far; weight: the probability that it holds
+    for (int k = lane; k < p.top; k += 32) {
+      float t; const int id = teacher_entry(p, row, k, t);
+      const float pk = !some || t == -INFINITY ? 0.f : exp2f((t - n.m) * c - n.l), s = id >= 0 ? to_f32(logits[id]) : 0.f;
+      if (pk != 0.f) {                                               // (an entry without weight says nothing, whatever the student has there)
+        if (s > r) { if (weight != 0.f) d += weight * (s - r); r = s; }      // sum of p (r - s) moves with r
+        d += pk * ((t - n.m) - (s - (r == -INFINITY ? 0.f : r))); weight += pk;
+      }
+      if constexpr (GRAD) {
+        p.stud[row * p.top + k] = s; id_of[k] = id; prob_of[k] = pk; look[k] = 0;
+        if (id >= 0) table[id & (TEACHER_TABLE - 1)] = (unsigned short)k;
+      }
     }
-    if (keep) { ids[k] = id; prob[k] = pk; stud[k] = s; }
+    const float top = warp_max(r), ref = top == -INFINITY ? 0.f : top;
+    if (weight != 0.f) d += weight * (ref - (r == -INFINITY ? 0.f : r));
+    out = Teacher{n.l, warp_sum(d), ref, some ? w : 0.f};
+    if constexpr (GRAD) {
+      __syncwarp();
+      for (int k = lane; k < p.top; k += 32) {
+        const int id = id_of[k];
+        if (id < 0) continue;
+        const int found = table[id & (TEACHER_TABLE - 1)];
+        if (found != k) { look[k] = 1; if (id_of[found] == id) look[found] = 1; }
+      }
+      __syncwarp();
+      for (int k = lane; k < p.top; k += 32) {
+        int id = id_of[k]; float pk = prob_of[k];
+        if (look[k]) {
+          pk = 0.f;
+          for (int f = 0; f < p.top; f++) if (id_of[f] == id) { if (f < k) { id = -1; break; } pk += prob_of[f]; }
+        }
+        p.id[row * p.top + k] = id; p.prob[row * p.top + k] = pk;
+      }
+    }
   }
-  const float top = warp_max(r), ref = top == -INFINITY ? 0.f : top;
-  if (weight != 0.f) d += weight * (ref - (r == -INFINITY ? 0.f : r));
-  out.r = ref; out.d = warp_sum(d); return out;
+  if (lane == 0) p.teach[row] = out;
 }
 // w T^2 sum of p (log p - log q), from p = 2^((t - max t) c - l_t) and q = 2^((s - M) c - l), as the p add up to 1
-__device__ __forceinline__ float distill_loss(const Teacher& t, Norm n, float tau, float w, bool on) {
-  return on ? w * tau * (t.d + (n.m - t.r) + tau * 0.69314718055994531f * (n.l - t.l)) : 0.f;
+__device__ __forceinline__ float distill_loss(const Teacher& t, Norm n, float tau) { return t.w != 0.f ? t.w * tau * (t.d + (n.m - t.r) + tau * 0.69314718055994531f * (n.l - t.l)) : 0.f; }
+// q - p where the teacher has entries of row r, over what is there, for ids in [lo, hi)
+template <class T>
+__device__ __forceinline__ void distill_entries(const DistillParams& p, long r, float w, Norm n, float c, long lo, long hi) {
+  if (w == 0.f) return;
+  T* out = static_cast<T*>(p.dlogits) + r * p.dstride;
+  for (int e = threadIdx.x; e < p.top; e += blockDim.x) {
+    const int id = p.id[r * p.top + e];
+    if (id >= lo && id < hi && id >= 0) out[id] = from_f32<T>(w * p.temperature * (ex2((p.stud[r * p.top + e] - n.m) * c - n.l) - p.prob[r * p.top + e]));
+  }
 }
 
 // Elements of a row from the 16-byte boundary at or before its first one.
 template <class T> __device__ __forceinline__ int row_lead(const T* row) { return (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T)); }
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
 
-// NT threads of CL blocks on a row, BUF rows of slots.
+// NT threads of `cl` blocks on a row, `per` 16-byte pieces of it (counted from its 16-byte boundary) for each block; BUF rows of slots.
 template <class T, int NT, bool GRAD>
-__global__ void __launch_bounds__(NT, 1024 / NT) distill_kernel(const __grid_constant__ DistillParams p, int cl, int buffers) {
+__global__ void __launch_bounds__(NT, 1024 / NT) distill_kernel(const __grid_constant__ DistillParams p, int cl, int per) {
   namespace cg = cooperative_groups;
-  constexpr int V = Vec<T>::N, J = DISTILL_ITEMS / V, W = NT / 32;   // J accesses of 16 bytes a thread
-  extern __shared__ uint4 slots[];                                   // [buffers][J][NT], then per row in turn of three the entries' ids, probabilities and student values
-  __shared__ MaxSum part[2][W]; __shared__ MaxSum peers[2][8]; __shared__ Teacher teach[3];
-  __shared__ Norm norms[3];
-  // Rows take turns with what their barrier guards: two sets where it is read before the next row's barrier, three where behind it (a warp may be a row
-  // ahead of another, never two).
-  float* const kept = reinterpret_cast<float*>(slots + (long)buffers * J * NT);
-  auto ids = [&](int t) { return reinterpret_cast<int*>(kept + t * 3 * p.top); };
-  auto prob = [&](int t) { return kept + t * 3 * p.top + p.top; };
-  auto stud = [&](int t) { return kept + t * 3 * p.top + 2 * p.top; };
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  constexpr int V = Vec<T>::N, J = DISTILL_ITEMS / V, W = NT / 32, BUF = sizeof(T) == 2 ? 2 : 1;      // J pieces a thread; two rows under way where 16-bit elements leave room for them
+  extern __shared__ uint4 slots[];                                   // [BUF][J][NT]
+  __shared__ MaxSum part[2][W]; __shared__ MaxSum peers[2][8];       // (rows take turns: a warp may be a row ahead of another, never two)
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, vocab = (int)p.vocab;
   const int rank = cl > 1 ? (int)(blockIdx.x % cl) : 0; const long row0 = blockIdx.x / cl, step = gridDim.x / cl;
   const float c = 1.4426950408889634f / p.temperature;
   const uint32_t slot0 = (uint32_t)__cvta_generic_to_shared(slots) + tid * 16;
-  // pieces of a row: [0, n) from its 16-byte boundary on, of which this block has [at, at + own)
-  struct Cut { const T* row; int lead; long n, at, own; };
-  auto cut = [&](long r) {
-    Cut k; k.row = static_cast<const T*>(p.logits) + r * p.stride; k.lead = row_lead(k.row);
-    k.n = (k.lead + p.vocab + V - 1) / V; const long per = (k.n + cl - 1) / cl;
-    k.at = min(k.n, rank * per); k.own = min(k.n, k.at + per) - k.at; return k;
-  };
-  auto weight_of = [&](long r) { return p.weight ? __ldg(p.weight + r) : 1.f; };
+  const int at = rank * per;                                         // this block's pieces: [at, at + per), as far as the row goes
+  auto row_of = [&](long r) { return static_cast<const T*>(p.logits) + r * p.stride; };
+  auto weight_of = [&](long r) { return r < p.rows ? __ldg(&p.teach[r].w) : 0.f; };
   // copies of this thread's pieces of row r into buffer b; pieces that the row does not fill are put together element by element, -inf where it has none
-  auto fetch = [&](long r, int b) {
-    if (r < p.rows && weight_of(r) != 0.f) {
-      const Cut k = cut(r);
+  auto fetch = [&](long r, float w, int b) {
+    if (w != 0.f) {
+      const T* row = row_of(r); const int lead = row_lead(row);
 #pragma unroll
       for (int j = 0; j < J; j++) {
-        const long i = j * NT + tid;
-        if (i < k.own) {
-          const long e = (k.at + i) * V - k.lead;                    // first element
-          uint4* s = slots + (long)(b * J + j) * NT + tid;
-          if (e >= 0 && e + V <= p.vocab) cp16(slot0 + (b * J + j) * NT * 16, k.row + e);
+        const int i = j * NT + tid, e = (at + i) * V - lead;         // e: first element
+        if (i < per && e < vocab) {
+          if (e >= 0 && e + V <= vocab) cp16(slot0 + (b * J + j) * NT * 16, row + e);
           else {
-            T* q = reinterpret_cast<T*>(s);
+            T* q = reinterpret_cast<T*>(slots + (b * J + j) * NT + tid);
 #pragma unroll
-            for (int l = 0; l < V; l++) q[l] = e + l >= 0 && e + l < p.vocab ? k.row[e + l] : from_f32<T>(-INFINITY);
+            for (int l = 0; l < V; l++) q[l] = e + l >= 0 && e + l < vocab ? row[e + l] : from_f32<T>(-INFINITY);
           }
         }
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  // q - p where the teacher has entries of row r, over the q of this block's elements; equal ids: the first one writes for all
-  auto entries = [&](long r, int t) {
-    const float w = weight_of(r); const Norm n = norms[t];
-    if (w == 0.f || !teach[t].some) return;
-    const Cut k = cut(r); const long lo = k.at * V - k.lead, hi = lo + k.own * V;
-    T* out = static_cast<T*>(p.dlogits) + r * p.dstride; const int* id_of = ids(t); const float* prob_of = prob(t);
-    for (int e = tid; e < p.top; e += NT) {
-      const int id = id_of[e];
-      if (id < 0 || id < lo || id >= hi) continue;
-      float sum = 0.f; bool first = true;
-      for (int f = 0; f < p.top; f++) if (id_of[f] == id) { if (f < e) { first = false; break; } sum += prob_of[f]; }
-      if (first) out[id] = from_f32<T>(w * p.temperature * (ex2((stud(t)[e] - n.m) * c - n.l) - sum));
-    }
-  };
 
-  for (int b = 0; b < buffers; b++) fetch(row0 + b * step, b);
-  int b = 0, par = 0, turn = 0; long done = -1;
+  for (int b = 0; b < BUF; b++) fetch(row0 + b * step, weight_of(row0 + b * step), b);
+  float ahead = weight_of(row0 + BUF * step);                        // weight of the row that is fetched next
+  int b = 0, par = 0; long done = -1; float done_w = 0.f; Norm done_n{0.f, 0.f};
   for (long r = row0; r < p.rows; r += step) {
-    const Cut k = cut(r); const float w = weight_of(r); const bool live = w != 0.f;
-    if (buffers == 1) asm volatile("cp.async.wait_group 0;" ::: "memory");
-    else if (buffers == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
-    else asm volatile("cp.async.wait_group 2;" ::: "memory");
+    const T* row = row_of(r); const int lead = row_lead(row);
+    const Teacher t = p.teach[r]; const bool on = t.w != 0.f;
+    if constexpr (BUF == 1) asm volatile("cp.async.wait_group 0;" ::: "memory"); else asm volatile("cp.async.wait_group 1;" ::: "memory");
     float x[DISTILL_ITEMS]; float m = -INFINITY;
 #pragma unroll
     for (int j = 0; j < J; j++) {
-      float v[V];
-      if (live && j * NT + tid < k.own) unpack<T>(slots[(long)(b * J + j) * NT + tid], v);
+      float v[V]; const int i = j * NT + tid;
+      if (on && i < per && (at + i) * V - lead < vocab) unpack<T>(slots[(b * J + j) * NT + tid], v);
       else {
 #pragma unroll
         for (int l = 0; l < V; l++) v[l] = -INFINITY;
@@ -164,53 +180,53 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_kernel(const __grid_con
 #pragma unroll
       for (int l = 0; l < V; l++) { x[j * V + l] = v[l]; m = fmaxf(m, v[l]); }
     }
-    fetch(r + buffers * step, b);                                    // (the values have been read: m depends on them all)
-    if (warp == 0) {                                                 // the teacher's part, and the student's values there, before anything of the row is overwritten
-      Teacher t{};
-      if (live) t = teacher_row<T>(p, r, k.row, c, lane, GRAD, ids(turn), prob(turn), stud(turn), rank == 0);
-      if (lane == 0) teach[turn] = t;
-    }
+    fetch(r + BUF * step, ahead, b);                                 // (the values have been read: m depends on them all)
+    ahead = weight_of(r + (BUF + 1) * step);
+    m = warp_max(m);
     const float ref = m == -INFINITY ? 0.f : m;
     float s = 0.f;
 #pragma unroll
     for (int j = 0; j < DISTILL_ITEMS; j++) { x[j] = ex2((x[j] - ref) * c); s += x[j]; }
-    MaxSum v = warp_join(MaxSum{m, s}, c);
-    if (lane == 0) part[par][warp] = v;
+    s = warp_sum(s);
+    if (lane == 0) part[par][warp] = MaxSum{m, s};
     __syncthreads();
-    v = warp_join(lane < W ? part[par][lane] : MaxSum{-INFINITY, 0.f}, c);
+    auto meet = [&](MaxSum v) {
+      const float top = warp_max(v.m), to = top == -INFINITY ? 0.f : top;
+      return MaxSum{top, warp_sum(v.s * ex2((v.m - to) * c))};
+    };
+    MaxSum v = meet(lane < W ? part[par][lane] : MaxSum{-INFINITY, 0.f});
     if (cl > 1) {
       cg::cluster_group cluster = cg::this_cluster();
       if (tid < cl) *cluster.map_shared_rank(&peers[par][rank], tid) = v;
       cluster.sync();
-      v = warp_join(lane < cl ? peers[par][lane] : MaxSum{-INFINITY, 0.f}, c);
+      v = meet(lane < cl ? peers[par][lane] : MaxSum{-INFINITY, 0.f});
     }
-    const Norm n = norm_of(v); const Teacher t = teach[turn]; const bool on = live && t.some;
-    if (tid == 0) { norms[turn] = n; if (rank == 0) p.loss[r] = distill_loss(t, n, p.temperature, w, on); }
+    const Norm n = norm_of(v);
+    if (tid == 0 && rank == 0) p.loss[r] = distill_loss(t, n, p.temperature);
     if constexpr (GRAD) {
-      if (done >= 0) entries(done, turn == 0 ? 2 : turn - 1);
-      const float f = !on || (m == -INFINITY && n.m > -INFINITY) ? 0.f : w * p.temperature * ex2((m - n.m) * c - n.l);
-      T* out = static_cast<T*>(p.dlogits) + r * p.dstride; const bool same = row_lead(out) == k.lead;
+      const float f = !on || (m == -INFINITY && n.m > -INFINITY) ? 0.f : t.w * p.temperature * ex2((m - n.m) * c - n.l);
+      T* out = static_cast<T*>(p.dlogits) + r * p.dstride; const bool same = row_lead(out) == lead;
 #pragma unroll
       for (int j = 0; j < J; j++) {
-        const long i = j * NT + tid;
-        if (i >= k.own) continue;
-        const long e = (k.at + i) * V - k.lead;
+        const int i = j * NT + tid, e = (at + i) * V - lead;
+        if (i >= per || e >= vocab) continue;
         float y[V];
 #pragma unroll
         for (int l = 0; l < V; l++) y[l] = on ? x[j * V + l] * f : 0.f;
-        if (same && e >= 0 && e + V <= p.vocab) *reinterpret_cast<uint4*>(out + e) = pack<T>(y);
+        if (same && e >= 0 && e + V <= vocab) *reinterpret_cast<uint4*>(out + e) = pack<T>(y);
         else {
 #pragma unroll
-          for (int l = 0; l < V; l++) if (e + l >= 0 && e + l < p.vocab) out[e + l] = from_f32<T>(y[l]);
+          for (int l = 0; l < V; l++) if (e + l >= 0 && e + l < vocab) out[e + l] = from_f32<T>(y[l]);
         }
       }
-      done = r;
+      if (done >= 0) { const int l0 = row_lead(row_of(done)); distill_entries<T>(p, done, done_w, done_n, c, (long)at * V - l0, (long)(at + per) * V - l0); }
+      done = r; done_w = t.w; done_n = n;
     }
-    par ^= 1; if (++turn == 3) turn = 0; if (++b == buffers) b = 0;
+    par ^= 1; if (++b == BUF) b = 0;
   }
   if constexpr (GRAD) {
     __syncthreads();
-    if (done >= 0) entries(done, turn == 0 ? 2 : turn - 1);
+    if (done >= 0) { const int l0 = row_lead(row_of(done)); distill_entries<T>(p, done, done_w, done_n, c, (long)at * V - l0, (long)(at + per) * V - l0); }
   }
   if (cl > 1) cg::this_cluster().sync();                             // (no block leaves while another may still write into it)
 }
@@ -218,13 +234,12 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_kernel(const __grid_con
 // A row that does not fit on chip: one block reads it twice.
 template <class T, bool GRAD>
 __global__ void __launch_bounds__(1024) distill_long_kernel(const __grid_constant__ DistillParams p) {
-  __shared__ MaxSum part[32]; __shared__ Teacher teach;
-  __shared__ int ids[DISTILL_TOP]; __shared__ float prob[DISTILL_TOP], stud[DISTILL_TOP];
+  __shared__ MaxSum part[32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5; const float c = 1.4426950408889634f / p.temperature;
   for (long r = blockIdx.x; r < p.rows; r += gridDim.x) {
-    const T* row = static_cast<const T*>(p.logits) + r * p.stride; const float w = p.weight ? __ldg(p.weight + r) : 1.f; const bool live = w != 0.f;
+    const T* row = static_cast<const T*>(p.logits) + r * p.stride; const Teacher t = p.teach[r]; const bool on = t.w != 0.f;
     MaxSum v{-INFINITY, 0.f};
-    if (live) {
+    if (on)
       for (long e0 = tid; e0 < p.vocab; e0 += 8 * 1024) {
         float x[8]; float m = -INFINITY;
 #pragma unroll
@@ -234,25 +249,16 @@ __global__ void __launch_bounds__(1024) distill_long_kernel(const __grid_constan
         for (int j = 0; j < 8; j++) s += ex2((x[j] - ref) * c);
         v = join(v, MaxSum{m, s}, c);
       }
-      if (warp == 0) { const Teacher t = teacher_row<T>(p, r, row, c, lane, true, ids, prob, stud, true); if (lane == 0) teach = t; }
-    } else if (tid == 0) teach = Teacher{};
     v = warp_join(v, c);
     if (lane == 0) part[warp] = v;
     __syncthreads();
-    v = warp_join(part[lane], c);
-    const Norm n = norm_of(v); const Teacher t = teach; const bool on = live && t.some;
-    if (tid == 0) p.loss[r] = distill_loss(t, n, p.temperature, w, on);
+    const Norm n = norm_of(warp_join(part[lane], c));
+    if (tid == 0) p.loss[r] = distill_loss(t, n, p.temperature);
     if constexpr (GRAD) {
       T* out = static_cast<T*>(p.dlogits) + r * p.dstride;
-      for (long e = tid; e < p.vocab; e += 1024) out[e] = from_f32<T>(on ? w * p.temperature * ex2((to_f32(row[e]) - n.m) * c - n.l) : 0.f);
+      for (long e = tid; e < p.vocab; e += 1024) out[e] = from_f32<T>(on ? t.w * p.temperature * ex2((to_f32(row[e]) - n.m) * c - n.l) : 0.f);
       __syncthreads();
-      if (on)
-        for (int e = tid; e < p.top; e += 1024) {
-          const int id = ids[e]; if (id < 0) continue;
-          float sum = 0.f; bool first = true;
-          for (int f = 0; f < p.top; f++) if (ids[f] == id) { if (f < e) { first = false; break; } sum += prob[f]; }
-          if (first) out[id] = from_f32<T>(w * p.temperature * (ex2((stud[e] - n.m) * c - n.l) - sum));
-        }
+      distill_entries<T>(p, r, t.w, n, c, 0, p.vocab);
     }
     __syncthreads();
   }
@@ -261,22 +267,36 @@ __global__ void __launch_bounds__(1024) distill_long_kernel(const __grid_constan
 template <class T, bool GRAD>
 inline int distill_launch(gn_ctx* ctx, const DistillParams& p, void* stream) {
   const int sms = ctx->c.sm_count; const DistillPlan pl = distill_plan(p.rows, p.vocab, sms);
+  const int tsmem = teacher_smem(GRAD ? p.top : 0);
+  if (tsmem > 48 * 1024) GN_TRY(op_smem("distill_teacher", distill_teacher_kernel<T, GRAD>, tsmem));
+  GN_TRY(op_launch("distill_teacher", stream, distill_teacher_kernel<T, GRAD>, dim3(cdiv(p.rows, TEACHER_WARPS)), dim3(32 * TEACHER_WARPS), tsmem, 0, p));
   if (pl.cluster == 0) return op_launch("distill_long", stream, distill_long_kernel<T, GRAD>, dim3((unsigned)std::min<int64_t>(p.rows, 2L * sms)), dim3(1024), 0, 0, p);
-  // two rows of slots where 16-bit elements leave room for them: 128 KB for 1024 threads either way
-  const int buffers = sizeof(T) == 2 ? 2 : 1, smem = buffers * pl.threads * DISTILL_ITEMS * (int)sizeof(T) + (GRAD ? 3 * 12 * p.top : 0);
-  const int64_t per_sm = std::max<int64_t>(1, std::min<int64_t>(1024 / pl.threads, 220 * 1024 / (smem + 2048)));
-  const dim3 grid((unsigned)(std::min<int64_t>(p.rows, std::max<int64_t>(1, sms * per_sm / pl.cluster)) * pl.cluster));
-  auto go = [&](auto kernel) { GN_TRY(op_smem("distill", kernel, smem)); return op_launch("distill", stream, kernel, grid, dim3(pl.threads), smem, pl.cluster, p, pl.cluster, buffers); };
+  const int V = 16 / (int)sizeof(T), smem = (sizeof(T) == 2 ? 2 : 1) * pl.threads * DISTILL_ITEMS * (int)sizeof(T);      // 64 KB for 512 threads
+  const int per = (int)ceil_div(ceil_div(p.vocab + V - 1, V), pl.cluster);
+  const dim3 grid((unsigned)(std::min<int64_t>(p.rows, std::max<int64_t>(1, (int64_t)sms * (1024 / pl.threads) / pl.cluster)) * pl.cluster));
+  auto go = [&](auto kernel) { if (smem > 48 * 1024) GN_TRY(op_smem("distill", kernel, smem)); return op_launch("distill", stream, kernel, grid, dim3(pl.threads), smem, pl.cluster, p, pl.cluster, per); };
   return pl.threads == 1024 ? go(distill_kernel<T, 1024, GRAD>) : pl.threads == 512 ? go(distill_kernel<T, 512, GRAD>) : pl.threads == 256 ? go(distill_kernel<T, 256, GRAD>) : go(distill_kernel<T, 64, GRAD>);
 }
 
 }  // namespace gn
 
-extern "C" int gn_op_distill(gn_ctx* ctx, int dtype, int64_t rows, int64_t vocab, int top, float temperature, const void* logits, int64_t row_stride, const void* top_ids, int index_type, const float* top_logits,
-                             const float* weight, float* loss, void* dlogits, int64_t drow_stride, void* stream) {
+extern "C" {
+
+int gn_op_distill_workspace(gn_ctx* ctx, int64_t rows, int top, int gradient, int64_t* bytes) {
+  using namespace gn;
+  if (!ctx || !ctx->alive || !bytes || rows < 0 || rows > OP_MAX_ROWS || top < 0 || top > DISTILL_TOP) return fail(GN_ERR_INVALID_ARG, "op_distill_workspace: bad argument");
+  *bytes = distill_workspace(rows, top, gradient != 0); return GN_OK;
+}
+
+int gn_op_distill(gn_ctx* ctx, int dtype, int64_t rows, int64_t vocab, int top, float temperature, const void* logits, int64_t row_stride, const void* top_ids, int index_type, const float* top_logits,
+                  const float* weight, float* loss, void* dlogits, int64_t drow_stride, void* workspace, int64_t workspace_bytes, void* stream) {
   using namespace gn;
   GN_OP_BEGIN("op_distill", check_distill(dtype, rows, vocab, top, temperature, logits, row_stride, top_ids, index_type, top_logits, weight, loss, dlogits, drow_stride));
   if (rows == 0) return GN_OK;
-  const DistillParams p{logits, (long)row_stride, top_ids, index_type, top_logits, weight, loss, dlogits, (long)drow_stride, (long)rows, (long)vocab, top, temperature};
+  if (!workspace || !aligned_to(workspace, 16) || workspace_bytes < distill_workspace(rows, top, dlogits != nullptr)) return fail(GN_ERR_INVALID_ARG, "op_distill: the workspace is too small, null or not aligned");
+  Teacher* teach = static_cast<Teacher*>(workspace); int* id = reinterpret_cast<int*>(teach + rows); float* prob = reinterpret_cast<float*>(id + rows * top);
+  const DistillParams p{logits, (long)row_stride, top_ids, index_type, top_logits, weight, loss, dlogits, (long)drow_stride, (long)rows, (long)vocab, top, temperature, teach, id, prob, prob + rows * top};
   return with_type(dtype, [&](auto t) { using T = decltype(t); return dlogits ? distill_launch<T, true>(ctx, p, stream) : distill_launch<T, false>(ctx, p, stream); });
 }
+
+}  // extern "C"

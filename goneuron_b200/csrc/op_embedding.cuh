@@ -264,29 +264,50 @@ __global__ void __launch_bounds__(EMB_THREADS) embedding_sum_kernel(const T* __r
   }
 }
 // A run that goes on over the end of the piece where it began: that piece's last sum, then the first sums of the pieces behind it up to the one where the run ends.
-// Eight threads a column, each a run of neighbouring pieces, added in order.
-__global__ void __launch_bounds__(256) embedding_join_kernel(const unsigned* __restrict__ keys, long tokens, long vocab, int dim, int chunk, long chunks, const float* __restrict__ partial, float* __restrict__ dtable) {
-  __shared__ float red[8][32];
+// Most blocks find no such run and leave after three independent loads.  (Looking the run's end up by bisection, and 32 columns of a block at a time: 127 us of a gradient over
+// 131072 tokens whose other launches take 100.)  Four threads a column, each a run of neighbouring pieces, added in order; V columns of a thread.
+constexpr int JOIN_COLS = 64;
+template <int V>
+__global__ void __launch_bounds__(4 * JOIN_COLS) embedding_join_kernel(const unsigned* __restrict__ keys, long tokens, long vocab, int dim, int chunk, long chunks, const float* __restrict__ partial, float* __restrict__ dtable) {
+  __shared__ float red[3][JOIN_COLS * V];
+  __shared__ int found;
   const long c = blockIdx.x, end = (c + 1) * chunk;                  // (a last piece has nothing behind it: the launch leaves it out)
-  const unsigned key = __ldg(keys + end - 1);
-  if (key >= (unsigned)vocab || __ldg(keys + end) != key) return;
-  if (c > 0 && __ldg(keys + c * chunk) == key && __ldg(keys + c * chunk - 1) == key) return;      // it began before
-  const long stop = first_place(keys, tokens, key + 1), m = (stop - 1) / chunk - c;      // pieces behind this one with a part of it
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5; const long per = (m + 7) / 8;
-  for (long col0 = (long)blockIdx.y * 32; col0 < dim; col0 += (long)gridDim.y * 32) {
-    const long col = col0 + lane; float v = 0.f;
-    if (col < dim) {
-      if (w == 0) v = __ldg(partial + (2 * c + 1) * dim + col);
-#pragma unroll 4
-      for (long i = w * per; i < min(m, (w + 1) * per); i++) v += __ldg(partial + 2 * (c + 1 + i) * dim + col);
-    }
+  const unsigned key = __ldg(keys + end - 1), next = __ldg(keys + end), begin = __ldg(keys + c * chunk), before = c > 0 ? __ldg(keys + c * chunk - 1) : 0xffffffffu;
+  if (key >= (unsigned)vocab || next != key || (begin == key && before == key)) return;      // no row, no run over the end, or one that began before
+  long m = 1;                                                        // pieces behind this one that begin within the run
+  for (long i0 = c + 1;; i0 += blockDim.x) {
+    if (threadIdx.x == 0) found = 0x7fffffff;
     __syncthreads();
-    red[w][lane] = v;
+    const long i = i0 + threadIdx.x;
+    if (i >= chunks || __ldg(keys + i * chunk) != key) atomicMin(&found, (int)threadIdx.x);
     __syncthreads();
-    if (w == 0 && col < dim) {
-      for (int i = 1; i < 8; i++) v += red[i][lane];
-      dtable[(long)key * dim + col] = v;
-    }
+    const int f = found;
+    __syncthreads();
+    if (f != 0x7fffffff) { m = i0 + f - c - 1; break; }
+  }
+  const int w = threadIdx.x / JOIN_COLS, lane = threadIdx.x % JOIN_COLS; const long per = (m + 3) / 4, col = ((long)blockIdx.y * JOIN_COLS + lane) * V; const bool in = col < dim;
+  float v[V];
+#pragma unroll
+  for (int j = 0; j < V; j++) v[j] = 0.f;
+  auto add = [&](const float* row) {
+    if constexpr (V == 1) v[0] += __ldg(row + col);
+    else { const float4 u = __ldg(reinterpret_cast<const float4*>(row + col)); v[0] += u.x; v[1] += u.y; v[2] += u.z; v[3] += u.w; }
+  };
+  if (in) {
+    if (w == 0) add(partial + (2 * c + 1) * dim);
+#pragma unroll 8
+    for (long i = w * per; i < min(m, (w + 1) * per); i++) add(partial + 2 * (c + 1 + i) * dim);
+  }
+  if (w > 0) {
+#pragma unroll
+    for (int j = 0; j < V; j++) red[w - 1][lane * V + j] = v[j];
+  }
+  __syncthreads();
+  if (w == 0 && in) {
+    float* out = dtable + (long)key * dim + col;
+#pragma unroll
+    for (int j = 0; j < V; j++) { for (int i = 0; i < 3; i++) v[j] += red[i][lane * V + j]; }
+    if constexpr (V == 1) *out = v[0]; else *reinterpret_cast<float4*>(out) = make_float4(v[0], v[1], v[2], v[3]);
   }
 }
 
@@ -297,11 +318,13 @@ inline int embedding_sums(const EmbeddingPlan& pl, const void* dout, long stride
   constexpr int N = Vec<T>::N;
   const bool vec = dim % N == 0 && stride % N == 0 && aligned_to(dout, 16) && aligned_to(dtable, 16);
   const dim3 grid((unsigned)(pl.chunks + ceil_div(vocab, EMB_ZERO_ROWS)), (unsigned)ceil_div(dim, EMB_THREADS * (vec ? N : 1)));
-  if (grid.y > 65535) return fail(GN_ERR_UNSUPPORTED, "op_embedding_backward: dim is too large");
+  if (ceil_div(dim, JOIN_COLS) > 65535) return fail(GN_ERR_UNSUPPORTED, "op_embedding_backward: dim is too large");
   if (vec) GN_TRY(op_launch("embedding_sum", stream, embedding_sum_kernel<T, N>, grid, dim3(EMB_THREADS), 0, 0, static_cast<const T*>(dout), stride, keys, order, tokens, vocab, dim, scale, pl.chunk, (long)pl.chunks, dtable, partial));
   else GN_TRY(op_launch("embedding_sum", stream, embedding_sum_kernel<T, 1>, grid, dim3(EMB_THREADS), 0, 0, static_cast<const T*>(dout), stride, keys, order, tokens, vocab, dim, scale, pl.chunk, (long)pl.chunks, dtable, partial));
   if (pl.chunks < 2) return GN_OK;
-  return op_launch("embedding_join", stream, embedding_join_kernel, dim3((unsigned)(pl.chunks - 1), (unsigned)std::min<int64_t>(8, ceil_div(dim, 32))), dim3(256), 0, 0, keys, tokens, vocab, dim, pl.chunk, (long)pl.chunks, partial, dtable);
+  const bool vec4 = dim % 4 == 0 && aligned_to(dtable, 16);
+  const dim3 join((unsigned)(pl.chunks - 1), (unsigned)ceil_div(dim, JOIN_COLS * (vec4 ? 4 : 1)));
+  return op_launch("embedding_join", stream, vec4 ? embedding_join_kernel<4> : embedding_join_kernel<1>, join, dim3(4 * JOIN_COLS), 0, 0, keys, tokens, vocab, dim, pl.chunk, (long)pl.chunks, (const float*)partial, dtable);
 }
 
 }  // namespace gn

@@ -13,9 +13,9 @@
 
 namespace gn {
 
-struct QkHeads { const void* in; const void* dy; void* out; long in_t, in_h, dy_t, dy_h, out_t, out_h; int heads; const float* gain; };
+struct QkHeads { const void* in; const void* dy; void* out; long in_t, in_h, dy_t, dy_h, out_t, out_h; int heads, per_block; const float* gain; };      // per_block: tokens of a block at a time
 struct QkParams {
-  QkHeads t[2]; long tokens; int head, rot, inter, per_block; float eps; const void* pos; int index_type; const double* freq; float* partial;
+  QkHeads t[2]; long tokens; int head, rot, inter; float eps; const void* pos; int index_type; const double* freq; float* partial;
 };
 
 // cosine and sine of the angle of (token, pair)
@@ -25,126 +25,169 @@ __device__ __forceinline__ float2 qk_turn(const QkParams& p, long token, int pai
   float s, c; sincospif(2.f * (float)turns, &s, &c);
   return make_float2(c, s);
 }
-__device__ __forceinline__ void qk_turns(const QkParams& p, long base, int n, float2* cs) {
+// ... of n tokens from `base` on: per token the cosines of all pairs, then the sines
+__device__ __forceinline__ void qk_turns(const QkParams& p, long base, int n, float* cs) {
   const int half = p.rot >> 1;
-  for (int e = threadIdx.x; e < n * half; e += blockDim.x) { const int t = e / half; cs[e] = qk_turn(p, base + t, e - t * half); }
+  for (int e = threadIdx.x; e < n * half; e += blockDim.x) { const int t = e / half, i = e - t * half; const float2 v = qk_turn(p, base + t, i); cs[t * p.rot + i] = v.x; cs[t * p.rot + half + i] = v.y; }
 }
-// sign -1: R^T
-__device__ __forceinline__ void rotate(float& a, float& b, float2 cs, float sign) { const float sn = sign * cs.y, u = a * cs.x - b * sn; b = a * sn + b * cs.x; a = u; }
-// a lane's two pieces: whole halves of pairs (`split`), or neighbouring elements as pairs
-template <int V>
-__device__ __forceinline__ void qk_turn_pieces(const QkParams& p, float (&x)[V], float (&y)[V], const float2* cs, bool split, int s, int pa, int pb, float sign) {
-  if (split) {
+__device__ __forceinline__ void rotate(float& a, float& b, float c, float s) { const float u = a * c - b * s; b = a * s + b * c; a = u; }
+
+// A lane's two pieces of a row: the halves of its pairs, or two neighbours behind the rotated part (interleaved: two neighbours everywhere), with the cosines and sines of
+// their pairs and the gain of their elements.  The same for all heads of a token, so that they stay in registers while a lane goes through QkTile::HB of them.
+template <class T> struct QkLane {
+  static constexpr int V = Vec<T>::N;
+  int pa, pb; bool has_a, has_b, split;
+  float ga[V], gb[V], c[V], s[V];
+  __device__ __forceinline__ QkLane(const QkParams& p, int slot) {
+    const int pieces = p.head / V, turned = (p.rot >> 1) / V;
+    split = !p.inter && slot < turned;
+    pa = split ? slot : 2 * slot; pb = split ? slot + turned : 2 * slot + 1;
+    has_a = pa < pieces; has_b = pb < pieces;
+  }
+  __device__ __forceinline__ void gain(const float* g) {
 #pragma unroll
-    for (int j = 0; j < V; j++) rotate(x[j], y[j], cs[s * V + j], sign);
-  } else if (p.inter) {
+    for (int j = 0; j < V; j++) { ga[j] = g && has_a ? __ldg(g + pa * V + j) : 1.f; gb[j] = g && has_b ? __ldg(g + pb * V + j) : 1.f; }
+  }
+  __device__ __forceinline__ void turns(const QkParams& p, const float* cs, float sign) {      // cs: the token's
+    const int half = p.rot >> 1;
+    if (split) {
 #pragma unroll
-    for (int j = 0; j < V; j += 2) {
-      if (pa * V + j < p.rot) rotate(x[j], x[j + 1], cs[(pa * V + j) >> 1], sign);
-      if (pb * V + j < p.rot) rotate(y[j], y[j + 1], cs[(pb * V + j) >> 1], sign);
+      for (int j = 0; j < V; j += 4) {
+        const float4 u = *reinterpret_cast<const float4*>(cs + pa * V + j), w = *reinterpret_cast<const float4*>(cs + half + pa * V + j);
+        c[j] = u.x; c[j + 1] = u.y; c[j + 2] = u.z; c[j + 3] = u.w; s[j] = sign * w.x; s[j + 1] = sign * w.y; s[j + 2] = sign * w.z; s[j + 3] = sign * w.w;
+      }
+    } else if (p.inter) {
+#pragma unroll
+      for (int j = 0; j < V; j++) { const int i = (j < V / 2 ? pa : pb) * (V / 2) + j % (V / 2); c[j] = i < half ? cs[i] : 1.f; s[j] = i < half ? sign * cs[half + i] : 0.f; }
     }
   }
-}
+  __device__ __forceinline__ void turn(const QkParams& p, float (&a)[V], float (&b)[V]) const {
+    if (split) {
+#pragma unroll
+      for (int j = 0; j < V; j++) rotate(a[j], b[j], c[j], s[j]);
+    } else if (p.inter) {                                            // (elements that do not turn are left alone: 0 times an infinity is none)
+#pragma unroll
+      for (int j = 0; j < V / 2; j++) {
+        if (pa * V + 2 * j < p.rot) rotate(a[2 * j], a[2 * j + 1], c[j], s[j]);
+        if (pb * V + 2 * j < p.rot) rotate(b[2 * j], b[2 * j + 1], c[V / 2 + j], s[V / 2 + j]);
+      }
+    }
+  }
+  __device__ __forceinline__ void load(const void* row, uint4& a, uint4& b) const {
+    a = make_uint4(0, 0, 0, 0); b = a;
+    if (has_a) a = reinterpret_cast<const uint4*>(row)[pa];
+    if (has_b) b = reinterpret_cast<const uint4*>(row)[pb];
+  }
+  __device__ __forceinline__ void store(void* row, const float (&a)[V], const float (&b)[V]) const {
+    if (has_a) reinterpret_cast<uint4*>(row)[pa] = pack<T>(a);
+    if (has_b) reinterpret_cast<uint4*>(row)[pb] = pack<T>(b);
+  }
+};
 
 constexpr int QK_THREADS = 256;
+// A group of G lanes takes HB heads of one token at a time.  Forward: four, eight 16-byte loads of a lane under way; backward two, x and dy.  (One head at a time, with the cosines read from
+// shared memory for each: 129 us forward and 236 backward for 65536 tokens of 16 + 4 heads of 64, bf16; bound by instructions, 14 an element.)
 template <class T, int G, bool BWD>
-__global__ void __launch_bounds__(QK_THREADS, BWD ? QK_PER_SM : 4) qk_vec_kernel(const __grid_constant__ QkParams p) {
-  constexpr int V = Vec<T>::N, ROWS = QK_THREADS / G;
+__global__ void __launch_bounds__(QK_THREADS, QK_PER_SM) qk_vec_kernel(const __grid_constant__ QkParams p) {
+  constexpr int V = Vec<T>::N, GROUPS = QK_THREADS / G, HB = BWD ? QK_HEADS_BWD : QK_HEADS_FWD;
   extern __shared__ float4 qk_smem[];
-  float2* cs = reinterpret_cast<float2*>(qk_smem);
+  float* cs = reinterpret_cast<float*>(qk_smem);
   __shared__ float red[BWD ? QK_THREADS / 32 * G * 2 * V : 1];
-  const int s = threadIdx.x % G, g0 = threadIdx.x / G, half = p.rot >> 1, pieces = p.head / V, turned = half / V;
-  // this lane's two pieces: the halves of its pairs, or two neighbours behind the rotated part (interleaved: two neighbours everywhere)
-  const int pa = p.inter ? 2 * s : s < turned ? s : 2 * s, pb = p.inter || s >= turned ? pa + 1 : s + turned;
-  const bool has_a = pa < pieces, has_b = pb < pieces, split = !p.inter && s < turned;
-#pragma unroll 1
-  for (int kind = 0; kind < 2; kind++) {
-    const QkHeads& h = p.t[kind];
-    if (h.heads == 0) continue;
-    float ga[V], gb[V], acc[BWD ? 2 * V : 1];
-#pragma unroll
-    for (int j = 0; j < V; j++) { ga[j] = h.gain && has_a ? __ldg(h.gain + pa * V + j) : 1.f; gb[j] = h.gain && has_b ? __ldg(h.gain + pb * V + j) : 1.f; }
+  const int slot = threadIdx.x % G, g0 = threadIdx.x / G;
+  QkLane<T> lane(p, slot);
+  const int kind = blockIdx.y; const QkHeads& h = p.t[kind];
+  if (h.heads == 0) return;
+  {
+    const int per_token = (h.heads + HB - 1) / HB;
+    lane.gain(h.gain);
+    float acc[BWD ? 2 * V : 1];
     if constexpr (BWD) {
 #pragma unroll
       for (int j = 0; j < 2 * V; j++) acc[j] = 0.f;
     }
-    for (long base = (long)blockIdx.x * p.per_block; base < p.tokens; base += (long)gridDim.x * p.per_block) {
-      const int n = (int)min((long)p.per_block, p.tokens - base), rows = n * h.heads;
-      __syncthreads();
-      qk_turns(p, base, n, cs);
-      __syncthreads();
-      for (int r0 = 0; r0 < rows; r0 += ROWS) {                      // (the same count for a whole block: the shuffles below want whole warps)
-        const int r = r0 + g0; const bool on = r < rows;
-        const int t = on ? r / h.heads : 0, hd = r - t * h.heads;
+    for (long base = (long)blockIdx.x * h.per_block; base < p.tokens; base += (long)gridDim.x * h.per_block) {
+      const int n = (int)min((long)h.per_block, p.tokens - base), items = n * per_token;
+      for (int i0 = 0; i0 < items; i0 += GROUPS) {                   // (the same count for a whole block: barriers and shuffles want all of it)
+        const int i = i0 + g0; const bool on = i < items;
+        const int t = on ? i / per_token : 0, h0 = on ? (i - t * per_token) * HB : 0, heads = on ? min(HB, h.heads - h0) : 0;
         const long tok = base + t;
-        uint4 ua = make_uint4(0, 0, 0, 0), ub = ua, wa = ua, wb = ua;
-        if (on) {
-          const uint4* x = reinterpret_cast<const uint4*>(static_cast<const T*>(h.in) + tok * h.in_t + hd * h.in_h);
-          if (has_a) ua = x[pa];
-          if (has_b) ub = x[pb];
-          if constexpr (BWD) {
-            const uint4* d = reinterpret_cast<const uint4*>(static_cast<const T*>(h.dy) + tok * h.dy_t + hd * h.dy_h);
-            if (has_a) wa = d[pa];
-            if (has_b) wb = d[pb];
+        const T* x = static_cast<const T*>(h.in) + tok * h.in_t + h0 * h.in_h;
+        uint4 ua[HB], ub[HB], wa[BWD ? HB : 1], wb[BWD ? HB : 1];
+#pragma unroll
+        for (int q = 0; q < HB; q++) {
+          ua[q] = ub[q] = make_uint4(0, 0, 0, 0);
+          if (q < heads) lane.load(x + q * h.in_h, ua[q], ub[q]);
+        }
+        if constexpr (BWD) {
+          const T* d = static_cast<const T*>(h.dy) + tok * h.dy_t + h0 * h.dy_h;
+#pragma unroll
+          for (int q = 0; q < HB; q++) {
+            wa[q] = wb[q] = make_uint4(0, 0, 0, 0);
+            if (q < heads) lane.load(d + q * h.dy_h, wa[q], wb[q]);
           }
         }
-        float a[V], b[V]; unpack<T>(ua, a); unpack<T>(ub, b);
-        float ss = 0.f;
-#pragma unroll
-        for (int j = 0; j < V; j++) ss += a[j] * a[j] + b[j] * b[j];
-        const float2* c = cs + t * half;
-        float ya[V], yb[V];
-        if constexpr (!BWD) {
-#pragma unroll
-          for (int o = G / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-          const float rs = rsqrtf(ss / p.head + p.eps);
-#pragma unroll
-          for (int j = 0; j < V; j++) { ya[j] = a[j] * rs * ga[j]; yb[j] = b[j] * rs * gb[j]; }
-          qk_turn_pieces<V>(p, ya, yb, c, split, s, pa, pb, 1.f);
-        } else {
-          unpack<T>(wa, ya); unpack<T>(wb, yb);
-          qk_turn_pieces<V>(p, ya, yb, c, split, s, pa, pb, -1.f);
-          float sx = 0.f;
-#pragma unroll
-          for (int j = 0; j < V; j++) sx += ya[j] * ga[j] * a[j] + yb[j] * gb[j] * b[j];
-#pragma unroll
-          for (int o = G / 2; o > 0; o >>= 1) { ss += __shfl_xor_sync(0xffffffffu, ss, o); sx += __shfl_xor_sync(0xffffffffu, sx, o); }
-          const float rs = rsqrtf(ss / p.head + p.eps), m = rs * rs * (sx / p.head);
-#pragma unroll
-          for (int j = 0; j < V; j++) {
-            acc[j] += ya[j] * (a[j] * rs); acc[V + j] += yb[j] * (b[j] * rs);      // (rows that are not there have zeros)
-            ya[j] = rs * (ya[j] * ga[j] - a[j] * m); yb[j] = rs * (yb[j] * gb[j] - b[j] * m);
-          }
+        if (i0 == 0) {                                               // under the loads
+          __syncthreads();
+          qk_turns(p, base, n, cs);
+          __syncthreads();
         }
-        if (on) {
-          uint4* o = reinterpret_cast<uint4*>(static_cast<T*>(h.out) + tok * h.out_t + hd * h.out_h);
-          if (has_a) o[pa] = pack<T>(ya);
-          if (has_b) o[pb] = pack<T>(yb);
+        lane.turns(p, cs + t * p.rot, BWD ? -1.f : 1.f);
+        T* o = static_cast<T*>(h.out) + tok * h.out_t + h0 * h.out_h;
+#pragma unroll
+        for (int q = 0; q < HB; q++) {
+          float a[V], b[V]; unpack<T>(ua[q], a); unpack<T>(ub[q], b);
+          float ss = 0.f;
+#pragma unroll
+          for (int j = 0; j < V; j++) { ss = fmaf(a[j], a[j], ss); ss = fmaf(b[j], b[j], ss); }
+          if constexpr (!BWD) {
+#pragma unroll
+            for (int m = G / 2; m > 0; m >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
+            const float rs = rsqrtf(ss / p.head + p.eps);
+#pragma unroll
+            for (int j = 0; j < V; j++) { a[j] *= lane.ga[j]; b[j] *= lane.gb[j]; }
+            lane.turn(p, a, b);
+#pragma unroll
+            for (int j = 0; j < V; j++) { a[j] *= rs; b[j] *= rs; }
+            if (q < heads) lane.store(o + q * h.out_h, a, b);
+          } else {
+            float ya[V], yb[V]; unpack<T>(wa[q], ya); unpack<T>(wb[q], yb);
+            lane.turn(p, ya, yb);
+            float sx = 0.f;
+#pragma unroll
+            for (int j = 0; j < V; j++) { sx = fmaf(ya[j] * lane.ga[j], a[j], sx); sx = fmaf(yb[j] * lane.gb[j], b[j], sx); }
+#pragma unroll
+            for (int m = G / 2; m > 0; m >>= 1) { ss += __shfl_xor_sync(0xffffffffu, ss, m); sx += __shfl_xor_sync(0xffffffffu, sx, m); }
+            const float rs = rsqrtf(ss / p.head + p.eps), m = rs * rs * (sx / p.head);
+#pragma unroll
+            for (int j = 0; j < V; j++) {
+              acc[j] = fmaf(ya[j], a[j] * rs, acc[j]); acc[V + j] = fmaf(yb[j], b[j] * rs, acc[V + j]);      // (rows that are not there have zeros)
+              ya[j] = rs * fmaf(-a[j], m, ya[j] * lane.ga[j]); yb[j] = rs * fmaf(-b[j], m, yb[j] * lane.gb[j]);
+            }
+            if (q < heads) lane.store(o + q * h.out_h, ya, yb);
+          }
         }
       }
     }
     if constexpr (BWD) {
-      if (!p.partial) continue;
+      if (!p.partial) return;
 #pragma unroll
-      for (int o = 16; o >= G; o >>= 1) {
+      for (int m = 16; m >= G; m >>= 1) {
 #pragma unroll
-        for (int j = 0; j < 2 * V; j++) acc[j] += __shfl_xor_sync(0xffffffffu, acc[j], o);
+        for (int j = 0; j < 2 * V; j++) acc[j] += __shfl_xor_sync(0xffffffffu, acc[j], m);
       }
       const int warp = threadIdx.x >> 5;
       __syncthreads();
       if ((threadIdx.x & 31) < G) {
 #pragma unroll
-        for (int j = 0; j < 2 * V; j++) red[(warp * G + s) * 2 * V + j] = acc[j];
+        for (int j = 0; j < 2 * V; j++) red[(warp * G + slot) * 2 * V + j] = acc[j];
       }
       __syncthreads();
       float* out = p.partial + ((long)blockIdx.x * 2 + kind) * p.head;
       for (int e = threadIdx.x; e < G * 2 * V; e += QK_THREADS) {
-        const int ls = e / (2 * V), j = e % (2 * V);                 // lane, its element
-        const int qa = p.inter ? 2 * ls : ls < turned ? ls : 2 * ls, qb = p.inter || ls >= turned ? qa + 1 : ls + turned;
-        const int piece = j < V ? qa : qb;
+        const int j = e % (2 * V); const QkLane<T> of(p, e / (2 * V)); const int piece = j < V ? of.pa : of.pb;
         float v = 0.f;
         for (int w = 0; w < QK_THREADS / 32; w++) v += red[w * G * 2 * V + e];
-        if (piece < pieces) out[piece * V + j % V] = v;
+        if (piece * V < p.head) out[piece * V + j % V] = v;
       }
     }
   }
@@ -155,12 +198,12 @@ constexpr int QK_ROW_WARPS = 4;
 template <class T, bool BWD>
 __global__ void __launch_bounds__(32 * QK_ROW_WARPS) qk_rows_kernel(const __grid_constant__ QkParams p) {
   extern __shared__ float4 qk_smem[];
-  float2* cs = reinterpret_cast<float2*>(qk_smem);
+  float* cs = reinterpret_cast<float*>(qk_smem);
   const int half = p.rot >> 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  float* acc = reinterpret_cast<float*>(cs + p.per_block * half) + warp * p.head;      // this warp's share of the gain's gradient; an element belongs to one lane
-  for (int kind = 0; kind < 2; kind++) {
-    const QkHeads& h = p.t[kind];
-    if (h.heads == 0) continue;
+  const int kind = blockIdx.y; const QkHeads& h = p.t[kind];
+  if (h.heads == 0) return;
+  float* acc = cs + h.per_block * p.rot + warp * p.head;             // this warp's share of the gain's gradient; an element belongs to one lane
+  {
     auto first = [&](int i) { return p.inter ? 2 * i : i; };
     auto second = [&](int i) { return p.inter ? 2 * i + 1 : i + half; };
     auto gain = [&](int e) { return h.gain ? __ldg(h.gain + e) : 1.f; };
@@ -168,8 +211,8 @@ __global__ void __launch_bounds__(32 * QK_ROW_WARPS) qk_rows_kernel(const __grid
       __syncthreads();
       for (int e = threadIdx.x; e < QK_ROW_WARPS * p.head; e += blockDim.x) acc[e - warp * p.head] = 0.f;
     }
-    for (long base = (long)blockIdx.x * p.per_block; base < p.tokens; base += (long)gridDim.x * p.per_block) {
-      const int n = (int)min((long)p.per_block, p.tokens - base), rows = n * h.heads;
+    for (long base = (long)blockIdx.x * h.per_block; base < p.tokens; base += (long)gridDim.x * h.per_block) {
+      const int n = (int)min((long)h.per_block, p.tokens - base), rows = n * h.heads;
       __syncthreads();
       qk_turns(p, base, n, cs);
       __syncthreads();
@@ -177,7 +220,7 @@ __global__ void __launch_bounds__(32 * QK_ROW_WARPS) qk_rows_kernel(const __grid
         const int t = r / h.heads, hd = r - t * h.heads;
         const T* x = static_cast<const T*>(h.in) + (base + t) * h.in_t + hd * h.in_h;
         T* o = static_cast<T*>(h.out) + (base + t) * h.out_t + hd * h.out_h;
-        const float2* c = cs + t * half;
+        const float *c = cs + t * p.rot, *s = c + half;
         float ss = 0.f;
         for (int e = lane; e < p.head; e += 32) { const float v = to_f32(x[e]); ss += v * v; }
         const float rs = rsqrtf(warp_sum(ss) / p.head + p.eps);
@@ -185,7 +228,7 @@ __global__ void __launch_bounds__(32 * QK_ROW_WARPS) qk_rows_kernel(const __grid
           for (int i = lane; i < half; i += 32) {
             const int e = first(i), f = second(i);
             float a = to_f32(x[e]) * rs * gain(e), b = to_f32(x[f]) * rs * gain(f);
-            rotate(a, b, c[i], 1.f); o[e] = from_f32<T>(a); o[f] = from_f32<T>(b);
+            rotate(a, b, c[i], s[i]); o[e] = from_f32<T>(a); o[f] = from_f32<T>(b);
           }
           for (int e = p.rot + lane; e < p.head; e += 32) o[e] = from_f32<T>(to_f32(x[e]) * rs * gain(e));
         } else {
@@ -193,7 +236,7 @@ __global__ void __launch_bounds__(32 * QK_ROW_WARPS) qk_rows_kernel(const __grid
           float sx = 0.f;
           for (int i = lane; i < half; i += 32) {
             const int e = first(i), f = second(i);
-            float a = to_f32(d[e]), b = to_f32(d[f]); rotate(a, b, c[i], -1.f);
+            float a = to_f32(d[e]), b = to_f32(d[f]); rotate(a, b, c[i], -s[i]);
             sx += a * gain(e) * to_f32(x[e]) + b * gain(f) * to_f32(x[f]);
           }
           for (int e = p.rot + lane; e < p.head; e += 32) sx += to_f32(d[e]) * gain(e) * to_f32(x[e]);
@@ -204,7 +247,7 @@ __global__ void __launch_bounds__(32 * QK_ROW_WARPS) qk_rows_kernel(const __grid
           };
           for (int i = lane; i < half; i += 32) {
             const int e = first(i), f = second(i);
-            float a = to_f32(d[e]), b = to_f32(d[f]); rotate(a, b, c[i], -1.f);
+            float a = to_f32(d[e]), b = to_f32(d[f]); rotate(a, b, c[i], -s[i]);
             put(e, a); put(f, b);
           }
           for (int e = p.rot + lane; e < p.head; e += 32) put(e, to_f32(d[e]));
@@ -223,35 +266,40 @@ __global__ void __launch_bounds__(32 * QK_ROW_WARPS) qk_rows_kernel(const __grid
   }
 }
 
-// dgain[e] = sum of the blocks' partial sums: eight threads a column, each a run of neighbouring blocks, in order
-__global__ void __launch_bounds__(256) qk_gain_kernel(const float* __restrict__ partial, int blocks, int head, float* __restrict__ dq, float* __restrict__ dk) {
-  __shared__ float red[8][32];
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, col = blockIdx.x * 32 + lane, per = (blocks + 7) / 8;
+// dgain[e] = sum of the blocks' partial sums: 32 threads a column, each a run of neighbouring blocks, in order
+__global__ void __launch_bounds__(1024) qk_gain_kernel(const float* __restrict__ partial, int blocks, int head, float* __restrict__ dq, float* __restrict__ dk) {
+  __shared__ float red[32][33];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, col = blockIdx.x * 32 + lane, per = (blocks + 31) / 32;
   float v = 0.f;
-  if (col < 2 * head && (col < head ? dq : dk))
+  if (col < 2 * head && (col < head ? dq : dk)) {
+#pragma unroll 8
     for (int b = w * per; b < min(blocks, (w + 1) * per); b++) v += __ldg(partial + (long)b * 2 * head + col);
+  }
   red[w][lane] = v;
   __syncthreads();
-  if (w == 0 && col < 2 * head) {
-    float* out = col < head ? dq : dk;
-    for (int i = 1; i < 8; i++) v += red[i][lane];
-    if (out) out[col < head ? col : col - head] = v;
-  }
+  v = warp_sum(red[lane][w]);                                        // column w of the 32
+  const int out = blockIdx.x * 32 + w;
+  if (lane == 0 && out < 2 * head) { float* d = out < head ? dq : dk; if (d) d[out < head ? out : out - head] = v; }
 }
 
+// Sets the tokens of a block and launches; *blocks: partial sums that the gradient of a gain leaves.
 template <class T, bool BWD>
-inline int qk_launch(QkParams& p, int group, unsigned grid, void* stream) {
-  const size_t turns = (size_t)p.per_block * (p.rot / 2) * sizeof(float2);
-  if (group == 0) {
-    const size_t smem = turns + (BWD ? (size_t)QK_ROW_WARPS * p.head * sizeof(float) : 0);      // at most 16 + 16 KB
-    return op_launch("qk_rows", stream, qk_rows_kernel<T, BWD>, grid, 32 * QK_ROW_WARPS, smem, 0, p);
+inline int qk_launch(QkParams p, int group, int sms, void* stream, unsigned* blocks) {
+  int most = 0; int64_t n = 1;
+  for (QkHeads& h : p.t) {
+    h.per_block = qk_tokens(p.tokens, sms, group, h.heads, BWD ? QK_HEADS_BWD : QK_HEADS_FWD, p.rot);
+    if (h.heads) { most = std::max(most, h.per_block); n = std::max(n, qk_blocks(p.tokens, sms, h.per_block)); }
   }
+  *blocks = (unsigned)n;
+  const dim3 grid((unsigned)n, p.t[1].heads ? 2 : 1);
+  const size_t turns = (size_t)most * p.rot * sizeof(float);         // at most 32 KB
   switch (group) {
-    case 2: return op_launch("qk_vec", stream, qk_vec_kernel<T, 2, BWD>, grid, QK_THREADS, turns, 0, p);
-    case 4: return op_launch("qk_vec", stream, qk_vec_kernel<T, 4, BWD>, grid, QK_THREADS, turns, 0, p);
-    case 8: return op_launch("qk_vec", stream, qk_vec_kernel<T, 8, BWD>, grid, QK_THREADS, turns, 0, p);
-    case 16: return op_launch("qk_vec", stream, qk_vec_kernel<T, 16, BWD>, grid, QK_THREADS, turns, 0, p);
-    default: return op_launch("qk_vec", stream, qk_vec_kernel<T, 32, BWD>, grid, QK_THREADS, turns, 0, p);
+    case 0: return op_launch("qk_rows", stream, qk_rows_kernel<T, BWD>, grid, dim3(32 * QK_ROW_WARPS), turns + (BWD ? (size_t)QK_ROW_WARPS * p.head * sizeof(float) : 0), 0, p);
+    case 2: return op_launch("qk_vec", stream, qk_vec_kernel<T, 2, BWD>, grid, dim3(QK_THREADS), turns, 0, p);
+    case 4: return op_launch("qk_vec", stream, qk_vec_kernel<T, 4, BWD>, grid, dim3(QK_THREADS), turns, 0, p);
+    case 8: return op_launch("qk_vec", stream, qk_vec_kernel<T, 8, BWD>, grid, dim3(QK_THREADS), turns, 0, p);
+    case 16: return op_launch("qk_vec", stream, qk_vec_kernel<T, 16, BWD>, grid, dim3(QK_THREADS), turns, 0, p);
+    default: return op_launch("qk_vec", stream, qk_vec_kernel<T, 32, BWD>, grid, dim3(QK_THREADS), turns, 0, p);
   }
 }
 inline QkHeads qk_heads(const gn_heads* x, const gn_heads* dy, const gn_heads* out, const float* gain) {
@@ -278,10 +326,10 @@ int gn_op_qk_norm_rope(gn_ctx* ctx, int dtype, int64_t tokens, int head_size, in
   GN_OP_BEGIN("op_qk_norm_rope", wrong);
   if (tokens == 0 || q->heads + (k ? k->heads : 0) == 0) return GN_OK;
   const int sms = ctx->c.sm_count; const gn_heads* all[] = {q, k, q_out, k ? k_out : nullptr};
-  QkParams p{{qk_heads(q, nullptr, q_out, gain_q), qk_heads(k, nullptr, k_out, gain_k)}, tokens, head_size, rotated, interleaved != 0, qk_tokens(tokens, sms), eps, positions, index_type, frequencies, nullptr};
+  QkParams p{{qk_heads(q, nullptr, q_out, gain_q), qk_heads(k, nullptr, k_out, gain_k)}, tokens, head_size, rotated, interleaved != 0, eps, positions, index_type, frequencies, nullptr};
   const int group = qk_group(dtype, head_size, rotated, interleaved != 0, all, 4);
-  const unsigned grid = (unsigned)qk_blocks(tokens, sms, 8);
-  return with_type(dtype, [&](auto t) { using T = decltype(t); return qk_launch<T, false>(p, group, grid, stream); });
+  unsigned blocks = 0;
+  return with_type(dtype, [&](auto t) { using T = decltype(t); return qk_launch<T, false>(p, group, sms, stream, &blocks); });
 }
 
 int gn_op_qk_norm_rope_workspace(gn_ctx* ctx, int64_t tokens, int q_heads, int k_heads, int head_size, int64_t* bytes) {
@@ -312,15 +360,15 @@ int gn_op_qk_norm_rope_backward(gn_ctx* ctx, int dtype, int64_t tokens, int head
   }
   if (gains && (!workspace || !aligned_to(workspace, 16) || workspace_bytes < qk_workspace(tokens, head_size, sms))) return fail(GN_ERR_INVALID_ARG, "op_qk_norm_rope_backward: the workspace is too small, null or not aligned");
   const gn_heads* all[] = {q, k, dq_out, k ? dk_out : nullptr, dq, k ? dk : nullptr};
-  QkParams p{{qk_heads(q, dq_out, dq, gain_q), qk_heads(k, dk_out, dk, gain_k)}, tokens, head_size, rotated, interleaved != 0, qk_tokens(tokens, sms), eps, positions, index_type, frequencies, gains ? (float*)workspace : nullptr};
+  QkParams p{{qk_heads(q, dq_out, dq, gain_q), qk_heads(k, dk_out, dk, gain_k)}, tokens, head_size, rotated, interleaved != 0, eps, positions, index_type, frequencies, gains ? (float*)workspace : nullptr};
   const int group = qk_group(dtype, head_size, rotated, interleaved != 0, all, 6);
-  const unsigned grid = (unsigned)qk_blocks(tokens, sms, QK_PER_SM);
-  if (p.t[0].heads + p.t[1].heads) GN_TRY(with_type(dtype, [&](auto t) { using T = decltype(t); return qk_launch<T, true>(p, group, grid, stream); }));
+  unsigned blocks = 0;
+  if (p.t[0].heads + p.t[1].heads) GN_TRY(with_type(dtype, [&](auto t) { using T = decltype(t); return qk_launch<T, true>(p, group, sms, stream, &blocks); }));
   // a tensor of no heads has left no partial sums
   if (dgain_q && !p.t[0].heads) { GN_CUDA(cudaMemsetAsync(dgain_q, 0, 4L * head_size, (cudaStream_t)stream)); dgain_q = nullptr; }
   if (dgain_k && !p.t[1].heads) { GN_CUDA(cudaMemsetAsync(dgain_k, 0, 4L * head_size, (cudaStream_t)stream)); dgain_k = nullptr; }
   if (!dgain_q && !dgain_k) return GN_OK;
-  return op_launch("qk_gain", stream, qk_gain_kernel, dim3((2 * head_size + 31) / 32), dim3(256), 0, 0, (const float*)workspace, (int)grid, head_size, dgain_q, dgain_k);
+  return op_launch("qk_gain", stream, qk_gain_kernel, dim3((2 * head_size + 31) / 32), dim3(1024), 0, 0, (const float*)workspace, (int)blocks, head_size, dgain_q, dgain_k);
 }
 
 }  // extern "C"

@@ -61,12 +61,18 @@ inline int qk_group(int dtype, int head_size, int rotated, bool interleaved, con
   while (2 * g < pieces) g *= 2;
   return g;
 }
-// Tokens of a block at a time: four share their block's cosines' latency once there is work for every multiprocessor, one each before that.
-inline int qk_tokens(int64_t tokens, int sms) { return tokens >= 8L * sms ? 4 : 1; }
-// Blocks: all resident at once, so that a gradient's blocks leave no more partial sums than those.
-inline int64_t qk_blocks(int64_t tokens, int sms, int per_sm) { return std::max<int64_t>(1, std::min<int64_t>(ceil_div(tokens, qk_tokens(tokens, sms)), (int64_t)sms * per_sm)); }
-constexpr int QK_PER_SM = 3;                                      // (of the gradient: 85 registers a thread; with four blocks of 64 it spilled)
-inline int64_t qk_workspace(int64_t tokens, int head_size, int sms) { return qk_blocks(tokens, sms, QK_PER_SM) * 2 * head_size * 4; }
+// Work of the queries and of the keys goes to blocks of their own.  A block takes as many tokens at a time as its groups of lanes fill, where that leaves work for all blocks, and at most
+// 32 KB of cosines and sines.
+constexpr int QK_PER_SM = 2, QK_HEADS_FWD = 4, QK_HEADS_BWD = 2;     // heads of a token that a group of lanes takes at a time
+inline int qk_tokens(int64_t tokens, int sms, int group, int heads, int heads_at_a_time, int rotated) {
+  const int64_t per_token = group ? std::max<int64_t>(1, ceil_div(heads, heads_at_a_time)) : heads, groups = group ? 256 / group : 4;
+  int64_t n = std::max<int64_t>(1, groups / std::max<int64_t>(1, per_token));
+  n = std::min(n, std::max<int64_t>(1, ceil_div(tokens, (int64_t)sms * QK_PER_SM)));
+  return (int)std::min<int64_t>(n, rotated ? std::max(1, 8192 / rotated) : 256);
+}
+// All blocks are resident at once, so that a gradient leaves no more partial sums than those.
+inline int64_t qk_blocks(int64_t tokens, int sms, int tokens_at_a_time) { return std::max<int64_t>(1, std::min<int64_t>(ceil_div(tokens, tokens_at_a_time), (int64_t)sms * QK_PER_SM)); }
+inline int64_t qk_workspace(int64_t tokens, int head_size, int sms) { return qk_blocks(tokens, sms, 1) * 2 * head_size * 4; }
 
 // ------------------------------------------------------------------ distillation
 inline const char* check_distill(int dtype, int64_t rows, int64_t vocab, int top, float temperature, const void* logits, int64_t row_stride, const void* top_ids, int index_type,
@@ -85,19 +91,21 @@ inline const char* check_distill(int dtype, int64_t rows, int64_t vocab, int top
   return nullptr;
 }
 // A row is kept on chip: `threads` threads of each of `cluster` blocks hold DISTILL_ITEMS elements each in registers.  cluster 0: the row does not fit, and is
-// read again instead.  Few rows are cut further, so that they fill the multiprocessors, down to a thousand elements per block.
+// read again instead.  512 threads at most as long as eight blocks hold the row: two blocks of an SM overlap each other's barriers.  Few rows are cut further, so that they fill the
+// multiprocessors, down to a thousand elements per block.
 constexpr int DISTILL_ITEMS = 32;
 struct DistillPlan { int cluster, threads; };
 inline DistillPlan distill_plan(int64_t rows, int64_t vocab, int sms) {
-  const int64_t slack = 16;                                          // a row may begin inside a 16-byte piece
+  const int64_t slack = 16;                                          // a row may begin inside a 16-byte piece, and blocks take whole pieces
+  auto fits = [&](int c, int threads) { return ceil_div(vocab, c) + slack <= (int64_t)threads * DISTILL_ITEMS; };
   int c = 1;
-  while (c < 8 && vocab + slack * c > (int64_t)c * 1024 * DISTILL_ITEMS) c *= 2;
-  if (vocab + slack * c > (int64_t)c * 1024 * DISTILL_ITEMS) return {0, 1024};
+  while (c < 8 && !fits(c, 512)) c *= 2;
+  if (!fits(c, 1024)) return {0, 1024};
   while (c < 8 && rows * c * 2 <= sms && vocab >= 2048L * c) c *= 2;
-  int threads = 1024;                                                // the fewest of 64, 256, 512, 1024 that hold a block's part: blocks of one multiprocessor overlap each other's barriers
-  for (int t : {512, 256, 64}) if (ceil_div(vocab, c) + slack <= (int64_t)t * DISTILL_ITEMS) threads = t;
-  return {c, threads};
+  for (int threads : {64, 256, 512}) if (fits(c, threads)) return {c, threads};
+  return {c, 1024};
 }
+inline int64_t distill_workspace(int64_t rows, int top, bool gradient) { return rows * (16 + (gradient ? 12 * (int64_t)top : 0)); }
 
 // ------------------------------------------------------------------ embedding
 inline const char* check_embedding(int dtype, int64_t tokens, int64_t vocab, int dim, float scale, const void* rows_in, int64_t in_stride, int64_t in_rows, const void* ids, int index_type,

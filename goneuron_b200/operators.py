@@ -5,205 +5,218 @@ They have no counterpart in the reference, whose layers are float32 on host slic
 (goneuron_b200.sequential) and tensors on that GPU; it enqueues its kernels on torch's current stream there, waits for nothing
 and can be captured into a CUDA graph.  Outputs and workspaces are torch allocations of the call.  Wrong arguments raise
 ValueError, failures of the library GoNeuronCudaError; what only the kernels can find (an index out of range) is kept until
-`check` reads it."""
+`check` reads it.
+
+A decoding step's kernel takes less time than an ordinary Python function around it: messages are formatted only when they are
+raised, and structures go to the library as packed bytes (norm of queries and keys for five tokens: 52 us a call with messages
+formatted ahead and ctypes structures)."""
 import ctypes as C
+from struct import Struct
+
+import torch
 
 from . import _lib
 
-
-class _Heads(C.Structure):
-    _fields_ = [("data", C.c_void_p), ("token_stride", C.c_int64), ("head_stride", C.c_int64), ("heads", C.c_int32), ("reserved", C.c_int32)]
-
-
-def _torch():
-    import torch
-    return torch
+_F32, _F64, _I32, _I64 = torch.float32, torch.float64, torch.int32, torch.int64
+_DTYPE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_heads_struct = Struct("@qqqii").pack      # gn_heads: data, token_stride, head_stride, heads, reserved
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else lambda i: torch.cuda.current_stream(i).cuda_stream
 
 
-def _dtype(t):
-    torch = _torch()
-    return {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}.get(t.dtype)
+def _here(dev, name, t):
+    """Refuses what is not a tensor on the device's GPU."""
+    if not isinstance(t, torch.Tensor):
+        raise ValueError(f"{name} is not a torch tensor")
+    if not t.is_cuda or t.get_device() != dev.device:
+        raise ValueError(f"{name} is on {t.device}, the operator runs on cuda:{dev.device}")
 
 
-def _need(ok, message):
-    if not ok:
-        raise ValueError(message)
+def _floating(dev, name, t, dtype=None):
+    """... or not of a floating type (of `dtype`), or without a contiguous last dimension; returns its shape."""
+    _here(dev, name, t)
+    if t.dtype is not dtype and (dtype is not None or t.dtype not in _DTYPE):
+        raise ValueError(f"{name} is {t.dtype}: {dtype or 'float32, float16 or bfloat16'} is needed")
+    shape = t.shape
+    if len(shape) == 0 or (t.stride(-1) != 1 and shape[-1] > 1 and t.numel()):
+        raise ValueError(f"the last dimension of {name} is not contiguous")
+    return shape
 
 
-def _tensor(dev, name, t, dims=None, dtype=None, dense=False):
-    """Checks one argument; its values are not looked at."""
-    torch = _torch()
-    _need(isinstance(t, torch.Tensor), f"{name} is not a torch tensor")
-    _need(t.is_cuda and t.device.index == dev.device, f"{name} is on {t.device}, the operator runs on cuda:{dev.device}")
-    _need(dims is None or t.dim() in ((dims,) if isinstance(dims, int) else dims), f"{name} has {t.dim()} dimensions, {dims} are needed")
-    _need(dtype is None or t.dtype == dtype, f"{name} is {t.dtype}, {dtype} is needed")
-    _need(not dense or t.is_contiguous(), f"{name} is not contiguous")
-    return t
-
-
-def _floating(dev, name, t, dims, dtype=None):
-    _tensor(dev, name, t, dims, dtype)
-    _need(_dtype(t) is not None, f"{name} is {t.dtype}: float32, float16 or bfloat16 is needed")
-    _need(t.numel() == 0 or t.shape[-1] <= 1 or t.stride(-1) == 1, f"the last dimension of {name} is not contiguous")
-    return t
+def _dense(dev, name, t, dtype, *shape):
+    """... or not a contiguous tensor of this type and shape (-1: any)."""
+    _here(dev, name, t)
+    if t.dtype is not dtype or not t.is_contiguous():
+        raise ValueError(f"{name} is {t.dtype}{'' if t.is_contiguous() else ' and not contiguous'}: contiguous {dtype} is needed")
+    if t.dim() != len(shape) or any(n != m for n, m in zip(t.shape, shape) if m >= 0):
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, {shape} is needed")
 
 
 def _index(dev, name, t):
-    torch = _torch()
-    _tensor(dev, name, t, dense=True)
-    _need(t.dtype in (torch.int32, torch.int64), f"{name} is {t.dtype}: int32 or int64 is needed")
-    return t, int(t.dtype == torch.int64)
+    """... or not contiguous int32 or int64; returns its gn_index_type."""
+    _here(dev, name, t)
+    if t.dtype is _I64:
+        wide = 1
+    elif t.dtype is _I32:
+        wide = 0
+    else:
+        raise ValueError(f"{name} is {t.dtype}: int32 or int64 is needed")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} is not contiguous")
+    return wide
 
 
 def _p(t):
-    return None if t is None or t.numel() == 0 else C.c_void_p(t.data_ptr())
+    return None if t is None else t.data_ptr() or None
 
 
-def _stream(dev):
-    return C.c_void_p(_torch().cuda.current_stream(dev.device).cuda_stream)
-
-
-def _workspace(dev, function, *args):
+def _workspace(dev, like, function, *args):
     """A workspace of the bytes that the C function gives, and those."""
     n = C.c_int64()
     _lib.check(function(dev.handle, *args, C.byref(n)))
-    torch = _torch()
-    return torch.empty(n.value, dtype=torch.uint8, device=f"cuda:{dev.device}"), n.value
+    return like.new_empty(n.value, dtype=torch.uint8), n.value
 
 
 def check(dev):
     """Waits for the current stream and raises GoNeuronCudaError for what operators found wrong on the GPU since the last call
     that did: an id or index out of range, a bounded wait that gave up."""
-    _lib.check(_lib.load().gn_op_status(dev.handle, _stream(dev)))
+    _lib.check(_lib.load().gn_op_status(dev.handle, _raw_stream(dev.device)))
 
 
 # ------------------------------------------------------------------ norm of queries and keys with the rotation
-def _as_heads(dev, name, t, like=None):
-    """[tokens, heads, size] of a tensor [..., heads, size] without copying."""
-    _floating(dev, name, t, (3, 4), None if like is None else like.dtype)
-    _need(like is None or t.shape == like.shape, f"{name} has shape {tuple(t.shape)}" + ("" if like is None else f", {tuple(like.shape)} is needed"))
-    if t.dim() == 4:
+def _heads(dev, name, t, like=None):
+    """gn_heads of a tensor [..., heads, size] without copying, and its tokens, heads and head size."""
+    shape = _floating(dev, name, t, None if like is None else like.dtype)
+    if like is not None and shape != like.shape:
+        raise ValueError(f"{name} has shape {tuple(shape)}, {tuple(like.shape)} is needed")
+    if len(shape) == 4:
         try:
-            t = t.view(t.shape[0] * t.shape[1], t.shape[2], t.shape[3])
+            t = t.view(shape[0] * shape[1], shape[2], shape[3])
         except RuntimeError:
             raise ValueError(f"{name}: the strides of its first two dimensions do not make one of tokens") from None
-    return t
+        shape = t.shape
+    elif len(shape) != 3:
+        raise ValueError(f"{name} has {len(shape)} dimensions: [tokens, heads, size] or [batch, tokens, heads, size] is needed")
+    stride = t.stride()
+    return _heads_struct(t.data_ptr(), stride[0], stride[1], shape[1], 0), shape
 
 
-def _heads(t):
-    return None if t is None else C.byref(_Heads(t.data_ptr() if t.numel() else None, t.stride(0), t.stride(1), t.shape[1], 0))
-
-
-def _qk(dev, q, k, gain_q, gain_k, positions, frequencies):
-    torch = _torch()
-    q3 = _as_heads(dev, "q", q)
-    n, _, size = q3.shape
-    k3 = None if k is None else _as_heads(dev, "k", k)
-    _need(k3 is None or (k3.dtype == q3.dtype and k3.shape[0] == n and k3.shape[2] == size), "q and k differ in type, tokens or head size")
-    for name, g in (("gain_q", gain_q), ("gain_k", gain_k)):
-        _need(g is None or _tensor(dev, name, g, 1, torch.float32, True).shape[0] == size, f"{name} has another length than a head")
-    wide, rotated = 0, 0
+def _qk(dev, q, k, gain_q, gain_k, positions, frequencies, eps, interleaved):
+    """The arguments that both directions begin with; tokens, heads of q and k, head size."""
+    hq, (n, heads, size) = _heads(dev, "q", q)
+    hk, kv = None, 0
+    if k is not None:
+        hk, (n_k, kv, size_k) = _heads(dev, "k", k)
+        if k.dtype is not q.dtype or n_k != n or size_k != size:
+            raise ValueError("q and k differ in type, tokens or head size")
+    if gain_q is not None:
+        _dense(dev, "gain_q", gain_q, _F32, size)
+    if gain_k is not None:
+        _dense(dev, "gain_k", gain_k, _F32, size)
+    wide, rotated, at = 0, 0, None
     if frequencies is not None:
-        rotated = 2 * _tensor(dev, "frequencies", frequencies, 1, torch.float64, True).shape[0]
-        _need(positions is not None, "positions are needed for a rotation")
-        positions, wide = _index(dev, "positions", positions)
-        _need(positions.numel() == n, "positions: one for each token is needed")
-    return q3, k3, rotated, wide
-
-
-def _qk_args(q3, k3, gain_q, gain_k, positions, frequencies, eps, interleaved, rotated, wide):
-    return (_dtype(q3), q3.shape[0], q3.shape[2], rotated, int(bool(interleaved)), eps, _heads(q3), _heads(k3), _p(gain_q), _p(gain_k),
-            _p(positions) if rotated else None, wide, _p(frequencies))
+        _dense(dev, "frequencies", frequencies, _F64, -1)
+        rotated = 2 * frequencies.shape[0]
+        if positions is None:
+            raise ValueError("positions are needed for a rotation")
+        wide, at = _index(dev, "positions", positions), positions.data_ptr() or None
+        if positions.numel() != n:
+            raise ValueError("positions: one for each token is needed")
+    return (_DTYPE[q.dtype], n, size, rotated, 1 if interleaved else 0, eps, hq, hk, _p(gain_q), _p(gain_k), at, wide, _p(frequencies)), n, heads, kv, size
 
 
 def qk_norm_rope(dev, q, k, gain_q=None, gain_k=None, positions=None, frequencies=None, eps=1e-5, interleaved=False, out=None):
     """RMS norm of every head of q and k ([tokens, heads, size] or [batch, tokens, heads, size]; any strides of the first dimensions,
     k may be None) with gains [size] (float32), then the rotation of the pairs by positions * frequencies.  Without frequencies
     ([rotated / 2], float64) nothing is rotated.  out: a pair of tensors for the results, q and k themselves among them."""
-    q3, k3, rotated, wide = _qk(dev, q, k, gain_q, gain_k, positions, frequencies)
-    torch = _torch()
-    qo, ko = out if out is not None else (torch.empty(q.shape, dtype=q.dtype, device=q.device), None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device))
-    qo3, ko3 = _as_heads(dev, "out[0]", qo, q), None if k is None else _as_heads(dev, "out[1]", ko, k)
-    _lib.check(_lib.load().gn_op_qk_norm_rope(dev.handle, *_qk_args(q3, k3, gain_q, gain_k, positions, frequencies, eps, interleaved, rotated, wide),
-                                              _heads(qo3), _heads(ko3), _stream(dev)))
+    args = _qk(dev, q, k, gain_q, gain_k, positions, frequencies, eps, interleaved)[0]
+    qo, ko = out if out is not None else (q.new_empty(q.shape), None if k is None else k.new_empty(k.shape))
+    _lib.check(_lib.load().gn_op_qk_norm_rope(dev.handle, *args, _heads(dev, "out[0]", qo, q)[0], None if k is None else _heads(dev, "out[1]", ko, k)[0], _raw_stream(dev.device)))
     return qo, ko
 
 
 def qk_norm_rope_backward(dev, dq_out, dk_out, q, k, gain_q=None, gain_k=None, positions=None, frequencies=None, eps=1e-5, interleaved=False):
     """Gradients (dq, dk, dgain_q, dgain_k) from those of the outputs and the forward call's inputs; those of the gains are float32."""
-    q3, k3, rotated, wide = _qk(dev, q, k, gain_q, gain_k, positions, frequencies)
-    torch = _torch()
-    dqo = _as_heads(dev, "dq_out", dq_out, q)
-    dko = None if k is None else _as_heads(dev, "dk_out", dk_out, k)
-    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    dk = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    size = q3.shape[2]
-    gains = [None if g is None or t is None else torch.empty(size, dtype=torch.float32, device=q.device) for g, t in ((gain_q, q), (gain_k, k))]
+    args, n, heads, kv, size = _qk(dev, q, k, gain_q, gain_k, positions, frequencies, eps, interleaved)
+    hdq, hdk = _heads(dev, "dq_out", dq_out, q)[0], None if k is None else _heads(dev, "dk_out", dk_out, k)[0]
+    dq, dk = q.new_empty(q.shape), None if k is None else k.new_empty(k.shape)
+    dgq = None if gain_q is None else gain_q.new_empty(size)
+    dgk = None if gain_k is None or k is None else gain_k.new_empty(size)
     L = _lib.load()
-    ws, n = _workspace(dev, L.gn_op_qk_norm_rope_workspace, q3.shape[0], q3.shape[1], 0 if k3 is None else k3.shape[1], size)
-    _lib.check(L.gn_op_qk_norm_rope_backward(dev.handle, *_qk_args(q3, k3, gain_q, gain_k, positions, frequencies, eps, interleaved, rotated, wide),
-                                             _heads(dqo), _heads(dko), _heads(_as_heads(dev, "dq", dq)), _heads(None if dk is None else _as_heads(dev, "dk", dk)),
-                                             _p(gains[0]), _p(gains[1]), _p(ws), n, _stream(dev)))
-    return dq, dk, gains[0], gains[1]
+    ws, bytes_ = _workspace(dev, q, L.gn_op_qk_norm_rope_workspace, n, heads, kv, size) if dgq is not None or dgk is not None else (None, 0)
+    _lib.check(L.gn_op_qk_norm_rope_backward(dev.handle, *args, hdq, hdk, _heads(dev, "dq", dq)[0], None if k is None else _heads(dev, "dk", dk)[0],
+                                             _p(dgq), _p(dgk), _p(ws), bytes_, _raw_stream(dev.device)))
+    return dq, dk, dgq, dgk
 
 
 # ------------------------------------------------------------------ distillation
-def _distill(dev, logits, top_ids, top_logits, temperature, row_weight, dlogits):
-    torch = _torch()
-    _floating(dev, "logits", logits, 2)
-    rows, vocab = logits.shape
-    top_ids, wide = _index(dev, "top_ids", top_ids)
-    _tensor(dev, "top_logits", top_logits, 2, torch.float32, True)
-    _need(top_ids.shape == top_logits.shape and top_ids.shape[0] == rows, "top_ids and top_logits: [rows, top] each are needed")
+def _distill(dev, logits, shape, top_ids, top_logits, temperature, row_weight, dlogits):
+    if len(shape) != 2:
+        raise ValueError(f"logits has shape {tuple(shape)}: [rows, vocabulary] is needed")
+    rows, vocab = shape
+    wide = _index(dev, "top_ids", top_ids)
+    _dense(dev, "top_logits", top_logits, _F32, rows, -1)
+    if top_ids.shape != top_logits.shape:
+        raise ValueError(f"top_ids has shape {tuple(top_ids.shape)}, top_logits {tuple(top_logits.shape)}")
     if row_weight is not None:
-        _need(_tensor(dev, "row_weight", row_weight, 1, torch.float32, True).shape[0] == rows, "row_weight: one for each row is needed")
-    loss = torch.empty(rows, dtype=torch.float32, device=logits.device)
-    _lib.check(_lib.load().gn_op_distill(dev.handle, _dtype(logits), rows, vocab, top_ids.shape[1], temperature, _p(logits), logits.stride(0), _p(top_ids), wide,
-                                         _p(top_logits), _p(row_weight), _p(loss), _p(dlogits), 0 if dlogits is None else dlogits.stride(0), _stream(dev)))
+        _dense(dev, "row_weight", row_weight, _F32, rows)
+    loss, L = top_logits.new_empty(rows), _lib.load()
+    ws, bytes_ = _workspace(dev, logits, L.gn_op_distill_workspace, rows, top_ids.shape[1], dlogits is not None)
+    _lib.check(L.gn_op_distill(dev.handle, _DTYPE[logits.dtype], rows, vocab, top_ids.shape[1], temperature, _p(logits), logits.stride(0), _p(top_ids), wide, _p(top_logits),
+                               _p(row_weight), _p(loss), _p(dlogits), 0 if dlogits is None else dlogits.stride(0), _p(ws), bytes_, _raw_stream(dev.device)))
     return loss
 
 
 def distill_loss(dev, logits, top_ids, top_logits, temperature=1.0, row_weight=None):
     """Loss of each row of logits [rows, vocab] against the teacher's top logits (top_ids with -1 for unused entries, top_logits float32,
     [rows, top] each), times row_weight."""
-    return _distill(dev, logits, top_ids, top_logits, temperature, row_weight, None)
+    return _distill(dev, logits, _floating(dev, "logits", logits), top_ids, top_logits, temperature, row_weight, None)
 
 
 def distill_loss_grad(dev, logits, top_ids, top_logits, temperature=1.0, row_weight=None, out=None):
     """(loss, dlogits): the same with the derivative of each row's loss by its logits, which are read once.  out: a tensor for dlogits, logits among them."""
-    torch = _torch()
-    _floating(dev, "logits", logits, 2)
-    d = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device) if out is None else _floating(dev, "out", out, 2, logits.dtype)
-    _need(d.shape == logits.shape, "out has another shape than logits")
-    return _distill(dev, logits, top_ids, top_logits, temperature, row_weight, d), d
+    shape = _floating(dev, "logits", logits)
+    if out is None:
+        out = logits.new_empty(shape)
+    elif _floating(dev, "out", out, logits.dtype) != shape:
+        raise ValueError("out has another shape than logits")
+    return _distill(dev, logits, shape, top_ids, top_logits, temperature, row_weight, out), out
 
 
 # ------------------------------------------------------------------ embedding
 def embedding(dev, table, ids, scale=1.0):
     """scale * table[ids]: [..., dim] for ids of any shape; rows of zeros where an id is -1."""
-    torch = _torch()
-    _floating(dev, "table", table, 2)
-    ids, wide = _index(dev, "ids", ids)
-    out = torch.empty(*ids.shape, table.shape[1], dtype=table.dtype, device=table.device)
-    _lib.check(_lib.load().gn_op_embedding(dev.handle, _dtype(table), ids.numel(), table.shape[0], table.shape[1], scale, _p(table), table.stride(0), _p(ids), wide,
-                                           _p(out), table.shape[1], _stream(dev)))
+    shape = _floating(dev, "table", table)
+    if len(shape) != 2:
+        raise ValueError(f"table has shape {tuple(shape)}: [vocab, dim] is needed")
+    wide = _index(dev, "ids", ids)
+    vocab, dim = shape
+    out = table.new_empty((*ids.shape, dim))
+    _lib.check(_lib.load().gn_op_embedding(dev.handle, _DTYPE[table.dtype], ids.numel(), vocab, dim, scale, _p(table), table.stride(0), _p(ids), wide, _p(out), dim, _raw_stream(dev.device)))
     return out
 
 
 def embedding_backward(dev, dout, ids, vocab, scale=1.0):
     """Gradient of the table, float32 [vocab, dim], from that of the lookup's output [..., dim]."""
-    torch = _torch()
-    ids, wide = _index(dev, "ids", ids)
-    _tensor(dev, "dout", dout)
-    _need(dout.dim() == ids.dim() + 1 and dout.shape[:-1] == ids.shape, "dout: a row for each id is needed")
-    dim = dout.shape[-1]
-    try:
-        rows = dout.view(ids.numel(), dim)
-    except RuntimeError:
-        raise ValueError("dout: the strides of its first dimensions do not make one of tokens") from None
-    _floating(dev, "dout", rows, 2)
-    dtable = torch.empty(vocab, dim, dtype=torch.float32, device=dout.device)
-    L = _lib.load()
-    ws, n = _workspace(dev, L.gn_op_embedding_workspace, ids.numel(), vocab, dim)
-    _lib.check(L.gn_op_embedding_backward(dev.handle, _dtype(rows), ids.numel(), vocab, dim, scale, _p(rows), rows.stride(0), _p(ids), wide, _p(dtable), _p(ws), n, _stream(dev)))
+    wide = _index(dev, "ids", ids)
+    rows, dim = _rows(dev, "dout", dout)
+    if dout.shape[:-1] != ids.shape:
+        raise ValueError("dout: a row for each id is needed")
+    dtable = dout.new_empty((vocab, dim), dtype=_F32)
+    L, n = _lib.load(), ids.numel()
+    ws, bytes_ = _workspace(dev, dout, L.gn_op_embedding_workspace, n, vocab, dim)
+    _lib.check(L.gn_op_embedding_backward(dev.handle, _DTYPE[dout.dtype], n, vocab, dim, scale, _p(rows), rows.stride(0), _p(ids), wide, _p(dtable), _p(ws), bytes_, _raw_stream(dev.device)))
     return dtable
+
+
+def _rows(dev, name, t, like=None):
+    """[tokens, dim] of a tensor [..., dim] without copying, and dim."""
+    shape = _floating(dev, name, t, None if like is None else like.dtype)
+    if like is not None and shape != like.shape:
+        raise ValueError(f"{name} has shape {tuple(shape)}, {tuple(like.shape)} is needed")
+    dim = shape[-1]
+    if len(shape) == 2:
+        return t, dim
+    try:
+        return t.view(t.numel() // dim if dim else 0, dim), dim
+    except RuntimeError:
+        raise ValueError(f"{name}: the strides of its first dimensions do not make one of tokens") from None

@@ -30,8 +30,11 @@ def _check(dev, ids, vocab, dim, type, scale, dout=None):
     d = ops.embedding_backward(dev, dout, ids, vocab, scale=scale)
     rows = dout.reshape(-1, dim).double()[there] * scale
     want, size = (torch.zeros(vocab, dim, dtype=torch.float64, device="cuda").index_add_(0, flat[there], r) for r in (rows, rows.abs()))
-    # a row's sum: at most 64 additions in a row in a piece, then an eighth of the pieces and eight more; two products
-    longest = 64 + max(1, flat.numel() // 64) / 8 + 12
+    # a row's sum: the additions of a piece of 4 to 64 places (as embedding_plan cuts them), then those of a quarter of the pieces, and four more; two products
+    chunk = 4
+    while chunk < 64 and flat.numel() > chunk * 8 * 148:
+        chunk *= 2
+    longest = chunk + flat.numel() / chunk / 4 + 8
     assert_near(d, want, 2.0 ** -24 * longest * size, "dtable")
     assert torch.equal(d, ops.embedding_backward(dev, dout, ids, vocab, scale=scale))
     return out, d

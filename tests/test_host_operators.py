@@ -48,9 +48,9 @@ static void qk() {
   IS(qk_group(GN_F16, 65, 64, false, all, 3) == 0); IS(qk_group(GN_F16, 64, 24, false, all, 3) == 0); IS(qk_group(GN_F16, 64, 24, true, all, 3) == 4); IS(qk_group(GN_F16, 1024, 0, false, all, 3) == 0);
   gn_heads odd = q; odd.token_stride = 513; all[0] = &odd; IS(qk_group(GN_F16, 64, 64, false, all, 3) == 0);
   odd = q; odd.data = at(4098); IS(qk_group(GN_F16, 64, 64, false, all, 3) == 0);
-  for (long n : {1L, 7L, 1184L, 65536L, 2000000000L}) for (int sms : {1, 148}) {
-    const long blocks = qk_blocks(n, sms, QK_PER_SM);
-    IS(blocks >= 1 && blocks <= (long)sms * QK_PER_SM && blocks <= n); IS(qk_workspace(n, 128, sms) == blocks * 1024);
+  for (long n : {1L, 7L, 1184L, 65536L, 2000000000L}) for (int sms : {1, 148}) for (int group : {0, 4, 32}) for (int heads : {0, 1, 5, 300}) for (int rot : {0, 64, 1024}) {
+    const int t = qk_tokens(n, sms, group, heads, QK_HEADS_BWD, rot); const long blocks = qk_blocks(n, sms, t);
+    IS(t >= 1 && (long)t * rot * 4 <= 32768); IS(blocks >= 1 && blocks <= (long)sms * QK_PER_SM && blocks <= n); IS(qk_workspace(n, 128, sms) >= blocks * 1024);
   }
 }
 static void distill() {
@@ -68,12 +68,12 @@ static void distill() {
   NO(check_distill(GN_BF16, 4, 100, 8, 1.f, x, 100, ids, GN_I64, t, w, l, d, 99)); OK(check_distill(GN_BF16, 1, 100, 8, 1.f, x, 100, ids, GN_I64, t, w, l, d, 0));
   NO(check_distill(GN_BF16, 4, 100, 8, 1.f, x, 104, ids, GN_I64, t, w, l, x, 100)); OK(check_distill(GN_BF16, 4, 100, 8, 1.f, x, 104, ids, GN_I64, t, w, l, x, 104));
   // a block's part of a row, wherever it begins within 16 bytes, fits its threads' registers
-  for (long rows : {1L, 24L, 149L, 100000L}) for (int v = 0; v < 40; v++) for (long vocab = std::max(1L, (1L << v / 2) - 17); vocab < (1L << v / 2) + 17 && vocab < 2000000; vocab++)
+  for (long rows : {1L, 24L, 149L, 100000L}) for (int v = 0; v < 22; v++) for (long vocab = std::max(1L, (1L << v) - 20 * (1 + v / 14)); vocab < (1L << v) + 20; vocab++)
     for (int size : {2, 4}) {
       const DistillPlan p = distill_plan(rows, vocab, 148);
       if (p.cluster == 0) { IS(vocab > 8 * 32768 - 200); continue; }
       const int V = 16 / size;
-      for (int lead = 0; lead < V; lead++) { const long pieces = ceil_div(lead + vocab, V); if (ceil_div(pieces, p.cluster) > (long)p.threads * DISTILL_ITEMS / V) { bad++; std::printf("vocab %ld rows %ld\n", vocab, rows); } }
+      for (int lead = 0; lead < V; lead++) { const long pieces = ceil_div(vocab + V - 1, V); if (lead + vocab > pieces * V || ceil_div(pieces, p.cluster) > (long)p.threads * DISTILL_ITEMS / V) { bad++; std::printf("vocab %ld rows %ld\n", vocab, rows); } }
     }
 }
 static void embedding() {
