@@ -19,6 +19,7 @@ EXPORTS = [
     "gn_op_gemm_nt", "gn_op_adam", "gn_op_layernorm", "gn_op_conv2d", "gn_op_softmax_ce", "gn_op_lstm", "gn_op_gemm_nt_static", "gn_op_attention", "gn_model_state_count", "gn_model_get_state", "gn_model_set_state",
     "gn_op_status", "gn_op_qk_norm_rope", "gn_op_qk_norm_rope_workspace", "gn_op_qk_norm_rope_backward", "gn_op_distill", "gn_op_distill_workspace",
     "gn_op_embedding", "gn_op_embedding_workspace", "gn_op_embedding_backward",
+    "gn_op_gated_ffn_saved", "gn_op_gated_ffn_workspace", "gn_op_gated_ffn", "gn_op_gated_ffn_backward",
 ]
 
 
@@ -98,6 +99,10 @@ def load():
     L.gn_op_embedding.argtypes = [vp, i, i64, i64, i, f, vp, i64, vp, i, vp, i64, vp]
     L.gn_op_embedding_workspace.argtypes = [vp, i64, i64, i, i64p]
     L.gn_op_embedding_backward.argtypes = [vp, i, i64, i64, i, f, vp, i64, vp, i, vp, vp, i64, vp]
+    L.gn_op_gated_ffn_saved.argtypes = [vp, i64, i, i, i64p]
+    L.gn_op_gated_ffn_workspace.argtypes = [vp, i64, i, i, i, i64p]
+    L.gn_op_gated_ffn.argtypes = [vp, i, i, i64, i, i, vp, i64, vp, vp, vp, vp, i64, vp, vp, i64, vp]
+    L.gn_op_gated_ffn_backward.argtypes = [vp, i, i, i64, i, i, vp, i64, vp, i64, vp, vp, vp, vp, vp, i64, vp, vp, vp, vp, i64, vp]
     _lib = L
     return L
 

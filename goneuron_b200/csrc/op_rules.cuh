@@ -4,6 +4,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
+#include <initializer_list>
 
 #include "../../include/goneuron_cuda.h"
 
@@ -142,6 +143,72 @@ inline EmbeddingPlan embedding_plan(int64_t tokens, int64_t vocab, int dim, int 
   p.hist = take(p.small ? 0 : 4 * (p.tiles << SORT_BITS));
   p.partial = take(p.chunks * 2 * (int64_t)dim * 4);                 // a piece's first and last sum may go on in its neighbours
   p.bytes = at; return p;
+}
+
+// ------------------------------------------------------------------ gated feed-forward block
+inline const char* check_ffn_sizes(int64_t tokens, int dim, int ff) {
+  if (tokens < 0 || tokens > OP_MAX_ROWS - 1024) return "tokens out of range";
+  if (dim < 8 || ff < 8 || dim % 8 || ff % 8 || dim > (1 << 24) || ff > (1 << 24)) return "dim and ff have to be multiples of 8, at most 2^24";
+  return nullptr;
+}
+inline const char* check_ffn_strides(int64_t tokens, int dim, std::initializer_list<int64_t> strides) {
+  if (tokens > 1) for (int64_t s : strides) if (s < dim || s % 8 || s >= (1LL << 38)) return "a row stride is below dim, no multiple of 8 or too large";
+  return nullptr;
+}
+inline const char* check_ffn(int dtype, int activation, int64_t tokens, int dim, int ff, std::initializer_list<const void*> pointers, std::initializer_list<int64_t> strides) {
+  if (dtype != GN_F16 && dtype != GN_BF16) return "dtype is neither GN_F16 nor GN_BF16";
+  if (activation != GN_ACT_SILU && activation != GN_ACT_GELU && activation != GN_ACT_RELU) return "activation is none of GN_ACT_SILU, GN_ACT_GELU, GN_ACT_RELU";
+  if (const char* e = check_ffn_sizes(tokens, dim, ff)) return e;
+  for (const void* p : pointers) {
+    if (tokens && !p) return "a data pointer is null";
+    if (!aligned_to(p, 16)) return "a pointer is not 16-byte aligned";
+  }
+  return check_ffn_strides(tokens, dim, strides);
+}
+// Width of the output tiles (128 x bn) and slices of the contraction of a plain product.
+struct FfnCut { int bn, splits; };
+// Left-over tiles of a last round that would keep at most half of the multiprocessors busy: they run as two halves each.
+inline int64_t ffn_tail(int64_t items, int sms) { const int64_t left = items % sms; return items > sms && 2 * left <= sms ? left : 0; }
+// The cheapest cut by a count of tensor-core cycles: a block of 64 indices takes 512 in a tile 256 wide and 330 in one 128 wide (256 of arithmetic; shared memory bounds it), a tile 4000
+// around its main loop in the first round; slices cost a launch (4000) and the float32 partial sums' way to memory and back.
+struct FfnShape { int64_t M, N; };
+inline FfnCut ffn_cut(std::initializer_list<FfnShape> shapes, int64_t kb, int sms) {
+  FfnCut best{256, 1}; double least = 1e300;
+  for (int bn : {256, 128}) {
+    int64_t tiles = 0; double elements = 0;
+    for (const FfnShape& s : shapes) { tiles += ceil_div(s.M, 128) * ceil_div(s.N, bn); elements += 128.0 * bn * ceil_div(s.M, 128) * ceil_div(s.N, bn); }
+    for (int splits = 1; splits <= 32 && splits <= kb; splits++) {
+      if (splits > 1 && (tiles * splits > 8 * sms || kb / splits < 2)) break;
+      const int64_t items = tiles * splits; double rounds = (double)ceil_div(items, sms);
+      if (splits == 1 && bn == 256 && ffn_tail(items, sms)) rounds -= 0.4;
+      double cost = rounds * (double)ceil_div(kb, splits) * (bn == 256 ? 512 : 330) + 4000;
+      if (splits > 1) cost += 4000 + elements * splits * 8 / (2500.0 * sms / 148);      // 4 bytes written, 4 read; some 2500 bytes a cycle
+      if (cost < least) { least = cost; best = FfnCut{bn, splits}; }
+    }
+  }
+  return best;
+}
+inline int64_t ffn_partial(std::initializer_list<FfnShape> shapes, const FfnCut& c) {
+  int64_t tiles = 0;
+  for (const FfnShape& s : shapes) tiles += ceil_div(s.M, 128) * ceil_div(s.N, c.bn);
+  return c.splits > 1 ? tiles * c.splits * 128 * c.bn * 4 : 0;
+}
+// Places, in bytes, in what the forward pass saves (g and u in blocks of 32 x 32, then h) and in the workspaces.
+struct FfnPlan { FfnCut y, dx, dw; int64_t saved_h, saved, fwd_h, fwd_partial, fwd, bwd_dg, bwd_du, bwd_partial, bwd; };
+inline FfnPlan ffn_plan(int64_t M, int64_t D, int64_t F, int sms) {
+  FfnPlan p{};
+  const int64_t kf = ceil_div(F, 64), h = round_up(2 * M * F, 256);
+  p.y = ffn_cut({{M, D}}, kf, sms); p.dx = ffn_cut({{M, D}}, 2 * kf, sms); p.dw = ffn_cut({{F, D}, {F, D}, {D, F}}, std::max<int64_t>(1, ceil_div(M, 64)), sms);
+  p.saved_h = ceil_div(M, 32) * ceil_div(F, 32) * 8192; p.saved = p.saved_h + h;
+  p.fwd_h = 0; p.fwd_partial = h; p.fwd = h + ffn_partial({{M, D}}, p.y);
+  p.bwd_dg = 0; p.bwd_du = h; p.bwd_partial = 2 * h; p.bwd = 2 * h + std::max(ffn_partial({{M, D}}, p.dx), ffn_partial({{F, D}, {F, D}, {D, F}}, p.dw));
+  return p;
+}
+// Few tokens: blocks of a cluster that share the contraction of 16 rows, until there are blocks for every multiprocessor.
+inline int ffn_few_cluster(int64_t N, int64_t K, int sms) {
+  int c = 1;
+  while (c < 8 && ceil_div(N, 16) * c < sms && K >= 512L * c) c *= 2;
+  return c;
 }
 
 }  // namespace gn

@@ -3,6 +3,7 @@
 #include "op_qk_norm_rope.cuh"
 #include "op_distill.cuh"
 #include "op_embedding.cuh"
+#include "op_gated_ffn.cuh"
 
 namespace gn {
 __global__ void op_status_clear_kernel(int bits) { atomicAnd(&op_status_word, ~bits); }

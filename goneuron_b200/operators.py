@@ -16,9 +16,11 @@ from struct import Struct
 import torch
 
 from . import _lib
+from .descriptors import GELU, RELU, SILU
 
 _F32, _F64, _I32, _I64 = torch.float32, torch.float64, torch.int32, torch.int64
 _DTYPE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_ACTIVATION = {"silu": SILU, "gelu": GELU, "relu": RELU}
 _heads_struct = Struct("@qqqii").pack      # gn_heads: data, token_stride, head_stride, heads, reserved
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else lambda i: torch.cuda.current_stream(i).cuda_stream
 
@@ -220,3 +222,46 @@ def _rows(dev, name, t, like=None):
         return t.view(t.numel() // dim if dim else 0, dim), dim
     except RuntimeError:
         raise ValueError(f"{name}: the strides of its first dimensions do not make one of tokens") from None
+
+
+# ------------------------------------------------------------------ gated feed-forward block
+def _ffn(dev, x, w_gate, w_up, w_down, activation):
+    """x as rows, dim and ff."""
+    if activation not in _ACTIVATION:
+        raise ValueError(f"activation {activation!r} is none of {sorted(_ACTIVATION)}")
+    rows, dim = _rows(dev, "x", x)
+    t = x.dtype
+    if t is _F32:
+        raise ValueError("x is float32: float16 or bfloat16 is needed (TransformerBlock has the 32-bit form)")
+    _dense(dev, "w_gate", w_gate, t, -1, dim)
+    ff = w_gate.shape[0]
+    _dense(dev, "w_up", w_up, t, ff, dim)
+    _dense(dev, "w_down", w_down, t, dim, ff)
+    return rows, dim, ff
+
+
+def gated_ffn(dev, x, w_gate, w_up, w_down, activation="silu", save=False):
+    """(act(x w_gate^T) * (x w_up^T)) w_down^T for x [..., dim], w_gate and w_up [ff, dim], w_down [dim, ff]; activation "silu", "gelu" (tanh form)
+    or "relu".  save: also returns what gated_ffn_backward reads, (y, saved)."""
+    rows, dim, ff = _ffn(dev, x, w_gate, w_up, w_down, activation)
+    L, n = _lib.load(), rows.shape[0]
+    y = x.new_empty(x.shape)
+    saved = _workspace(dev, x, L.gn_op_gated_ffn_saved, n, dim, ff)[0] if save else None
+    ws, bytes_ = _workspace(dev, x, L.gn_op_gated_ffn_workspace, n, dim, ff, 0)
+    _lib.check(L.gn_op_gated_ffn(dev.handle, _DTYPE[x.dtype], _ACTIVATION[activation], n, dim, ff, _p(rows), rows.stride(0), _p(w_gate), _p(w_up), _p(w_down),
+                                 _p(y), dim, _p(saved), _p(ws), bytes_, _raw_stream(dev.device)))
+    return (y, saved) if save else y
+
+
+def gated_ffn_backward(dev, dy, x, w_gate, w_up, w_down, saved, activation="silu"):
+    """Gradients (dx, dw_gate, dw_up, dw_down) from that of y, the forward call's inputs and what it saved."""
+    rows, dim, ff = _ffn(dev, x, w_gate, w_up, w_down, activation)
+    d = _rows(dev, "dy", dy, x)[0]
+    L, n, size = _lib.load(), rows.shape[0], C.c_int64()
+    _lib.check(L.gn_op_gated_ffn_saved(dev.handle, n, dim, ff, C.byref(size)))
+    _dense(dev, "saved", saved, torch.uint8, size.value)
+    dx, dwg, dwu, dwd = x.new_empty(x.shape), w_gate.new_empty((ff, dim)), w_gate.new_empty((ff, dim)), w_gate.new_empty((dim, ff))
+    ws, bytes_ = _workspace(dev, x, L.gn_op_gated_ffn_workspace, n, dim, ff, 1)
+    _lib.check(L.gn_op_gated_ffn_backward(dev.handle, _DTYPE[x.dtype], _ACTIVATION[activation], n, dim, ff, _p(d), d.stride(0), _p(rows), rows.stride(0), _p(w_gate), _p(w_up), _p(w_down),
+                                          _p(saved), _p(dx), dim, _p(dwg), _p(dwu), _p(dwd), _p(ws), bytes_, _raw_stream(dev.device)))
+    return dx, dwg, dwu, dwd

@@ -352,6 +352,23 @@ int gn_op_embedding_workspace(gn_ctx* ctx, int64_t tokens, int64_t vocab, int di
 int gn_op_embedding_backward(gn_ctx* ctx, int dtype, int64_t tokens, int64_t vocab, int dim, float scale, const void* dout, int64_t dout_stride,
                              const void* ids, int index_type, float* dtable, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* Gated feed-forward block: h = act(x Wg^T) * (x Wu^T), y = h Wd^T with x [tokens, dim] (rows x_stride apart), Wg and Wu [ff, dim],
+ * Wd [dim, ff], dense; all GN_F16 or GN_BF16 (GN_F32: GN_ERR_UNSUPPORTED, TransformerBlock has the 32-bit form).  activation: GN_ACT_SILU,
+ * GN_ACT_GELU (tanh form) or GN_ACT_RELU.  dim and ff are multiples of 8, pointers 16-byte aligned, x_stride and y_stride multiples of 8.
+ * One kernel forms both projections, the activation and the product; h is rounded to `dtype` between the two kernels.  `saved`: null, or
+ * gn_op_gated_ffn_saved bytes that the backward pass reads (both projections in float32 in the kernels' own order, and h). */
+int gn_op_gated_ffn_saved(gn_ctx* ctx, int64_t tokens, int dim, int ff, int64_t* bytes);
+int gn_op_gated_ffn_workspace(gn_ctx* ctx, int64_t tokens, int dim, int ff, int backward, int64_t* bytes);
+int gn_op_gated_ffn(gn_ctx* ctx, int dtype, int activation, int64_t tokens, int dim, int ff, const void* x, int64_t x_stride,
+                    const void* w_gate, const void* w_up, const void* w_down, void* y, int64_t y_stride, void* saved,
+                    void* workspace, int64_t workspace_bytes, void* stream);
+/* Gradients from dy [tokens, dim] (rows dy_stride apart) and what the forward call saved for the same x and weights: dx (rows dx_stride
+ * apart), dw_gate, dw_up, dw_down (dense, like the weights), all of `dtype`, each null where not wanted. */
+int gn_op_gated_ffn_backward(gn_ctx* ctx, int dtype, int activation, int64_t tokens, int dim, int ff, const void* dy, int64_t dy_stride,
+                             const void* x, int64_t x_stride, const void* w_gate, const void* w_up, const void* w_down, const void* saved,
+                             void* dx, int64_t dx_stride, void* dw_gate, void* dw_up, void* dw_down,
+                             void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

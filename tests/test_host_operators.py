@@ -93,7 +93,24 @@ static void embedding() {
     if (!p.small) IS(p.keys2 >= p.order + 4 * n && p.order2 >= p.keys2 + 4 * n && p.hist >= p.order2 + 4 * n && p.partial >= p.hist + 4 * (p.tiles << SORT_BITS));
   }
 }
-int main() { qk(); distill(); embedding(); std::printf("%d bad\n", bad); return bad != 0; }
+static void ffn() {
+  void *x = at(4096), *w = at(8192), *y = at(16384);
+  OK(check_ffn(GN_BF16, GN_ACT_SILU, 5, 64, 128, {x, w, w, w, y}, {64, 72})); OK(check_ffn(GN_F16, GN_ACT_GELU, 1, 8, 8, {x, w, w, w, y}, {0, 1})); OK(check_ffn(GN_F16, GN_ACT_RELU, 0, 8, 8, {nullptr, w}, {0}));
+  NO(check_ffn(GN_F32, GN_ACT_SILU, 5, 64, 128, {x, w}, {64})); NO(check_ffn(GN_F16, GN_ACT_TANH, 5, 64, 128, {x, w}, {64})); NO(check_ffn(GN_F16, GN_ACT_SILU, -1, 64, 128, {x, w}, {64}));
+  for (int bad : {0, -8, 4, 12, 1 << 25}) { NO(check_ffn(GN_F16, GN_ACT_SILU, 5, bad, 128, {x, w}, {1 << 26})); NO(check_ffn(GN_F16, GN_ACT_SILU, 5, 64, bad, {x, w}, {64})); }
+  NO(check_ffn(GN_F16, GN_ACT_SILU, 5, 64, 128, {x, nullptr}, {64})); NO(check_ffn(GN_F16, GN_ACT_SILU, 5, 64, 128, {x, at(4104)}, {64}));
+  for (long bad : {0L, 56L, 65L, -64L, 1L << 38}) NO(check_ffn(GN_F16, GN_ACT_SILU, 5, 64, 128, {x, w}, {64, bad}));
+  for (long m : {1L, 17L, 128L, 129L, 8192L, 16384L, 100000000L}) for (long d : {8L, 64L, 1024L, 16384L}) for (long f : {8L, 1400L, 4096L}) for (int sms : {1, 148}) {
+    const FfnPlan p = ffn_plan(m, d, f, sms);
+    const long kb[] = {ceil_div(f, 64), 2 * ceil_div(f, 64), ceil_div(m, 64)}; const FfnCut* cut[] = {&p.y, &p.dx, &p.dw};
+    for (int i = 0; i < 3; i++) IS((cut[i]->bn == 128 || cut[i]->bn == 256) && cut[i]->splits >= 1 && cut[i]->splits <= kb[i]);      // no slice is empty
+    IS(p.saved_h >= m * f * 8 && p.saved == p.saved_h + round_up(2 * m * f, 256)); IS(p.fwd_partial >= 2 * m * f && p.fwd - p.fwd_partial == ffn_partial({{m, d}}, p.y));
+    IS(p.bwd_du >= 2 * m * f && p.bwd_partial >= p.bwd_du + 2 * m * f && p.bwd - p.bwd_partial >= ffn_partial({{m, d}}, p.dx) && p.bwd - p.bwd_partial >= ffn_partial({{f, d}, {f, d}, {d, f}}, p.dw));
+  }
+  for (int sms : {1, 148}) for (long items : {1L, 147L, 148L, 149L, 222L, 223L, 512L}) { const long h = ffn_tail(items, sms); IS(h >= 0 && 2 * h <= sms && (h == 0 || h == items % sms)); }
+  for (long n : {8L, 1024L, 100000L}) for (long k : {8L, 4096L, 100000L}) { const int c = ffn_few_cluster(n, k, 148); IS(c == 1 || c == 2 || c == 4 || c == 8); }
+}
+int main() { qk(); distill(); embedding(); ffn(); std::printf("%d bad\n", bad); return bad != 0; }
 '''
 
 
@@ -140,6 +157,13 @@ def test_python_refusals_need_no_gpu():
         lambda: ops.distill_loss_grad(dev, _gpu(4, 10), _gpu(4, 3, dtype=torch.int32), _gpu(4, 3), out=_gpu(4, 9)),
         lambda: ops.embedding(dev, _gpu(10), ids), lambda: ops.embedding(dev, _gpu(10, 4), ids.float()), lambda: ops.embedding(dev, _gpu(10, 4).t(), ids), lambda: ops.embedding(dev, _gpu(10, 4), ids[::2]),
         lambda: ops.embedding_backward(dev, _gpu(5, 4), ids, 10), lambda: ops.embedding_backward(dev, _gpu(6, 4, dtype=torch.int32), ids, 10),
+    ]
+    x, w, d = _gpu(5, 16, dtype=torch.float16), _gpu(24, 16, dtype=torch.float16), _gpu(16, 24, dtype=torch.float16)
+    refused += [
+        lambda: ops.gated_ffn(dev, x, w, w, d, "tanh"), lambda: ops.gated_ffn(dev, x.float(), w.float(), w.float(), d.float()), lambda: ops.gated_ffn(dev, x.bfloat16(), w, w, d),
+        lambda: ops.gated_ffn(dev, x, w[:8], w, d), lambda: ops.gated_ffn(dev, x, w, w, w.t()), lambda: ops.gated_ffn(dev, x, w, w, w), lambda: ops.gated_ffn(dev, x[:, :8], w, w, d),
+        lambda: ops.gated_ffn(dev, torch.zeros(5, 16).half(), w, w, d), lambda: ops.gated_ffn(dev, _gpu(3, 4, 32, dtype=torch.float16)[:, :, :16].transpose(0, 1), w, w, d),
+        lambda: ops.gated_ffn_backward(dev, x[:4], x, w, w, d, w),
     ]
     for i, call in enumerate(refused):
         with pytest.raises(ValueError):
