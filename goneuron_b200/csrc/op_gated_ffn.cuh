@@ -5,7 +5,9 @@
 //
 // One kernel template for all six products: TMA loads of 64 contraction indices a stage -> shared memory -> tcgen05.mma (fp32 accumulators in tensor memory, two slots, so that
 // a tile's epilogue runs under the next tile's main loop) -> epilogue.  Operands are read as they lie in memory, rows along the contraction (K-major) or across it (MN-major), so that no
-// product needs a transposed copy.
+// product needs a transposed copy.  Pairs of blocks share a tile of 256 x 256 (cta_group::2): each holds half of A's rows and half of B's, so that an MMA of 128 cycles reads 8 KB of a
+// block's shared memory and TMA writes as much, the 128 bytes a cycle that there are.  (A block by itself, 128 x 256: 12 + 12 KB, the main loop at 62 % of the MMA rate, 1327 TFLOP/s
+// at K = 4096.)
 //   - Forward: a tile's B operand is 128 rows of Wg followed by 128 of Wu, one 256-wide MMA for both projections, and a thread of the epilogue has g and u of the same elements:
 //     activation and product are formed there and only h is written (and, for the gradient, g and u in float32).
 //   - dh is not written: its epilogue reads g and u, and writes dg and du.
@@ -25,16 +27,16 @@
 
 namespace gn {
 
-constexpr int FG_BM = 128, FG_BK = 64, FG_EPI_WARPS = 8, FG_THREADS = 64 + 32 * FG_EPI_WARPS;
+constexpr int FG_BM = 256, FG_BK = 64, FG_EPI_WARPS = 8, FG_THREADS = 64 + 32 * FG_EPI_WARPS;
 enum FgKind { FG_PLAIN, FG_GATE, FG_GATE_BWD };
 // Maps of the operands (a0, b0 for the first kb0 blocks of the contraction, a1, b1 for the others; FG_GATE: b0 and b1 side by side) and of what is written.
 struct FgProblem { CUtensorMap a0, a1, b0, b1, d0, d1; int M, N, kb0, kb, tiles_n, tiles; };
 struct FgParams {
   FgProblem p[3]; int problems, splits, full, n_half;                // items: `full` whole tiles (times slices), then n_half halves of the tiles behind them
-  float* partial; float* saved; int saved_cols; int act; unsigned spin_limit; uint32_t idesc, idesc_half;
+  float* partial; float* saved; int saved_cols; unsigned spin_limit; uint32_t idesc, idesc_half;
 };
 template <int BN> struct FgCfg {
-  static constexpr int A_BYTES = FG_BM * 128, B_BYTES = BN * 128, STAGE = A_BYTES + B_BYTES, STAGES = 192 * 1024 / STAGE;
+  static constexpr int A_BYTES = FG_BM * 64, B_BYTES = BN * 64, STAGE = A_BYTES + B_BYTES, STAGES = 192 * 1024 / STAGE;      // of one block of the pair
   static constexpr int STG = FG_EPI_WARPS * 4096;                    // an epilogue warp's 32 rows of 128 bytes on their way out
   static constexpr int SMEM = STAGES * STAGE + STG + 1024 + 256, TMEM = 2 * BN;
   static_assert(TMEM <= 512 && SMEM <= 232448 && 2 * STAGES + 5 <= 30, "");
@@ -53,17 +55,18 @@ inline uint32_t fg_idesc(bool bf16, bool amn, bool bmn, int N) {
 
 // act(g) u, and the factors of dh in dg and du
 __device__ __forceinline__ float fg_sigmoid(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
-__device__ __forceinline__ float fg_act(int act, float g) { return act == GN_ACT_SILU ? g * fg_sigmoid(g) : act == GN_ACT_GELU ? gelu_f(g) : fmaxf(g, 0.f); }
-__device__ __forceinline__ void fg_act_grad(int act, float g, float& a, float& da) {
-  if (act == GN_ACT_SILU) { const float p = fg_sigmoid(g); a = g * p; da = p * (1.f + g * (1.f - p)); }
-  else if (act == GN_ACT_GELU) {                                     // (1 + tanh z) / 2 = sigmoid(2 z) = p, 1 - tanh^2 z = 4 p (1 - p)
+template <int act> __device__ __forceinline__ float fg_act(float g) { return act == GN_ACT_SILU ? g * fg_sigmoid(g) : act == GN_ACT_GELU ? gelu_f(g) : fmaxf(g, 0.f); }
+template <int act> __device__ __forceinline__ void fg_act_grad(float g, float& a, float& da) {
+  if constexpr (act == GN_ACT_SILU) { const float p = fg_sigmoid(g); a = g * p; da = p * (1.f + g * (1.f - p)); }
+  else if constexpr (act == GN_ACT_GELU) {                                     // (1 + tanh z) / 2 = sigmoid(2 z) = p, 1 - tanh^2 z = 4 p (1 - p)
     const float p = fg_sigmoid(g * fmaf(0.07135481627f * g, g, 1.5957691216057308f));
     a = g * p; da = p + g * 2.f * p * (1.f - p) * fmaf(0.10703222440890925f * g, g, 0.7978845608028654f);
   } else { a = fmaxf(g, 0.f); da = g > 0.f ? 1.f : 0.f; }
 }
 
-template <class T, int BN, bool AMN, bool BMN, FgKind KIND>
-__global__ void __launch_bounds__(FG_THREADS, 1) fg_gemm_kernel(const __grid_constant__ FgParams P) {
+// ACT: the activation of the gates' kinds (a choice inside the loop over a row's elements kept them from overlapping: 259 instead of 2xx us for g and u of 16384 tokens)
+template <class T, int BN, bool AMN, bool BMN, FgKind KIND, int ACT>
+__global__ void __launch_bounds__(FG_THREADS, 1) __cluster_dims__(2, 1, 1) fg_gemm_kernel(const __grid_constant__ FgParams P) {
   using Cfg = FgCfg<BN>;
   constexpr int STAGES = Cfg::STAGES, STAGE = Cfg::STAGE;
   extern __shared__ uint8_t fg_smem_raw[];
@@ -73,26 +76,27 @@ __global__ void __launch_bounds__(FG_THREADS, 1) fg_gemm_kernel(const __grid_con
   volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
   const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + STAGES), tfull0 = smem_u32(bars + 2 * STAGES), tempty0 = smem_u32(bars + 2 * STAGES + 2), drain = smem_u32(bars + 2 * STAGES + 4);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const uint32_t smem0 = smem_u32(smem); const unsigned limit = P.spin_limit;
+  const uint32_t smem0 = smem_u32(smem), rank = cluster_rank(), lead_full0 = cluster_address(full0, 0), lead_tempty0 = cluster_address(tempty0, 0); const unsigned limit = P.spin_limit;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; s++) { mbar_init(full0 + 8 * s, 1); mbar_init(empty0 + 8 * s, 1); }
-    for (int b = 0; b < 2; b++) { mbar_init(tfull0 + 8 * b, 1); mbar_init(tempty0 + 8 * b, FG_EPI_WARPS); }
+    for (int b = 0; b < 2; b++) { mbar_init(tfull0 + 8 * b, 1); mbar_init(tempty0 + 8 * b, 2 * FG_EPI_WARPS); }
     mbar_init(drain, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"((uint32_t)Cfg::TMEM) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"((uint32_t)Cfg::TMEM) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
   tc_fence_before();
   __syncthreads();
+  cluster_sync_all();                                                // the other block's barriers are there
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   auto give_up = [&]() { op_report(OP_TIMEOUT); *abort_flag = 1; __threadfence_block(); };
 
-  // Items of this block, the same in every role: blockIdx.x, + gridDim.x, ...
+  // Items of this pair, the same in every role of both blocks: its number, + the number of pairs, ...
   struct Item { int q, m0, n0, k0, k1, half, slot; };                // problem, first row and column, blocks of the contraction, half (-1: whole tile), place of the partial sums
   auto item = [&](long t, Item& w) -> bool {
     long tile = t; int z = 0; w.half = -1;
@@ -112,34 +116,35 @@ __global__ void __launch_bounds__(FG_THREADS, 1) fg_gemm_kernel(const __grid_con
   const bool elected = elect_one();
   if (warp == 0) {
     bool ok = true; uint32_t s = 0, ph = 0, issued = 0; Item w;
-    for (long t = blockIdx.x; ok && item(t, w); t += gridDim.x) {
+    for (long t = blockIdx.x >> 1; ok && item(t, w); t += gridDim.x >> 1) {
       const FgProblem& p = P.p[w.q]; const int bn = w.half < 0 ? BN : BN / 2;
       for (int k = w.k0; k < w.k1; k++) {
         if (issued >= (uint32_t)STAGES && !mbar_wait(empty0 + 8 * s, ph ^ 1, limit, abort_flag)) { ok = false; break; }
         if (elected) {
-          const uint32_t base = smem0 + s * STAGE, bar = full0 + 8 * s, bb = base + Cfg::A_BYTES;
-          const bool first = KIND == FG_GATE || k < p.kb0; const CUtensorMap *a = first ? &p.a0 : &p.a1, *b = first ? &p.b0 : &p.b1;
-          const int kc = (first ? k : k - p.kb0) * FG_BK;
-          mbar_expect_tx(bar, Cfg::A_BYTES + bn * 128);
-          if constexpr (AMN) { tma_load_2d(base, a, w.m0, kc, bar); tma_load_2d(base + 8192, a, w.m0 + 64, kc, bar); }
-          else tma_load_2d(base, a, kc, w.m0, bar);
-          if constexpr (KIND == FG_GATE) { tma_load_2d(bb, &p.b0, kc, w.n0, bar); tma_load_2d(bb + BN * 64, &p.b1, kc, w.n0, bar); }
-          else if constexpr (BMN) { for (int j = 0; j < bn / 64; j++) tma_load_2d(bb + j * 8192, b, w.n0 + 64 * j, kc, bar); }
-          else { for (int j = 0; j < bn / 128; j++) tma_load_2d(bb + j * 16384, b, kc, w.n0 + 128 * j, bar); }
+          const uint32_t base = smem0 + s * STAGE, bar = lead_full0 + 8 * s, bb = base + Cfg::A_BYTES;
+          const bool first = KIND == FG_GATE || k < p.kb0; const CUtensorMap *a = first ? &p.a0 : &p.a1, *b = KIND == FG_GATE ? (rank ? &p.b1 : &p.b0) : first ? &p.b0 : &p.b1;
+          const int kc = (first ? k : k - p.kb0) * FG_BK, m0 = w.m0 + (int)rank * 128, n0 = w.n0 + (KIND == FG_GATE ? 0 : (int)rank * (bn / 2));
+          if (rank == 0) mbar_expect_tx(full0 + 8 * s, 2 * Cfg::A_BYTES + bn * 128);      // both blocks' bytes
+          if constexpr (AMN) { tma_load_2d_pair(base, a, m0, kc, bar); tma_load_2d_pair(base + 8192, a, m0 + 64, kc, bar); }
+          else tma_load_2d_pair(base, a, kc, m0, bar);
+          for (int j = 0; j < bn / 128; j++) { if constexpr (BMN) tma_load_2d_pair(bb + j * 8192, b, n0 + 64 * j, kc, bar); else tma_load_2d_pair(bb + j * 8192, b, kc, n0 + 64 * j, bar); }
         }
         issued++;
         if (++s == STAGES) { s = 0; ph ^= 1; }
       }
     }
+    // The last arrivals at this block's barriers come from the other one's MMAs: they have to be there before it leaves.
+    if (ok) for (int i = 0; i < STAGES && issued > 0; i++, issued--) { const uint32_t q = (issued - 1) % STAGES, use = (issued - 1) / STAGES; if (!mbar_wait(empty0 + 8 * q, use & 1, limit, abort_flag)) { ok = false; break; } }
     if (!ok && !*abort_flag) give_up();
-    // copies in flight write into this block's shared memory: they have to land before it leaves (the other roles' waits see them land when nothing has given up)
-    if (!ok || *abort_flag) for (int i = 0; i < STAGES; i++) if ((uint32_t)i < issued) { const uint32_t q = (issued - 1 - i) % STAGES, use = (issued - 1 - i) / STAGES; mbar_wait(full0 + 8 * q, use & 1, TC_DRAIN_LIMIT); }
+    // Something gave up: copies in flight still write into this block's shared memory and count at the first block's barriers, which not all roles wait for any more.  They land within
+    // microseconds; the pair stays for some hundred.
+    if (*abort_flag) { const long long t0 = clock64(); while (clock64() - t0 < (1LL << 18)) __nanosleep(200); }
     __syncwarp();
   } else if (warp == 1) {
     bool ok = true; uint32_t s = 0, ph = 0, lt = 0; Item w;
     const uint64_t adesc0 = fg_desc<AMN>(smem0), bdesc0 = fg_desc<BMN>(smem0 + Cfg::A_BYTES);
     constexpr uint64_t ASTEP = AMN ? 2048 >> 4 : 2, BSTEP = BMN ? 2048 >> 4 : 2;      // 16 contraction indices
-    for (long t = blockIdx.x; ok && item(t, w); t += gridDim.x) {
+    if (rank == 0) for (long t = blockIdx.x >> 1; ok && item(t, w); t += gridDim.x >> 1) {      // the first block issues for both
       const uint32_t idesc = w.half < 0 ? P.idesc : P.idesc_half, slot = lt & 1, u = lt >> 1; lt++;
       if (!mbar_wait(tempty0 + 8 * slot, (u & 1) ^ 1, limit, abort_flag)) { ok = false; break; }
       tc_fence_after();
@@ -150,16 +155,16 @@ __global__ void __launch_bounds__(FG_THREADS, 1) fg_gemm_kernel(const __grid_con
         if (elected) {
           const uint64_t a = adesc0 + (uint64_t)(s * (STAGE >> 4)), b = bdesc0 + (uint64_t)(s * (STAGE >> 4));
 #pragma unroll
-          for (int i = 0; i < 4; i++) tc_mma_f16(acc, a + i * ASTEP, b + i * BSTEP, idesc, (k > w.k0 || i > 0) ? 1u : 0u);
-          tc_commit(empty0 + 8 * s);
-          if (k == w.k1 - 1) tc_commit(tfull0 + 8 * slot);
+          for (int i = 0; i < 4; i++) tc_mma_f16_pair(acc, a + i * ASTEP, b + i * BSTEP, idesc, (k > w.k0 || i > 0) ? 1u : 0u);
+          tc_commit_pair(empty0 + 8 * s);
+          if (k == w.k1 - 1) tc_commit_pair(tfull0 + 8 * slot);
         }
         if (++s == STAGES) { s = 0; ph ^= 1; }
       }
     }
     if (!ok) {
       if (!*abort_flag) give_up();
-      if (elected) { tc_commit(drain); mbar_wait(drain, 0, TC_DRAIN_LIMIT); }
+      if (elected) { tc_commit_pair(drain); mbar_wait(drain, 0, TC_DRAIN_LIMIT); }      // MMAs in flight
     }
     __syncwarp();
   } else {
@@ -169,9 +174,9 @@ __global__ void __launch_bounds__(FG_THREADS, 1) fg_gemm_kernel(const __grid_con
     auto unit = [&](int j) { return reinterpret_cast<uint4*>(stg + lane * 128 + ((j ^ (lane & 7)) << 4)); };
     auto unit64 = [&](int which, int j) { return reinterpret_cast<uint4*>(stg + which * 2048 + lane * 64 + ((j ^ (lane >> 1 & 3)) << 4)); };
     auto free_stage = [&]() { if (lane == 0) bulk_wait_read(); __syncwarp(); };
-    for (long t = blockIdx.x; item(t, w); t += gridDim.x) {
+    for (long t = blockIdx.x >> 1; item(t, w); t += gridDim.x >> 1) {
       const FgProblem& p = P.p[w.q]; const uint32_t slot = lt & 1, u = lt >> 1; lt++;
-      const int row0 = w.m0 + quad * 32, bw = w.half < 0 ? BN : BN / 2; const uint32_t acc = tmem_base + slot * BN + ((uint32_t)(quad * 32) << 16);
+      const int row0 = w.m0 + (int)rank * 128 + quad * 32, bw = w.half < 0 ? BN : BN / 2; const uint32_t acc = tmem_base + slot * BN + ((uint32_t)(quad * 32) << 16);
       // g and u of a 32-column block, kept by the forward pass
       auto saved_at = [&](int col) { return reinterpret_cast<float4*>(P.saved) + ((long)(row0 >> 5) * P.saved_cols + (col >> 5)) * 512 + lane; };
       float4 gn_[KIND == FG_GATE_BWD ? 8 : 1], un_[KIND == FG_GATE_BWD ? 8 : 1];
@@ -191,10 +196,10 @@ __global__ void __launch_bounds__(FG_THREADS, 1) fg_gemm_kernel(const __grid_con
       got = __shfl_sync(0xffffffffu, got, 0);
       if (!got) { if (lane == 0 && !*abort_flag) give_up(); break; }
       tc_fence_after();
-      auto release = [&]() { tc_fence_before(); __syncwarp(); if (lane == 0) mbar_arrive(tempty0 + 8 * slot); };
+      auto release = [&]() { tc_fence_before(); __syncwarp(); if (lane == 0) mbar_arrive_cluster(lead_tempty0 + 8 * slot); };
       if constexpr (KIND == FG_PLAIN) {
         if (P.partial) {
-          float4* out = reinterpret_cast<float4*>(P.partial) + (long)w.slot * (FG_BM * BN / 4) + (quad * (BN / 32)) * 256 + lane;
+          float4* out = reinterpret_cast<float4*>(P.partial) + (long)w.slot * (FG_BM * BN / 4) + ((rank * 4 + quad) * (BN / 32)) * 256 + lane;
 #pragma unroll 1
           for (int c = c0; c < c0 + bw / 2; c += 32) {
             uint32_t r[32]; tmem_ld32(acc + c, r);
@@ -242,7 +247,7 @@ __global__ void __launch_bounds__(FG_THREADS, 1) fg_gemm_kernel(const __grid_con
           for (int j = 0; j < 4; j++) {
             float h[8];
 #pragma unroll
-            for (int l = 0; l < 8; l++) h[l] = fg_act(P.act, __uint_as_float(g[8 * j + l])) * __uint_as_float(v[8 * j + l]);
+            for (int l = 0; l < 8; l++) h[l] = fg_act<ACT>(__uint_as_float(g[8 * j + l])) * __uint_as_float(v[8 * j + l]);
             *unit(b * 4 + j) = make_uint4(pack2(h[0], h[1], T()), pack2(h[2], h[3], T()), pack2(h[4], h[5], T()), pack2(h[6], h[7], T()));
           }
         }
@@ -261,7 +266,7 @@ __global__ void __launch_bounds__(FG_THREADS, 1) fg_gemm_kernel(const __grid_con
           for (int j = 0; j < 8; j++) {
             const float g4[4] = {gn_[j].x, gn_[j].y, gn_[j].z, gn_[j].w}, u4[4] = {un_[j].x, un_[j].y, un_[j].z, un_[j].w}; float a[4], b[4];
 #pragma unroll
-            for (int l = 0; l < 4; l++) { float av, da; fg_act_grad(P.act, g4[l], av, da); const float d = __uint_as_float(r[4 * j + l]); a[l] = d * u4[l] * da; b[l] = d * av; }
+            for (int l = 0; l < 4; l++) { float av, da; fg_act_grad<ACT>(g4[l], av, da); const float d = __uint_as_float(r[4 * j + l]); a[l] = d * u4[l] * da; b[l] = d * av; }
             dg[2 * j] = pack2(a[0], a[1], T()); dg[2 * j + 1] = pack2(a[2], a[3], T()); du[2 * j] = pack2(b[0], b[1], T()); du[2 * j + 1] = pack2(b[2], b[3], T());
           }
           if (c + 32 < c0 + bw / 2) fetch(col + 32);
@@ -282,9 +287,10 @@ __global__ void __launch_bounds__(FG_THREADS, 1) fg_gemm_kernel(const __grid_con
   }
   tc_fence_before();
   __syncthreads();
+  cluster_sync_all();                                                // neither block's barriers are needed any more
   if (warp == 1) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((uint32_t)Cfg::TMEM) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((uint32_t)Cfg::TMEM) : "memory");
   }
 }
 
@@ -292,7 +298,7 @@ __global__ void __launch_bounds__(FG_THREADS, 1) fg_gemm_kernel(const __grid_con
 struct FgReduce { const float* partial; int splits, problems; struct { void* out; long ld; int M, N, tiles_n, tiles; } p[3]; };
 template <class T, int BN>
 __global__ void __launch_bounds__(2 * BN) fg_reduce_kernel(const __grid_constant__ FgReduce R) {
-  int tile = blockIdx.x >> 2, q = 0; const int quad = blockIdx.x & 3, lane = threadIdx.x & 31, c16 = threadIdx.x >> 5;
+  int tile = blockIdx.x >> 3, q = 0; const int quad = blockIdx.x & 7, lane = threadIdx.x & 31, c16 = threadIdx.x >> 5;
   const float4* src = reinterpret_cast<const float4*>(R.partial) + (long)tile * R.splits * (FG_BM * BN / 4) + (quad * (BN / 32) + (c16 >> 1)) * 256 + (c16 & 1) * 128 + lane;
   while (q + 1 < R.problems && tile >= R.p[q].tiles) { tile -= R.p[q].tiles; q++; }
   const int mt = tile / R.p[q].tiles_n, nt = tile - mt * R.p[q].tiles_n, row = mt * FG_BM + quad * 32 + lane, col = nt * BN + c16 * 16;
@@ -320,8 +326,8 @@ template <> __device__ __forceinline__ void mma_16x8x16<__nv_bfloat16>(float (&d
 }
 constexpr int FEW_WARPS = 8, FEW_TOKENS = 16;
 // GATE: out[t][n] = act(x w0^T) (x w1^T), else x w0^T.  n in blocks of 16, `cl` blocks of a cluster share the contraction.  NB: blocks of eight tokens.
-template <class T, bool GATE, int NB>
-__global__ void __launch_bounds__(32 * FEW_WARPS) fg_few_kernel(const T* __restrict__ x, long x_stride, const T* __restrict__ w0, const T* __restrict__ w1, int tokens, int N, int K, int act, T* __restrict__ out, long out_stride, int cl) {
+template <class T, bool GATE, int NB, int ACT>
+__global__ void __launch_bounds__(32 * FEW_WARPS) fg_few_kernel(const T* __restrict__ x, long x_stride, const T* __restrict__ w0, const T* __restrict__ w1, int tokens, int N, int K, T* __restrict__ out, long out_stride, int cl) {
   namespace cg = cooperative_groups;
   constexpr int MATS = GATE ? 2 : 1;
   __shared__ float red[FEW_WARPS][MATS * NB][4][32];
@@ -376,7 +382,7 @@ __global__ void __launch_bounds__(32 * FEW_WARPS) fg_few_kernel(const T* __restr
         v[m] = sums[m * NB * 128 + e];
         for (int r = 1; r < cl; r++) v[m] += cg::this_cluster().map_shared_rank(sums, r)[m * NB * 128 + e];
       }
-      if (n < N && t < tokens) { if constexpr (GATE) out[t * out_stride + n] = from_f32<T>(fg_act(act, v[0]) * v[1]); else out[t * out_stride + n] = from_f32<T>(v[0]); }
+      if (n < N && t < tokens) { if constexpr (GATE) out[t * out_stride + n] = from_f32<T>(fg_act<ACT>(v[0]) * v[1]); else out[t * out_stride + n] = from_f32<T>(v[0]); }
     }
   if (cl > 1) cg::this_cluster().sync();                             // (the others' sums have been read)
 }
@@ -395,7 +401,7 @@ struct FgMatrix { const void* p; int64_t rows, cols, ld; };
 // One product of a launch: D [M, N] = A B over K, operands as they lie in memory: a K-major operand is [M or N, K], an MN-major one [K, M or N].
 struct FgProduct { FgMatrix a0, a1, b0, b1, d0, d1; int64_t M, N, K; };
 
-template <class T, int BN, bool AMN, bool BMN, FgKind KIND>
+template <class T, int BN, bool AMN, bool BMN, FgKind KIND, int ACT>
 inline int fg_launch_bn(gn_ctx* ctx, const FgProduct* pr, int n, const FfnCut& cut, FgParams& P, void* stream) {
   using Cfg = FgCfg<BN>; constexpr bool bf16 = std::is_same<T, __nv_bfloat16>::value; const Ctx& c = ctx->c;
   P.problems = n; P.splits = cut.splits; P.spin_limit = c.spin_limit;
@@ -404,8 +410,7 @@ inline int fg_launch_bn(gn_ctx* ctx, const FgProduct* pr, int n, const FfnCut& c
   for (int i = 0; i < n; i++) {
     FgProblem& q = P.p[i]; const FgProduct& w = pr[i];
     auto operand = [&](CUtensorMap* m, const FgMatrix& x, bool mn, int box) { return x.p ? fg_map(c, m, bf16, x.p, x.rows, x.cols, x.ld, mn ? 64 : box, 64) : GN_OK; };
-    GN_TRY(operand(&q.a0, w.a0, AMN, FG_BM)); GN_TRY(operand(&q.a1, w.a1, AMN, FG_BM));
-    GN_TRY(operand(&q.b0, w.b0, BMN, KIND == FG_GATE ? BN / 2 : 128)); GN_TRY(operand(&q.b1, w.b1, BMN, KIND == FG_GATE ? BN / 2 : 128));
+    GN_TRY(operand(&q.a0, w.a0, AMN, 128)); GN_TRY(operand(&q.a1, w.a1, AMN, 128)); GN_TRY(operand(&q.b0, w.b0, BMN, 64)); GN_TRY(operand(&q.b1, w.b1, BMN, 64));
     const int dbox = KIND == FG_GATE_BWD ? 32 : 64;
     if (w.d0.p && !P.partial) GN_TRY(fg_map(c, &q.d0, bf16, w.d0.p, w.d0.rows, w.d0.cols, w.d0.ld, 32, dbox));
     if (w.d1.p) GN_TRY(fg_map(c, &q.d1, bf16, w.d1.p, w.d1.rows, w.d1.cols, w.d1.ld, 32, dbox));
@@ -414,52 +419,52 @@ inline int fg_launch_bn(gn_ctx* ctx, const FgProduct* pr, int n, const FfnCut& c
   }
   const int64_t items = total * cut.splits;
   if (items > 0x7fffffff) return fail(GN_ERR_UNSUPPORTED, "gated_ffn: too many output tiles");
-  P.n_half = KIND == FG_GATE || BN < 256 || P.partial ? 0 : (int)(2 * ffn_tail(items, c.sm_count)); P.full = (int)(items - P.n_half / 2);
-  auto kernel = fg_gemm_kernel<T, BN, AMN, BMN, KIND>;
+  P.n_half = KIND == FG_GATE || BN < 256 || P.partial ? 0 : (int)(2 * ffn_tail(items, ffn_pairs(c.sm_count))); P.full = (int)(items - P.n_half / 2);
+  auto kernel = fg_gemm_kernel<T, BN, AMN, BMN, KIND, ACT>;
   GN_TRY(op_smem("gated_ffn", kernel, Cfg::SMEM));
-  GN_TRY(op_launch("gated_ffn", stream, kernel, dim3((unsigned)std::min<int64_t>(items, c.sm_count)), dim3(FG_THREADS), Cfg::SMEM, 0, P));
+  GN_TRY(op_launch("gated_ffn", stream, kernel, dim3((unsigned)(2 * std::min<int64_t>(P.full + P.n_half, ffn_pairs(c.sm_count)))), dim3(FG_THREADS), Cfg::SMEM, 0, P));
   if (!P.partial) return GN_OK;
   FgReduce R{P.partial, cut.splits, n, {}};
   for (int i = 0; i < n; i++) { R.p[i].out = const_cast<void*>(pr[i].d0.p); R.p[i].ld = pr[i].d0.ld; R.p[i].M = P.p[i].M; R.p[i].N = P.p[i].N; R.p[i].tiles_n = P.p[i].tiles_n; R.p[i].tiles = P.p[i].tiles; }
-  return op_launch("gated_ffn_reduce", stream, fg_reduce_kernel<T, BN>, dim3((unsigned)(total * 4)), dim3(2 * BN), 0, 0, R);
+  return op_launch("gated_ffn_reduce", stream, fg_reduce_kernel<T, BN>, dim3((unsigned)(total * 8)), dim3(2 * BN), 0, 0, R);
 }
 // products [M, N] of one shape class, plain output
 template <class T, bool AMN, bool BMN>
 inline int fg_plain(gn_ctx* ctx, const FgProduct* pr, int n, const FfnCut& cut, float* partial, void* stream) {
   FgParams P{}; P.partial = cut.splits > 1 ? partial : nullptr;
-  return cut.bn == 256 ? fg_launch_bn<T, 256, AMN, BMN, FG_PLAIN>(ctx, pr, n, cut, P, stream) : fg_launch_bn<T, 128, AMN, BMN, FG_PLAIN>(ctx, pr, n, cut, P, stream);
+  return cut.bn == 256 ? fg_launch_bn<T, 256, AMN, BMN, FG_PLAIN, GN_ACT_LINEAR>(ctx, pr, n, cut, P, stream) : fg_launch_bn<T, 128, AMN, BMN, FG_PLAIN, GN_ACT_LINEAR>(ctx, pr, n, cut, P, stream);
 }
 
-template <class T>
-inline int ffn_forward(gn_ctx* ctx, int act, int64_t M, int D, int F, const void* x, int64_t xs, const void* wg, const void* wu, const void* wd, void* y, int64_t ys, uint8_t* saved, uint8_t* ws, void* stream) {
+template <class T, int ACT>
+inline int ffn_forward(gn_ctx* ctx, int64_t M, int D, int F, const void* x, int64_t xs, const void* wg, const void* wu, const void* wd, void* y, int64_t ys, uint8_t* saved, uint8_t* ws, void* stream) {
   const FfnPlan pl = ffn_plan(M, D, F, ctx->c.sm_count);
   void* h = saved ? saved + pl.saved_h : ws + pl.fwd_h;
   if (!saved && M <= FEW_TOKENS) {
     auto few = [&](auto kernel, const void* in, int64_t in_s, const void* a, const void* b, int N, int K, void* out, int64_t os) {
       const int cl = ffn_few_cluster(N, K, ctx->c.sm_count);
-      return op_launch("gated_ffn_few", stream, kernel, dim3((unsigned)(ceil_div(N, 16) * cl)), dim3(32 * FEW_WARPS), 0, cl, static_cast<const T*>(in), (long)in_s, static_cast<const T*>(a), static_cast<const T*>(b), (int)M, N, K, act, static_cast<T*>(out), (long)os, cl);
+      return op_launch("gated_ffn_few", stream, kernel, dim3((unsigned)(ceil_div(N, 16) * cl)), dim3(32 * FEW_WARPS), 0, cl, static_cast<const T*>(in), (long)in_s, static_cast<const T*>(a), static_cast<const T*>(b), (int)M, N, K, static_cast<T*>(out), (long)os, cl);
     };
-    if (M <= 8) { GN_TRY(few(fg_few_kernel<T, true, 1>, x, xs, wg, wu, F, D, h, F)); return few(fg_few_kernel<T, false, 1>, h, F, wd, nullptr, D, F, y, ys); }
-    GN_TRY(few(fg_few_kernel<T, true, 2>, x, xs, wg, wu, F, D, h, F)); return few(fg_few_kernel<T, false, 2>, h, F, wd, nullptr, D, F, y, ys);
+    if (M <= 8) { GN_TRY(few(fg_few_kernel<T, true, 1, ACT>, x, xs, wg, wu, F, D, h, F)); return few(fg_few_kernel<T, false, 1, GN_ACT_LINEAR>, h, F, wd, nullptr, D, F, y, ys); }
+    GN_TRY(few(fg_few_kernel<T, true, 2, ACT>, x, xs, wg, wu, F, D, h, F)); return few(fg_few_kernel<T, false, 2, GN_ACT_LINEAR>, h, F, wd, nullptr, D, F, y, ys);
   }
   const FgMatrix none{};
-  FgParams P{}; P.act = act; P.saved = reinterpret_cast<float*>(saved); P.saved_cols = (int)ceil_div(F, 32);
+  FgParams P{}; P.saved = reinterpret_cast<float*>(saved); P.saved_cols = (int)ceil_div(F, 32);
   const FgProduct gate{{x, M, D, xs}, none, {wg, F, D, D}, {wu, F, D, D}, {h, M, F, F}, none, M, F, D};
-  GN_TRY((fg_launch_bn<T, 256, false, false, FG_GATE>(ctx, &gate, 1, FfnCut{256, 1}, P, stream)));
+  GN_TRY((fg_launch_bn<T, 256, false, false, FG_GATE, ACT>(ctx, &gate, 1, FfnCut{256, 1}, P, stream)));
   const FgProduct down{{h, M, F, F}, none, {wd, D, F, F}, none, {y, M, D, ys}, none, M, D, F};
   return fg_plain<T, false, false>(ctx, &down, 1, pl.y, reinterpret_cast<float*>(ws + pl.fwd_partial), stream);
 }
 
-template <class T>
-inline int ffn_backward(gn_ctx* ctx, int act, int64_t M, int D, int F, const void* dy, int64_t dys, const void* x, int64_t xs, const void* wg, const void* wu, const void* wd, const uint8_t* saved,
+template <class T, int ACT>
+inline int ffn_backward(gn_ctx* ctx, int64_t M, int D, int F, const void* dy, int64_t dys, const void* x, int64_t xs, const void* wg, const void* wu, const void* wd, const uint8_t* saved,
                         void* dx, int64_t dxs, void* dwg, void* dwu, void* dwd, uint8_t* ws, void* stream) {
   const FfnPlan pl = ffn_plan(M, D, F, ctx->c.sm_count);
   void *dg = ws + pl.bwd_dg, *du = ws + pl.bwd_du; const void* h = saved + pl.saved_h; float* partial = reinterpret_cast<float*>(ws + pl.bwd_partial);
   const FgMatrix none{};
   if (dx || dwg || dwu) {
-    FgParams P{}; P.act = act; P.saved = reinterpret_cast<float*>(const_cast<uint8_t*>(saved)); P.saved_cols = (int)ceil_div(F, 32);
+    FgParams P{}; P.saved = reinterpret_cast<float*>(const_cast<uint8_t*>(saved)); P.saved_cols = (int)ceil_div(F, 32);
     const FgProduct dh{{dy, M, D, dys}, none, {wd, D, F, F}, none, {dg, M, F, F}, {du, M, F, F}, M, F, D};
-    GN_TRY((fg_launch_bn<T, 256, false, true, FG_GATE_BWD>(ctx, &dh, 1, FfnCut{256, 1}, P, stream)));
+    GN_TRY((fg_launch_bn<T, 256, false, true, FG_GATE_BWD, ACT>(ctx, &dh, 1, FfnCut{256, 1}, P, stream)));
   }
   if (dx) {
     const FgProduct p{{dg, M, F, F}, {du, M, F, F}, {wg, F, D, D}, {wu, F, D, D}, {dx, M, D, dxs}, none, M, D, F};
@@ -470,6 +475,13 @@ inline int ffn_backward(gn_ctx* ctx, int act, int64_t M, int D, int F, const voi
   if (dwu) w[n++] = FgProduct{{du, M, F, F}, none, {x, M, D, xs}, none, {dwu, F, D, D}, none, F, D, M};
   if (dwd) w[n++] = FgProduct{{dy, M, D, dys}, none, {h, M, F, F}, none, {dwd, D, F, F}, none, D, F, M};
   return n ? fg_plain<T, true, true>(ctx, w, n, pl.dw, partial, stream) : GN_OK;
+}
+
+template <class F> inline int with_half_and_activation(int dtype, int activation, F&& f) {
+  auto act = [&](auto t) {
+    return activation == GN_ACT_SILU ? f(t, std::integral_constant<int, GN_ACT_SILU>()) : activation == GN_ACT_GELU ? f(t, std::integral_constant<int, GN_ACT_GELU>()) : f(t, std::integral_constant<int, GN_ACT_RELU>());
+  };
+  return dtype == GN_F16 ? act(__half()) : act(__nv_bfloat16());
 }
 
 }  // namespace gn
@@ -502,8 +514,7 @@ int gn_op_gated_ffn(gn_ctx* ctx, int dtype, int activation, int64_t tokens, int 
   if (tokens == 0) return GN_OK;
   if (!workspace || !aligned_to(workspace, 16) || workspace_bytes < ffn_plan(tokens, dim, ff, ctx->c.sm_count).fwd) return fail(GN_ERR_INVALID_ARG, "op_gated_ffn: the workspace is too small, null or not aligned");
   uint8_t *s = static_cast<uint8_t*>(saved), *ws = static_cast<uint8_t*>(workspace);
-  return dtype == GN_F16 ? ffn_forward<__half>(ctx, activation, tokens, dim, ff, x, x_stride, w_gate, w_up, w_down, y, y_stride, s, ws, stream)
-                         : ffn_forward<__nv_bfloat16>(ctx, activation, tokens, dim, ff, x, x_stride, w_gate, w_up, w_down, y, y_stride, s, ws, stream);
+  return with_half_and_activation(dtype, activation, [&](auto t, auto act) { using T = decltype(t); constexpr int A = decltype(act)::value; return ffn_forward<T, A>(ctx, tokens, dim, ff, x, x_stride, w_gate, w_up, w_down, y, y_stride, s, ws, stream); });
 }
 
 int gn_op_gated_ffn_backward(gn_ctx* ctx, int dtype, int activation, int64_t tokens, int dim, int ff, const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, const void* w_gate, const void* w_up, const void* w_down,
@@ -521,8 +532,10 @@ int gn_op_gated_ffn_backward(gn_ctx* ctx, int dtype, int activation, int64_t tok
   }
   if (!workspace || !aligned_to(workspace, 16) || workspace_bytes < ffn_plan(tokens, dim, ff, ctx->c.sm_count).bwd) return fail(GN_ERR_INVALID_ARG, "op_gated_ffn_backward: the workspace is too small, null or not aligned");
   const uint8_t* s = static_cast<const uint8_t*>(saved); uint8_t* ws = static_cast<uint8_t*>(workspace);
-  return dtype == GN_F16 ? ffn_backward<__half>(ctx, activation, tokens, dim, ff, dy, dy_stride, x, x_stride, w_gate, w_up, w_down, s, dx, dx_stride, dw_gate, dw_up, dw_down, ws, stream)
-                         : ffn_backward<__nv_bfloat16>(ctx, activation, tokens, dim, ff, dy, dy_stride, x, x_stride, w_gate, w_up, w_down, s, dx, dx_stride, dw_gate, dw_up, dw_down, ws, stream);
+  return with_half_and_activation(dtype, activation, [&](auto t, auto act) {
+    using T = decltype(t); constexpr int A = decltype(act)::value;
+    return ffn_backward<T, A>(ctx, tokens, dim, ff, dy, dy_stride, x, x_stride, w_gate, w_up, w_down, s, dx, dx_stride, dw_gate, dw_up, dw_down, ws, stream);
+  });
 }
 
 }  // extern "C"

@@ -165,24 +165,26 @@ inline const char* check_ffn(int dtype, int activation, int64_t tokens, int dim,
   }
   return check_ffn_strides(tokens, dim, strides);
 }
-// Width of the output tiles (128 x bn) and slices of the contraction of a plain product.
+// Pairs of blocks that share a tile of 256 rows.
+inline int ffn_pairs(int sms) { return std::max(1, sms / 2); }
+// Width of the output tiles (256 x bn) and slices of the contraction of a plain product.
 struct FfnCut { int bn, splits; };
-// Left-over tiles of a last round that would keep at most half of the multiprocessors busy: they run as two halves each.
-inline int64_t ffn_tail(int64_t items, int sms) { const int64_t left = items % sms; return items > sms && 2 * left <= sms ? left : 0; }
-// The cheapest cut by a count of tensor-core cycles: a block of 64 indices takes 512 in a tile 256 wide and 330 in one 128 wide (256 of arithmetic; shared memory bounds it), a tile 4000
+// Left-over tiles of a last round that would keep at most half of the pairs busy: they run as two halves each.
+inline int64_t ffn_tail(int64_t items, int pairs) { const int64_t left = items % pairs; return items > pairs && 2 * left <= pairs ? left : 0; }
+// The cheapest cut by a count of tensor-core cycles: a block of 64 indices takes 540 in a tile 256 wide and 400 in one 128 wide (256 of arithmetic; shared memory bounds it), a tile 4000
 // around its main loop in the first round; slices cost a launch (4000) and the float32 partial sums' way to memory and back.
 struct FfnShape { int64_t M, N; };
 inline FfnCut ffn_cut(std::initializer_list<FfnShape> shapes, int64_t kb, int sms) {
-  FfnCut best{256, 1}; double least = 1e300;
+  FfnCut best{256, 1}; double least = 1e300; const int pairs = ffn_pairs(sms);
   for (int bn : {256, 128}) {
-    int64_t tiles = 0; double elements = 0;
-    for (const FfnShape& s : shapes) { tiles += ceil_div(s.M, 128) * ceil_div(s.N, bn); elements += 128.0 * bn * ceil_div(s.M, 128) * ceil_div(s.N, bn); }
+    int64_t tiles = 0;
+    for (const FfnShape& s : shapes) tiles += ceil_div(s.M, 256) * ceil_div(s.N, bn);
     for (int splits = 1; splits <= 32 && splits <= kb; splits++) {
-      if (splits > 1 && (tiles * splits > 8 * sms || kb / splits < 2)) break;
-      const int64_t items = tiles * splits; double rounds = (double)ceil_div(items, sms);
-      if (splits == 1 && bn == 256 && ffn_tail(items, sms)) rounds -= 0.4;
-      double cost = rounds * (double)ceil_div(kb, splits) * (bn == 256 ? 512 : 330) + 4000;
-      if (splits > 1) cost += 4000 + elements * splits * 8 / (2500.0 * sms / 148);      // 4 bytes written, 4 read; some 2500 bytes a cycle
+      if (splits > 1 && (tiles * splits > 4 * pairs || kb / splits < 2)) break;
+      const int64_t items = tiles * splits; double rounds = (double)ceil_div(items, pairs);
+      if (splits == 1 && bn == 256 && ffn_tail(items, pairs)) rounds -= 0.4;
+      double cost = rounds * (double)ceil_div(kb, splits) * (bn == 256 ? 540 : 400) + 4000;
+      if (splits > 1) cost += 4000 + (double)items * 256 * bn * 8 / (2500.0 * sms / 148);      // 4 bytes written, 4 read; some 2500 bytes a cycle
       if (cost < least) { least = cost; best = FfnCut{bn, splits}; }
     }
   }
@@ -190,8 +192,8 @@ inline FfnCut ffn_cut(std::initializer_list<FfnShape> shapes, int64_t kb, int sm
 }
 inline int64_t ffn_partial(std::initializer_list<FfnShape> shapes, const FfnCut& c) {
   int64_t tiles = 0;
-  for (const FfnShape& s : shapes) tiles += ceil_div(s.M, 128) * ceil_div(s.N, c.bn);
-  return c.splits > 1 ? tiles * c.splits * 128 * c.bn * 4 : 0;
+  for (const FfnShape& s : shapes) tiles += ceil_div(s.M, 256) * ceil_div(s.N, c.bn);
+  return c.splits > 1 ? tiles * c.splits * 256 * c.bn * 4 : 0;
 }
 // Places, in bytes, in what the forward pass saves (g and u in blocks of 32 x 32, then h) and in the workspaces.
 struct FfnPlan { FfnCut y, dx, dw; int64_t saved_h, saved, fwd_h, fwd_partial, fwd, bwd_dg, bwd_du, bwd_partial, bwd; };
