@@ -13,8 +13,9 @@
 //   - dh is not written: its epilogue reads g and u, and writes dg and du.
 //   - dx is one product over 2 ff indices, the first half of them from (dg, Wg), the second from (du, Wu).
 //   - The three weight gradients are one launch.
-// g and u are kept in float32, in the order in which the tensor memory hands them to a warp (blocks of 32 rows x 32 columns, a column quadruple of 32 rows in a row), so that both
-// epilogues move them with whole 128-byte lines.  In 16 bits their rounding would add to those of dg and du and the error of dx be 1.7 times that of its own rounding instead of 1.4.
+// g and u are kept as the upper 24 bits of their float32 values, in the order in which the tensor memory hands them to a warp (blocks of 32 rows x 16 columns), so that both epilogues move
+// them with whole 128-byte lines.  In 16 bits their rounding would add to those of dg and du and the error of dx be 1.7 times that of its own rounding instead of 1.4; the last 8 bits of
+// float32 would be a quarter of what the epilogue of dh, which memory bounds, has to read.
 // h, dg and du are rounded to 16 bits because the tensor cores read them as operands.
 // Few output tiles: the contraction is cut into slices whose float32 sums a second launch adds in order.
 //
@@ -27,17 +28,19 @@
 
 namespace gn {
 
-constexpr int FG_BM = 256, FG_BK = 64, FG_EPI_WARPS = 8, FG_THREADS = 64 + 32 * FG_EPI_WARPS;
+constexpr int FG_BM = 256, FG_BK = 64, FG_SAVED = 192;      // FG_SAVED: 16-byte pieces of a saved block
 enum FgKind { FG_PLAIN, FG_GATE, FG_GATE_BWD };
 // Maps of the operands (a0, b0 for the first kb0 blocks of the contraction, a1, b1 for the others; FG_GATE: b0 and b1 side by side) and of what is written.
 struct FgProblem { CUtensorMap a0, a1, b0, b1, d0, d1; int M, N, kb0, kb, tiles_n, tiles; };
 struct FgParams {
   FgProblem p[3]; int problems, splits, full, n_half;                // items: `full` whole tiles (times slices), then n_half halves of the tiles behind them
-  float* partial; float* saved; int saved_cols; unsigned spin_limit; uint32_t idesc, idesc_half;
+  float* partial; uint8_t* saved; int saved_cols; unsigned spin_limit; uint32_t idesc, idesc_half;
 };
-template <int BN> struct FgCfg {
-  static constexpr int A_BYTES = FG_BM * 64, B_BYTES = BN * 64, STAGE = A_BYTES + B_BYTES, STAGES = 192 * 1024 / STAGE;      // of one block of the pair
-  static constexpr int STG = FG_EPI_WARPS * 4096;                    // an epilogue warp's 32 rows of 128 bytes on their way out
+// EW epilogue warps: what the gates compute for an element is a chain of some 40 instructions, which 16 warps overlap.
+template <int BN, FgKind KIND> struct FgCfg {
+  static constexpr int EW = KIND == FG_PLAIN ? 8 : 16, THREADS = 64 + 32 * EW, COLS = BN / (KIND == FG_GATE ? 2 : 1) / (EW / 4);      // COLS: output columns of a warp
+  static constexpr int STG_WARP = KIND == FG_GATE ? 2048 : 4096, STG = EW * STG_WARP;      // an epilogue warp's 32 rows of 64 or 128 bytes on their way out (dh: two of 64)
+  static constexpr int A_BYTES = FG_BM * 64, B_BYTES = BN * 64, STAGE = A_BYTES + B_BYTES, STAGES = (224 * 1024 - STG) / STAGE;      // of one block of the pair
   static constexpr int SMEM = STAGES * STAGE + STG + 1024 + 256, TMEM = 2 * BN;
   static_assert(TMEM <= 512 && SMEM <= 232448 && 2 * STAGES + 5 <= 30, "");
 };
@@ -65,9 +68,26 @@ template <int act> __device__ __forceinline__ void fg_act_grad(float g, float& a
 }
 
 // ACT: the activation of the gates' kinds (a choice inside the loop over a row's elements kept them from overlapping: 259 instead of 2xx us for g and u of 16384 tokens)
+// 16 float32 values of a lane as the upper halves of two in a word, and the bytes below of four: 48 bytes.  (What comes back repeats that byte below itself: infinities and zeros stay, and so
+// does a NaN of the tensor core.)
+__device__ __forceinline__ void fg_pack24(const uint32_t (&v)[16], uint4 (&q)[3]) {
+  uint32_t w[12];
+#pragma unroll
+  for (int j = 0; j < 8; j++) w[j] = __byte_perm(v[2 * j], v[2 * j + 1], 0x7632);
+#pragma unroll
+  for (int j = 0; j < 4; j++) w[8 + j] = __byte_perm(__byte_perm(v[4 * j], v[4 * j + 1], 0x0051), __byte_perm(v[4 * j + 2], v[4 * j + 3], 0x0051), 0x5410);
+#pragma unroll
+  for (int j = 0; j < 3; j++) q[j] = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+}
+__device__ __forceinline__ float fg_unpack24(const uint4 (&q)[3], int i) {      // i: a constant once unrolled
+  auto word = [&](int j) { const uint4& u = q[j >> 2]; return (j & 3) == 0 ? u.x : (j & 3) == 1 ? u.y : (j & 3) == 2 ? u.z : u.w; };
+  const uint32_t lo = 4 + (i & 3);
+  return __uint_as_float(__byte_perm(word(i >> 1), word(8 + (i >> 2)), (i & 1 ? 0x3200u : 0x1000u) | (lo << 4) | lo));
+}
+
 template <class T, int BN, bool AMN, bool BMN, FgKind KIND, int ACT>
-__global__ void __launch_bounds__(FG_THREADS, 1) __cluster_dims__(2, 1, 1) fg_gemm_kernel(const __grid_constant__ FgParams P) {
-  using Cfg = FgCfg<BN>;
+__global__ void __launch_bounds__(FgCfg<BN, KIND>::THREADS, 1) __cluster_dims__(2, 1, 1) fg_gemm_kernel(const __grid_constant__ FgParams P) {
+  using Cfg = FgCfg<BN, KIND>;
   constexpr int STAGES = Cfg::STAGES, STAGE = Cfg::STAGE;
   extern __shared__ uint8_t fg_smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)fg_smem_raw + 1023) & ~(uintptr_t)1023);
@@ -80,7 +100,7 @@ __global__ void __launch_bounds__(FG_THREADS, 1) __cluster_dims__(2, 1, 1) fg_ge
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; s++) { mbar_init(full0 + 8 * s, 1); mbar_init(empty0 + 8 * s, 1); }
-    for (int b = 0; b < 2; b++) { mbar_init(tfull0 + 8 * b, 1); mbar_init(tempty0 + 8 * b, 2 * FG_EPI_WARPS); }
+    for (int b = 0; b < 2; b++) { mbar_init(tfull0 + 8 * b, 1); mbar_init(tempty0 + 8 * b, 2 * Cfg::EW); }
     mbar_init(drain, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -169,28 +189,29 @@ __global__ void __launch_bounds__(FG_THREADS, 1) __cluster_dims__(2, 1, 1) fg_ge
     __syncwarp();
   } else {
     const int ew = warp - 2, quad = warp & 3, cg = ew >> 2; uint32_t lt = 0; Item w;
-    uint8_t* stg = smem + STAGES * STAGE + ew * 4096; const uint32_t stg_addr = smem_u32(stg);
+    uint8_t* stg = smem + STAGES * STAGE + ew * Cfg::STG_WARP; const uint32_t stg_addr = smem_u32(stg);
     // this lane's row of the staging buffer, 16-byte unit j of it, as the swizzles of the stores' maps want them
-    auto unit = [&](int j) { return reinterpret_cast<uint4*>(stg + lane * 128 + ((j ^ (lane & 7)) << 4)); };
-    auto unit64 = [&](int which, int j) { return reinterpret_cast<uint4*>(stg + which * 2048 + lane * 64 + ((j ^ (lane >> 1 & 3)) << 4)); };
+    [[maybe_unused]] auto unit = [&](int j) { return reinterpret_cast<uint4*>(stg + lane * 128 + ((j ^ (lane & 7)) << 4)); };
+    [[maybe_unused]] auto unit64 = [&](int which, int j) { return reinterpret_cast<uint4*>(stg + which * 2048 + lane * 64 + ((j ^ (lane >> 1 & 3)) << 4)); };
     auto free_stage = [&]() { if (lane == 0) bulk_wait_read(); __syncwarp(); };
-    for (long t = blockIdx.x >> 1; item(t, w); t += gridDim.x >> 1) {
-      const FgProblem& p = P.p[w.q]; const uint32_t slot = lt & 1, u = lt >> 1; lt++;
-      const int row0 = w.m0 + (int)rank * 128 + quad * 32, bw = w.half < 0 ? BN : BN / 2; const uint32_t acc = tmem_base + slot * BN + ((uint32_t)(quad * 32) << 16);
-      // g and u of a 32-column block, kept by the forward pass
-      auto saved_at = [&](int col) { return reinterpret_cast<float4*>(P.saved) + ((long)(row0 >> 5) * P.saved_cols + (col >> 5)) * 512 + lane; };
-      float4 gn_[KIND == FG_GATE_BWD ? 8 : 1], un_[KIND == FG_GATE_BWD ? 8 : 1];
-      auto fetch = [&](int col) {
-        if constexpr (KIND == FG_GATE_BWD) {
-          if (row0 < p.M && col < p.N) {
-            const float4* q = saved_at(col);
+    // g and u of a 32 x 16 block, kept by the forward pass
+    auto saved_at = [&](int row, int col) { return reinterpret_cast<uint4*>(P.saved) + ((long)(row >> 5) * P.saved_cols + (col >> 4)) * FG_SAVED + lane; };
+    auto row_of = [&](const Item& i) { return i.m0 + (int)rank * 128 + quad * 32; };
+    auto first_col = [&](const Item& i) { return cg * (Cfg::COLS >> (i.half >= 0)); };      // of this warp's, in the tile
+    uint4 gn_[3], un_[3];                                            // dh: those of the next block
+    auto fetch = [&](const Item& i, int col) {
+      if (row_of(i) < P.p[i.q].M && col < P.p[i.q].N) {
+        const uint4* q = saved_at(row_of(i), col);
 #pragma unroll
-            for (int j = 0; j < 8; j++) { gn_[j] = __ldcs(q + j * 32); un_[j] = __ldcs(q + 256 + j * 32); }
-          }
-        }
-      };
-      const int c0 = cg * (bw / 2);                                  // this warp's columns of the tile: [c0, c0 + bw / 2)
-      if constexpr (KIND == FG_GATE_BWD) fetch(w.n0 + c0);
+        for (int j = 0; j < 3; j++) { gn_[j] = __ldcs(q + j * 32); un_[j] = __ldcs(q + (3 + j) * 32); }
+      }
+    };
+    long t = blockIdx.x >> 1; Item next; bool more = item(t, next);
+    if constexpr (KIND == FG_GATE_BWD) { if (more) fetch(next, next.n0 + first_col(next)); }
+    while (more) {
+      w = next; t += gridDim.x >> 1; more = item(t, next);
+      const FgProblem& p = P.p[w.q]; const uint32_t slot = lt & 1, u = lt >> 1; lt++;
+      const int row0 = row_of(w), c0 = first_col(w), c1 = c0 + (Cfg::COLS >> (w.half >= 0)); const uint32_t acc = tmem_base + slot * BN + ((uint32_t)(quad * 32) << 16);
       int got = 1;
       if (lane == 0) got = mbar_wait(tfull0 + 8 * slot, u & 1, limit, abort_flag) ? 1 : 0;
       got = __shfl_sync(0xffffffffu, got, 0);
@@ -201,7 +222,7 @@ __global__ void __launch_bounds__(FG_THREADS, 1) __cluster_dims__(2, 1, 1) fg_ge
         if (P.partial) {
           float4* out = reinterpret_cast<float4*>(P.partial) + (long)w.slot * (FG_BM * BN / 4) + ((rank * 4 + quad) * (BN / 32)) * 256 + lane;
 #pragma unroll 1
-          for (int c = c0; c < c0 + bw / 2; c += 32) {
+          for (int c = c0; c < c1; c += 32) {
             uint32_t r[32]; tmem_ld32(acc + c, r);
             asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
@@ -210,10 +231,10 @@ __global__ void __launch_bounds__(FG_THREADS, 1) __cluster_dims__(2, 1, 1) fg_ge
           release();
         } else {
 #pragma unroll 1
-          for (int c = c0; c < c0 + bw / 2; c += 64) {
+          for (int c = c0; c < c1; c += 64) {
             uint32_t r[32], q[32]; tmem_ld32(acc + c, r); tmem_ld32(acc + c + 32, q);
             asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-            if (c + 64 >= c0 + bw / 2) release();
+            if (c + 64 >= c1) release();
             free_stage();
 #pragma unroll
             for (int j = 0; j < 4; j++) {
@@ -227,58 +248,66 @@ __global__ void __launch_bounds__(FG_THREADS, 1) __cluster_dims__(2, 1, 1) fg_ge
           }
         }
       } else if constexpr (KIND == FG_GATE) {
-        // BN / 4 columns of h a warp: 64
         free_stage();
-#pragma unroll 1
-        for (int b = 0; b < BN / 128; b++) {
-          const int c = cg * (BN / 4) + b * 32, col = w.n0 + c;
-          uint32_t g[32], v[32]; tmem_ld32(acc + c, g); tmem_ld32(acc + BN / 2 + c, v);
-          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-          if (b == BN / 128 - 1) release();
-          if (P.saved && row0 < p.M && col < p.N) {
-            float4* s = saved_at(col);
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-              __stcs(s + j * 32, make_float4(__uint_as_float(g[4 * j]), __uint_as_float(g[4 * j + 1]), __uint_as_float(g[4 * j + 2]), __uint_as_float(g[4 * j + 3])));
-              __stcs(s + 256 + j * 32, make_float4(__uint_as_float(v[4 * j]), __uint_as_float(v[4 * j + 1]), __uint_as_float(v[4 * j + 2]), __uint_as_float(v[4 * j + 3])));
-            }
+        for (int c = 0; c < Cfg::COLS; c += 16) {
+          const int col = w.n0 + c0 + c;
+          uint32_t g[16], v[16]; tmem_ld16(acc + c0 + c, g); tmem_ld16(acc + BN / 2 + c0 + c, v);
+          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+          if (c + 16 >= Cfg::COLS) release();
+          if (P.saved && row0 < p.M && col < p.N) {
+            uint4 *s = saved_at(row0, col), q[3];
+            fg_pack24(g, q);
+#pragma unroll
+            for (int j = 0; j < 3; j++) __stcs(s + j * 32, q[j]);
+            fg_pack24(v, q);
+#pragma unroll
+            for (int j = 0; j < 3; j++) __stcs(s + (3 + j) * 32, q[j]);
           }
 #pragma unroll
-          for (int j = 0; j < 4; j++) {
+          for (int j = 0; j < 2; j++) {
             float h[8];
 #pragma unroll
             for (int l = 0; l < 8; l++) h[l] = fg_act<ACT>(__uint_as_float(g[8 * j + l])) * __uint_as_float(v[8 * j + l]);
-            *unit(b * 4 + j) = make_uint4(pack2(h[0], h[1], T()), pack2(h[2], h[3], T()), pack2(h[4], h[5], T()), pack2(h[6], h[7], T()));
+            *unit64(0, c / 8 + j) = make_uint4(pack2(h[0], h[1], T()), pack2(h[2], h[3], T()), pack2(h[4], h[5], T()), pack2(h[6], h[7], T()));
           }
         }
         fence_async_smem();
         __syncwarp();
-        if (lane == 0 && row0 < p.M && w.n0 + cg * (BN / 4) < p.N) { tma_store_2d(&p.d0, w.n0 + cg * (BN / 4), row0, stg_addr); bulk_commit(); }
+        if (lane == 0 && row0 < p.M && w.n0 + c0 < p.N) { tma_store_2d(&p.d0, w.n0 + c0, row0, stg_addr); bulk_commit(); }
       } else {
 #pragma unroll 1
-        for (int c = c0; c < c0 + bw / 2; c += 32) {
-          const int col = w.n0 + c;
-          uint32_t r[32]; tmem_ld32(acc + c, r);
+        for (int c = c0; c < c1; c += 16) {
+          const int col = w.n0 + c; const bool odd = (c - c0) & 16;      // blocks of 32 columns go out, their halves one after the other
+          uint4 g[3], v[3];
+#pragma unroll
+          for (int j = 0; j < 3; j++) { g[j] = gn_[j]; v[j] = un_[j]; }
+          if (c + 16 < c1) fetch(w, col + 16); else if (more) fetch(next, next.n0 + first_col(next));      // on its way while this one is worked on
+          uint32_t r[16]; tmem_ld16(acc + c, r);
           asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-          if (c + 32 >= c0 + bw / 2) release();
-          uint32_t dg[16], du[16];
+          if (c + 16 >= c1) release();
+          uint32_t dg[8], du[8];
 #pragma unroll
           for (int j = 0; j < 8; j++) {
-            const float g4[4] = {gn_[j].x, gn_[j].y, gn_[j].z, gn_[j].w}, u4[4] = {un_[j].x, un_[j].y, un_[j].z, un_[j].w}; float a[4], b[4];
+            float a[2], b[2];
 #pragma unroll
-            for (int l = 0; l < 4; l++) { float av, da; fg_act_grad<ACT>(g4[l], av, da); const float d = __uint_as_float(r[4 * j + l]); a[l] = d * u4[l] * da; b[l] = d * av; }
-            dg[2 * j] = pack2(a[0], a[1], T()); dg[2 * j + 1] = pack2(a[2], a[3], T()); du[2 * j] = pack2(b[0], b[1], T()); du[2 * j + 1] = pack2(b[2], b[3], T());
+            for (int l = 0; l < 2; l++) {
+              float av, da; fg_act_grad<ACT>(fg_unpack24(g, 2 * j + l), av, da);
+              const float d = __uint_as_float(r[2 * j + l]); a[l] = d * fg_unpack24(v, 2 * j + l) * da; b[l] = d * av;
+            }
+            dg[j] = pack2(a[0], a[1], T()); du[j] = pack2(b[0], b[1], T());
           }
-          if (c + 32 < c0 + bw / 2) fetch(col + 32);
-          free_stage();
+          if (!odd) free_stage();
 #pragma unroll
-          for (int j = 0; j < 4; j++) {
-            *unit64(0, j) = make_uint4(dg[4 * j], dg[4 * j + 1], dg[4 * j + 2], dg[4 * j + 3]);
-            *unit64(1, j) = make_uint4(du[4 * j], du[4 * j + 1], du[4 * j + 2], du[4 * j + 3]);
+          for (int j = 0; j < 2; j++) {
+            *unit64(0, 2 * odd + j) = make_uint4(dg[4 * j], dg[4 * j + 1], dg[4 * j + 2], dg[4 * j + 3]);
+            *unit64(1, 2 * odd + j) = make_uint4(du[4 * j], du[4 * j + 1], du[4 * j + 2], du[4 * j + 3]);
           }
-          fence_async_smem();
-          __syncwarp();
-          if (lane == 0 && row0 < p.M && col < p.N) { tma_store_2d(&p.d0, col, row0, stg_addr); tma_store_2d(&p.d1, col, row0, stg_addr + 2048); bulk_commit(); }
+          if (odd) {
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0 && row0 < p.M && col - 16 < p.N) { tma_store_2d(&p.d0, col - 16, row0, stg_addr); tma_store_2d(&p.d1, col - 16, row0, stg_addr + 2048); bulk_commit(); }
+          }
         }
       }
     }
@@ -403,7 +432,7 @@ struct FgProduct { FgMatrix a0, a1, b0, b1, d0, d1; int64_t M, N, K; };
 
 template <class T, int BN, bool AMN, bool BMN, FgKind KIND, int ACT>
 inline int fg_launch_bn(gn_ctx* ctx, const FgProduct* pr, int n, const FfnCut& cut, FgParams& P, void* stream) {
-  using Cfg = FgCfg<BN>; constexpr bool bf16 = std::is_same<T, __nv_bfloat16>::value; const Ctx& c = ctx->c;
+  using Cfg = FgCfg<BN, KIND>; constexpr bool bf16 = std::is_same<T, __nv_bfloat16>::value; const Ctx& c = ctx->c;
   P.problems = n; P.splits = cut.splits; P.spin_limit = c.spin_limit;
   P.idesc = fg_idesc(bf16, AMN, BMN, BN); P.idesc_half = fg_idesc(bf16, AMN, BMN, BN / 2);
   int64_t total = 0;
@@ -411,7 +440,7 @@ inline int fg_launch_bn(gn_ctx* ctx, const FgProduct* pr, int n, const FfnCut& c
     FgProblem& q = P.p[i]; const FgProduct& w = pr[i];
     auto operand = [&](CUtensorMap* m, const FgMatrix& x, bool mn, int box) { return x.p ? fg_map(c, m, bf16, x.p, x.rows, x.cols, x.ld, mn ? 64 : box, 64) : GN_OK; };
     GN_TRY(operand(&q.a0, w.a0, AMN, 128)); GN_TRY(operand(&q.a1, w.a1, AMN, 128)); GN_TRY(operand(&q.b0, w.b0, BMN, 64)); GN_TRY(operand(&q.b1, w.b1, BMN, 64));
-    const int dbox = KIND == FG_GATE_BWD ? 32 : 64;
+    const int dbox = KIND == FG_PLAIN ? 64 : 32;
     if (w.d0.p && !P.partial) GN_TRY(fg_map(c, &q.d0, bf16, w.d0.p, w.d0.rows, w.d0.cols, w.d0.ld, 32, dbox));
     if (w.d1.p) GN_TRY(fg_map(c, &q.d1, bf16, w.d1.p, w.d1.rows, w.d1.cols, w.d1.ld, 32, dbox));
     q.M = (int)w.M; q.N = (int)w.N; q.kb0 = (int)ceil_div(w.K, FG_BK); q.kb = q.kb0 * (KIND == FG_PLAIN && w.a1.p ? 2 : 1);
@@ -422,7 +451,7 @@ inline int fg_launch_bn(gn_ctx* ctx, const FgProduct* pr, int n, const FfnCut& c
   P.n_half = KIND == FG_GATE || BN < 256 || P.partial ? 0 : (int)(2 * ffn_tail(items, ffn_pairs(c.sm_count))); P.full = (int)(items - P.n_half / 2);
   auto kernel = fg_gemm_kernel<T, BN, AMN, BMN, KIND, ACT>;
   GN_TRY(op_smem("gated_ffn", kernel, Cfg::SMEM));
-  GN_TRY(op_launch("gated_ffn", stream, kernel, dim3((unsigned)(2 * std::min<int64_t>(P.full + P.n_half, ffn_pairs(c.sm_count)))), dim3(FG_THREADS), Cfg::SMEM, 0, P));
+  GN_TRY(op_launch("gated_ffn", stream, kernel, dim3((unsigned)(2 * std::min<int64_t>(P.full + P.n_half, ffn_pairs(c.sm_count)))), dim3(Cfg::THREADS), Cfg::SMEM, 0, P));
   if (!P.partial) return GN_OK;
   FgReduce R{P.partial, cut.splits, n, {}};
   for (int i = 0; i < n; i++) { R.p[i].out = const_cast<void*>(pr[i].d0.p); R.p[i].ld = pr[i].d0.ld; R.p[i].M = P.p[i].M; R.p[i].N = P.p[i].N; R.p[i].tiles_n = P.p[i].tiles_n; R.p[i].tiles = P.p[i].tiles; }
@@ -448,7 +477,7 @@ inline int ffn_forward(gn_ctx* ctx, int64_t M, int D, int F, const void* x, int6
     GN_TRY(few(fg_few_kernel<T, true, 2, ACT>, x, xs, wg, wu, F, D, h, F)); return few(fg_few_kernel<T, false, 2, GN_ACT_LINEAR>, h, F, wd, nullptr, D, F, y, ys);
   }
   const FgMatrix none{};
-  FgParams P{}; P.saved = reinterpret_cast<float*>(saved); P.saved_cols = (int)ceil_div(F, 32);
+  FgParams P{}; P.saved = saved; P.saved_cols = (int)ceil_div(F, 16);
   const FgProduct gate{{x, M, D, xs}, none, {wg, F, D, D}, {wu, F, D, D}, {h, M, F, F}, none, M, F, D};
   GN_TRY((fg_launch_bn<T, 256, false, false, FG_GATE, ACT>(ctx, &gate, 1, FfnCut{256, 1}, P, stream)));
   const FgProduct down{{h, M, F, F}, none, {wd, D, F, F}, none, {y, M, D, ys}, none, M, D, F};
@@ -462,7 +491,7 @@ inline int ffn_backward(gn_ctx* ctx, int64_t M, int D, int F, const void* dy, in
   void *dg = ws + pl.bwd_dg, *du = ws + pl.bwd_du; const void* h = saved + pl.saved_h; float* partial = reinterpret_cast<float*>(ws + pl.bwd_partial);
   const FgMatrix none{};
   if (dx || dwg || dwu) {
-    FgParams P{}; P.saved = reinterpret_cast<float*>(const_cast<uint8_t*>(saved)); P.saved_cols = (int)ceil_div(F, 32);
+    FgParams P{}; P.saved = const_cast<uint8_t*>(saved); P.saved_cols = (int)ceil_div(F, 16);
     const FgProduct dh{{dy, M, D, dys}, none, {wd, D, F, F}, none, {dg, M, F, F}, {du, M, F, F}, M, F, D};
     GN_TRY((fg_launch_bn<T, 256, false, true, FG_GATE_BWD, ACT>(ctx, &dh, 1, FfnCut{256, 1}, P, stream)));
   }

@@ -55,10 +55,12 @@ def _check(dev, x, wg, wu, wd, dy, act):
     g, u, h = g.detach(), u.detach(), h.detach()
     # What the second products read is rounded once to 16 bits (half a step, or that of the subnormal numbers), behind float32: g, u and dh are sums over d with errors relative to the sums of
     # their sizes, which reach h, dg and du by the derivatives (act'' is at most 1.2); activation, derivative and products have 2^-19 (exponential and quotient of a few 2^-22).
+    # The gradient reads g and u with 24 bits: cut off below 2^-15 of them.
     rel, small = rounding(x.dtype)
     a, da = ACT[act](g).abs(), torch.autograd.functional.jvp(ACT[act], (g,), (torch.ones_like(g),))[1].abs()
     cd, eg, eu, edh = _accumulated(d), X.abs() @ G.abs().T, X.abs() @ U.abs().T, DY.abs() @ D.abs()
     Eh = rel * h.abs() + small + cd * (da * u.abs() * eg + a * eu) + 2.0 ** -19 * h.abs()
+    eg, eu = eg + 2.0 ** -15 * g.abs() / cd, eu + 2.0 ** -15 * u.abs() / cd
     Edg = rel * dg.abs() + small + cd * (u.abs() * da * edh + dh.abs() * da * eu + 1.2 * dh.abs() * u.abs() * eg) + 2.0 ** -19 * dh.abs() * u.abs() * (da + 0.1)
     Edu = rel * du.abs() + small + cd * (a * edh + dh.abs() * da * eg) + 2.0 ** -19 * du.abs()
     down = Eh @ D.abs().T + _accumulated(f) * (h.abs() @ D.abs().T)

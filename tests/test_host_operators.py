@@ -104,7 +104,7 @@ static void ffn() {
     const FfnPlan p = ffn_plan(m, d, f, sms);
     const long kb[] = {ceil_div(f, 64), 2 * ceil_div(f, 64), ceil_div(m, 64)}; const FfnCut* cut[] = {&p.y, &p.dx, &p.dw};
     for (int i = 0; i < 3; i++) IS((cut[i]->bn == 128 || cut[i]->bn == 256) && cut[i]->splits >= 1 && cut[i]->splits <= kb[i]);      // no slice is empty
-    IS(p.saved_h >= m * f * 8 && p.saved == p.saved_h + round_up(2 * m * f, 256)); IS(p.fwd_partial >= 2 * m * f && p.fwd - p.fwd_partial == ffn_partial({{m, d}}, p.y));
+    IS(p.saved_h >= m * f * 6 && p.saved == p.saved_h + round_up(2 * m * f, 256)); IS(p.fwd_partial >= 2 * m * f && p.fwd - p.fwd_partial == ffn_partial({{m, d}}, p.y));
     IS(p.bwd_du >= 2 * m * f && p.bwd_partial >= p.bwd_du + 2 * m * f && p.bwd - p.bwd_partial >= ffn_partial({{m, d}}, p.dx) && p.bwd - p.bwd_partial >= ffn_partial({{f, d}, {f, d}, {d, f}}, p.dw));
   }
   for (int sms : {1, 148}) for (long items : {1L, 147L, 148L, 149L, 222L, 223L, 512L}) { const long h = ffn_tail(items, sms); IS(h >= 0 && 2 * h <= sms && (h == 0 || h == items % sms)); }
