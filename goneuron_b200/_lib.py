@@ -89,7 +89,7 @@ def load():
     L.gn_op_attention.argtypes = [vp] + [C.c_int] * 6 + [f32p] * 10
     i, i64, f = C.c_int, C.c_int64, C.c_float
     L.gn_op_status.argtypes = [vp, vp]
-    heads = C.c_char_p      # gn_heads as packed bytes
+    heads = vp              # const gn_heads*
     qk = [vp, i, i64, i, i, i, f, heads, heads, vp, vp, vp, i, vp]
     L.gn_op_qk_norm_rope.argtypes = qk + [heads, heads, vp]
     L.gn_op_qk_norm_rope_workspace.argtypes = [vp, i64, i, i, i, i64p]

@@ -466,7 +466,7 @@ inline int fg_plain(gn_ctx* ctx, const FgProduct* pr, int n, const FfnCut& cut, 
 
 template <class T, int ACT>
 inline int ffn_forward(gn_ctx* ctx, int64_t M, int D, int F, const void* x, int64_t xs, const void* wg, const void* wu, const void* wd, void* y, int64_t ys, uint8_t* saved, uint8_t* ws, void* stream) {
-  const FfnPlan pl = ffn_plan(M, D, F, ctx->c.sm_count);
+  const FfnPlan& pl = ffn_plan(M, D, F, ctx->c.sm_count);
   void* h = saved ? saved + pl.saved_h : ws + pl.fwd_h;
   if (!saved && M <= FEW_TOKENS) {
     auto few = [&](auto kernel, const void* in, int64_t in_s, const void* a, const void* b, int N, int K, void* out, int64_t os) {
@@ -487,7 +487,7 @@ inline int ffn_forward(gn_ctx* ctx, int64_t M, int D, int F, const void* x, int6
 template <class T, int ACT>
 inline int ffn_backward(gn_ctx* ctx, int64_t M, int D, int F, const void* dy, int64_t dys, const void* x, int64_t xs, const void* wg, const void* wu, const void* wd, const uint8_t* saved,
                         void* dx, int64_t dxs, void* dwg, void* dwu, void* dwd, uint8_t* ws, void* stream) {
-  const FfnPlan pl = ffn_plan(M, D, F, ctx->c.sm_count);
+  const FfnPlan& pl = ffn_plan(M, D, F, ctx->c.sm_count);
   void *dg = ws + pl.bwd_dg, *du = ws + pl.bwd_du; const void* h = saved + pl.saved_h; float* partial = reinterpret_cast<float*>(ws + pl.bwd_partial);
   const FgMatrix none{};
   if (dx || dwg || dwu) {
@@ -528,7 +528,7 @@ int gn_op_gated_ffn_workspace(gn_ctx* ctx, int64_t tokens, int dim, int ff, int 
   using namespace gn;
   if (!ctx || !ctx->alive || !bytes) return fail(GN_ERR_INVALID_ARG, "op_gated_ffn_workspace: bad argument");
   if (const char* e = check_ffn_sizes(tokens, dim, ff)) return fail(GN_ERR_INVALID_ARG, "op_gated_ffn_workspace: %s", e);
-  const FfnPlan pl = ffn_plan(tokens, dim, ff, ctx->c.sm_count);
+  const FfnPlan& pl = ffn_plan(tokens, dim, ff, ctx->c.sm_count);
   *bytes = backward ? pl.bwd : pl.fwd; return GN_OK;
 }
 
