@@ -58,6 +58,7 @@ constexpr int TEACHER_WARPS = 4, TEACHER_TABLE = 2048;
 inline int teacher_smem(int top) { return TEACHER_WARPS * (TEACHER_TABLE * 2 + (top + 3) / 4 * 4 * 9); }      // table, ids, probabilities, flags
 template <class T, bool GRAD>
 __global__ void __launch_bounds__(32 * TEACHER_WARPS) distill_teacher_kernel(const __grid_constant__ DistillParams p) {
+  op_begin();
   extern __shared__ uint4 teacher_smem_raw[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, top4 = (p.top + 3) & ~3; const float c = 1.4426950408889634f / p.temperature;
   uint8_t* own = reinterpret_cast<uint8_t*>(teacher_smem_raw) + warp * (TEACHER_TABLE * 2 + top4 * 9);
@@ -132,6 +133,7 @@ template <class T, int NT, bool GRAD>
 __global__ void __launch_bounds__(NT, 1024 / NT) distill_kernel(const __grid_constant__ DistillParams p, int cl, int per) {
   namespace cg = cooperative_groups;
   constexpr int V = Vec<T>::N, J = DISTILL_ITEMS / V, W = NT / 32, BUF = sizeof(T) == 2 ? 2 : 1;      // J pieces a thread; two rows under way where 16-bit elements leave room for them
+  op_begin();
   extern __shared__ uint4 slots[];                                   // [BUF][J][NT]
   __shared__ MaxSum part[2][W]; __shared__ MaxSum peers[2][8];       // (rows take turns: a warp may be a row ahead of another, never two)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, vocab = (int)p.vocab;
@@ -234,6 +236,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_kernel(const __grid_con
 // A row that does not fit on chip: one block reads it twice.
 template <class T, bool GRAD>
 __global__ void __launch_bounds__(1024) distill_long_kernel(const __grid_constant__ DistillParams p) {
+  op_begin();
   __shared__ MaxSum part[32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5; const float c = 1.4426950408889634f / p.temperature;
   for (long r = blockIdx.x; r < p.rows; r += gridDim.x) {

@@ -16,6 +16,7 @@ namespace gn {
 template <class T, int V>
 __global__ void __launch_bounds__(256) embedding_kernel(const T* __restrict__ table, long table_stride, const void* __restrict__ ids, int index_type, long tokens, long vocab, int dim, float scale,
                                                         T* __restrict__ out, long out_stride) {
+  op_begin();
   const int lane = threadIdx.x & 31; const long warps = (long)gridDim.x * 8;
   for (long i = (long)blockIdx.x * 8 + (threadIdx.x >> 5); i < tokens; i += warps) {
     const int64_t id = load_index(ids, index_type, i); const bool there = id >= 0 && id < vocab;
@@ -69,6 +70,7 @@ struct TileDigit {
 // Few tokens: one block, everything in shared memory.
 constexpr int SORT_SMALL_THREADS = 1024;
 __global__ void __launch_bounds__(SORT_SMALL_THREADS) sort_small_kernel(const void* __restrict__ ids, int index_type, int tokens, long vocab, int passes, unsigned* __restrict__ keys, int* __restrict__ order) {
+  op_begin();
   extern __shared__ unsigned sort_smem[];
   constexpr int W = SORT_SMALL_THREADS / 32;
   unsigned* cnt = sort_smem;                                         // [W][256]
@@ -115,6 +117,7 @@ constexpr int SORT_SMALL_SMEM = (SORT_SMALL_THREADS / 32 * 256 + 2 * SORT_SMALL)
 constexpr int SORT_THREADS = 256;
 template <bool FIRST>
 __global__ void __launch_bounds__(SORT_THREADS) sort_count_kernel(const void* __restrict__ ids, int index_type, const unsigned* __restrict__ keys, long tokens, long vocab, int shift, unsigned* __restrict__ hist) {
+  op_begin();
   __shared__ unsigned cnt[256];
   cnt[threadIdx.x] = 0;
   __syncthreads();
@@ -129,6 +132,7 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_count_kernel(const void* __
 }
 // In place: every count becomes the sum of those before it.  One block.
 __global__ void __launch_bounds__(1024) sort_scan_kernel(unsigned* __restrict__ hist, long n) {
+  op_begin();
   __shared__ unsigned sums[32];
   __shared__ unsigned carry;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -158,6 +162,7 @@ template <bool FIRST>
 __global__ void __launch_bounds__(SORT_THREADS) sort_move_kernel(const void* __restrict__ ids, int index_type, const unsigned* __restrict__ keys, const int* __restrict__ order, long tokens, long vocab, int shift,
                                                                  const unsigned* __restrict__ hist, unsigned* __restrict__ keys_out, int* __restrict__ order_out) {
   constexpr int W = SORT_THREADS / 32, PER = SORT_TILE / SORT_THREADS;      // rows of 32 places of a warp
+  op_begin();
   __shared__ unsigned cnt[W * 256];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const long first = (long)blockIdx.x * SORT_TILE + warp * (PER * 32);
@@ -198,6 +203,7 @@ constexpr int EMB_THREADS = 128, EMB_ZERO_ROWS = 32;
 template <class T, int V>
 __global__ void __launch_bounds__(EMB_THREADS) embedding_sum_kernel(const T* __restrict__ dout, long stride, const unsigned* __restrict__ keys, const int* __restrict__ order, long tokens, long vocab, int dim,
                                                                     float scale, int chunk, long chunks, float* __restrict__ dtable, float* __restrict__ partial) {
+  op_begin();
   const long col = ((long)blockIdx.y * EMB_THREADS + threadIdx.x) * V; const bool in = col < dim;
   auto put = [&](float* row, const float (&v)[V]) {
     if (!in) return;
@@ -269,6 +275,7 @@ __global__ void __launch_bounds__(EMB_THREADS) embedding_sum_kernel(const T* __r
 constexpr int JOIN_COLS = 64;
 template <int V>
 __global__ void __launch_bounds__(4 * JOIN_COLS) embedding_join_kernel(const unsigned* __restrict__ keys, long tokens, long vocab, int dim, int chunk, long chunks, const float* __restrict__ partial, float* __restrict__ dtable) {
+  op_begin();
   __shared__ float red[3][JOIN_COLS * V];
   __shared__ int found;
   const long c = blockIdx.x, end = (c + 1) * chunk;                  // (a last piece has nothing behind it: the launch leaves it out)

@@ -98,6 +98,7 @@ __global__ void __launch_bounds__(FgCfg<BN, KIND>::THREADS, 1) __cluster_dims__(
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t smem0 = smem_u32(smem), rank = cluster_rank(), lead_full0 = cluster_address(full0, 0), lead_tempty0 = cluster_address(tempty0, 0); const unsigned limit = P.spin_limit;
 
+  pdl_launch();
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; s++) { mbar_init(full0 + 8 * s, 1); mbar_init(empty0 + 8 * s, 1); }
     for (int b = 0; b < 2; b++) { mbar_init(tfull0 + 8 * b, 1); mbar_init(tempty0 + 8 * b, 2 * Cfg::EW); }
@@ -114,6 +115,7 @@ __global__ void __launch_bounds__(FgCfg<BN, KIND>::THREADS, 1) __cluster_dims__(
   cluster_sync_all();                                                // the other block's barriers are there
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  pdl_wait();                                                        // set up under the kernel before this one
   auto give_up = [&]() { op_report(OP_TIMEOUT); *abort_flag = 1; __threadfence_block(); };
 
   // Items of this pair, the same in every role of both blocks: its number, + the number of pairs, ...
@@ -327,6 +329,7 @@ __global__ void __launch_bounds__(FgCfg<BN, KIND>::THREADS, 1) __cluster_dims__(
 struct FgReduce { const float* partial; int splits, problems; struct { void* out; long ld; int M, N, tiles_n, tiles; } p[3]; };
 template <class T, int BN>
 __global__ void __launch_bounds__(2 * BN) fg_reduce_kernel(const __grid_constant__ FgReduce R) {
+  op_begin();
   int tile = blockIdx.x >> 3, q = 0; const int quad = blockIdx.x & 7, lane = threadIdx.x & 31, c16 = threadIdx.x >> 5;
   const float4* src = reinterpret_cast<const float4*>(R.partial) + (long)tile * R.splits * (FG_BM * BN / 4) + (quad * (BN / 32) + (c16 >> 1)) * 256 + (c16 & 1) * 128 + lane;
   while (q + 1 < R.problems && tile >= R.p[q].tiles) { tile -= R.p[q].tiles; q++; }
@@ -356,7 +359,7 @@ template <> __device__ __forceinline__ void mma_16x8x16<__nv_bfloat16>(float (&d
 constexpr int FEW_WARPS = 8, FEW_TOKENS = 16;
 // GATE: out[t][n] = act(x w0^T) (x w1^T), else x w0^T.  n in blocks of 16, `cl` blocks of a cluster share the contraction.  NB: blocks of eight tokens.
 template <class T, bool GATE, int NB, int ACT>
-__global__ void __launch_bounds__(32 * FEW_WARPS) fg_few_kernel(const T* __restrict__ x, long x_stride, const T* __restrict__ w0, const T* __restrict__ w1, int tokens, int N, int K, T* __restrict__ out, long out_stride, int cl) {
+__global__ void __launch_bounds__(32 * FEW_WARPS) fg_few_kernel(const T* x, long x_stride, const T* __restrict__ w0, const T* __restrict__ w1, int tokens, int N, int K, T* __restrict__ out, long out_stride, int cl) {
   namespace cg = cooperative_groups;
   constexpr int MATS = GATE ? 2 : 1;
   __shared__ float red[FEW_WARPS][MATS * NB][4][32];
@@ -367,8 +370,8 @@ __global__ void __launch_bounds__(32 * FEW_WARPS) fg_few_kernel(const T* __restr
   const uint4 zero = make_uint4(0, 0, 0, 0);
   constexpr int U = NB == 1 ? 4 : 2;                                 // steps of 32 indices under way
   const int steps = (K + 31) / 32, parts = FEW_WARPS * cl, part = rank * FEW_WARPS + warp, s_end = (int)((long)steps * (part + 1) / parts);
-  for (int s0 = (int)((long)steps * part / parts); s0 < s_end; s0 += U) {
-    uint4 a[U][MATS][2], b[U][NB];
+  uint4 a[U][MATS][2], b[U][NB];
+  auto weights = [&](int s0) {
 #pragma unroll
     for (int i = 0; i < U; i++) {
       const int k = (s0 + i) * 32 + q * 8; const bool in = s0 + i < s_end && k < K;      // (K is a multiple of 8)
@@ -376,8 +379,17 @@ __global__ void __launch_bounds__(32 * FEW_WARPS) fg_few_kernel(const T* __restr
       for (int m = 0; m < MATS; m++)
 #pragma unroll
         for (int r = 0; r < 2; r++) { const int n = n0 + g + 8 * r; a[i][m][r] = in && n < N ? __ldcs(reinterpret_cast<const uint4*>((m ? w1 : w0) + (long)n * K + k)) : zero; }
+    }
+  };
+  int s0 = (int)((long)steps * part / parts);
+  // The second launch fetches its first weights while the first one still runs.  Whatever wrote them has finished: the first launch lets the second in only behind its own wait.
+  if constexpr (GATE) { pdl_wait(); pdl_launch(); weights(s0); } else { pdl_launch(); weights(s0); pdl_wait(); }
+  for (; s0 < s_end; s0 += U) {
 #pragma unroll
-      for (int j = 0; j < NB; j++) { const int t = 8 * j + g; b[i][j] = in && t < tokens ? __ldg(reinterpret_cast<const uint4*>(x + t * x_stride + k)) : zero; }
+    for (int i = 0; i < U; i++) {
+      const int k = (s0 + i) * 32 + q * 8; const bool in = s0 + i < s_end && k < K;
+#pragma unroll
+      for (int j = 0; j < NB; j++) { const int t = 8 * j + g; b[i][j] = in && t < tokens ? *reinterpret_cast<const uint4*>(x + t * x_stride + k) : zero; }
     }
 #pragma unroll
     for (int i = 0; i < U; i++)
@@ -388,6 +400,7 @@ __global__ void __launch_bounds__(32 * FEW_WARPS) fg_few_kernel(const T* __restr
           mma_16x8x16<T>(d[m][j], a[i][m][0].x, a[i][m][1].x, a[i][m][0].y, a[i][m][1].y, b[i][j].x, b[i][j].y);
           mma_16x8x16<T>(d[m][j], a[i][m][0].z, a[i][m][1].z, a[i][m][0].w, a[i][m][1].w, b[i][j].z, b[i][j].w);
         }
+    if (s0 + U < s_end) weights(s0 + U);
   }
 #pragma unroll
   for (int m = 0; m < MATS; m++)

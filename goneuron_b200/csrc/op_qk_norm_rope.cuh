@@ -90,6 +90,7 @@ constexpr int QK_THREADS = 256;
 template <class T, int G, bool BWD>
 __global__ void __launch_bounds__(QK_THREADS, QK_PER_SM) qk_vec_kernel(const __grid_constant__ QkParams p) {
   constexpr int V = Vec<T>::N, GROUPS = QK_THREADS / G, HB = BWD ? QK_HEADS_BWD : QK_HEADS_FWD;
+  op_begin();
   extern __shared__ float4 qk_smem[];
   float* cs = reinterpret_cast<float*>(qk_smem);
   __shared__ float red[BWD ? QK_THREADS / 32 * G * 2 * V : 1];
@@ -197,6 +198,7 @@ __global__ void __launch_bounds__(QK_THREADS, QK_PER_SM) qk_vec_kernel(const __g
 constexpr int QK_ROW_WARPS = 4;
 template <class T, bool BWD>
 __global__ void __launch_bounds__(32 * QK_ROW_WARPS) qk_rows_kernel(const __grid_constant__ QkParams p) {
+  op_begin();
   extern __shared__ float4 qk_smem[];
   float* cs = reinterpret_cast<float*>(qk_smem);
   const int half = p.rot >> 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -268,6 +270,7 @@ __global__ void __launch_bounds__(32 * QK_ROW_WARPS) qk_rows_kernel(const __grid
 
 // dgain[e] = sum of the blocks' partial sums: 32 threads a column, each a run of neighbouring blocks, in order
 __global__ void __launch_bounds__(1024) qk_gain_kernel(const float* __restrict__ partial, int blocks, int head, float* __restrict__ dq, float* __restrict__ dk) {
+  op_begin();
   __shared__ float red[32][33];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, col = blockIdx.x * 32 + lane, per = (blocks + 31) / 32;
   float v = 0.f;

@@ -6,7 +6,7 @@
 #include "op_gated_ffn.cuh"
 
 namespace gn {
-__global__ void op_status_clear_kernel(int bits) { atomicAnd(&op_status_word, ~bits); }
+__global__ void op_status_clear_kernel(int bits) { op_begin(); atomicAnd(&op_status_word, ~bits); }
 }  // namespace gn
 
 extern "C" int gn_op_status(gn_ctx* ctx, void* stream) {
