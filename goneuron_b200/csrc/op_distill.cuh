@@ -8,11 +8,11 @@
 // come before the factor: logits at the type's lowest value stay finite.
 //
 // Bound by memory: a row is read once and its gradient written once.  One launch forms what the teacher's few entries come to, a warp a row, so that no long
-// row waits for their chain of dependent loads; the second streams the rows.  A row stays on chip there, 32 elements a thread in registers as float32 exponentials (one exponential
-// an element: with two the special-function units bound it, 2 x 11 an SM and cycle at full bandwidth against the 16 they give).  While a row is in registers the same
-// thread's asynchronous copies fetch its elements of the next one, into slots of shared memory that no other thread touches, so that the only barrier
-// of a row is the one at which the sums meet.  A row that is too long for 512 threads is spread over a cluster of blocks, two of which share an SM and overlap each
-// other's barriers.  Each block writes q for all of its elements; where the teacher has entries q - p is written over it, behind the next row's barrier.
+// row waits for their chain of dependent loads; the second streams the rows.  A row, or a block's part of it, lies in shared memory; every thread copies there, sums over and writes back its own
+// 16-byte pieces of it, so that the only barrier of a row is the one at which the warps' sums meet, and the copies of a thread's next row are under way as soon as it has written this one.
+// Blocks of an SM (three for rows of 64 KB) overlap each other's phases.  (Rows held as exponentials in registers, 1024 threads a row: 26 instructions an element, most of them per row
+// and thread, 2.4 TB/s.)  A row of more than 72 KB is spread over a cluster of blocks, whose barrier is then the cluster's.
+// Each block writes q for all of its elements; where the teacher has entries q - p is written over it, behind the next row's barrier.
 #pragma once
 #include "device_ops.cuh"
 
@@ -51,40 +51,57 @@ __device__ __forceinline__ int teacher_entry(const DistillParams& p, long row, i
   t = there ? __ldg(p.top_logits + row * p.top + k) : -INFINITY;
   return there ? (int)id : -1;
 }
-// A warp a row.  With a gradient the entries' ids, probabilities and student values are kept for the second launch; of entries with the same id the first keeps all of their
-// probability and the others become -1.  Such entries are rare and found by a table: every entry writes its number at its id's place, and whoever finds another's number there, or is found by
-// another of the same id, looks through the row.
+// A warp a row, 128 entries of it at a time in registers.  With a gradient the entries' ids, probabilities and student values are kept for the second launch; of entries with the same id the
+// first keeps all of their probability and the others become -1.  Such entries are rare and found by a table: every entry writes its number at its id's place, and whoever finds
+// another's number there, or is found by another of the same id, looks through the row.
 constexpr int TEACHER_WARPS = 4, TEACHER_TABLE = 2048;
-inline int teacher_smem(int top) { return TEACHER_WARPS * (TEACHER_TABLE * 2 + (top + 3) / 4 * 4 * 9); }      // table, ids, probabilities, flags
+inline int teacher_smem(int top) { return TEACHER_WARPS * (TEACHER_TABLE * 2 + (top + 15) / 16 * 16 * 9); }      // table, ids, probabilities, flags
 template <class T, bool GRAD>
 __global__ void __launch_bounds__(32 * TEACHER_WARPS) distill_teacher_kernel(const __grid_constant__ DistillParams p) {
-  op_begin();
+  pdl_wait(); pdl_launch();                                          // (in this order: the launch behind fetches logits before this one has finished)
   extern __shared__ uint4 teacher_smem_raw[];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, top4 = (p.top + 3) & ~3; const float c = 1.4426950408889634f / p.temperature;
-  uint8_t* own = reinterpret_cast<uint8_t*>(teacher_smem_raw) + warp * (TEACHER_TABLE * 2 + top4 * 9);
-  int* id_of = reinterpret_cast<int*>(own); float* prob_of = reinterpret_cast<float*>(id_of + top4);
-  unsigned short* table = reinterpret_cast<unsigned short*>(prob_of + top4); uint8_t* look = reinterpret_cast<uint8_t*>(table + TEACHER_TABLE);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, top16 = (p.top + 15) & ~15; const float c = 1.4426950408889634f / p.temperature;
+  uint8_t* own = reinterpret_cast<uint8_t*>(teacher_smem_raw) + warp * (TEACHER_TABLE * 2 + top16 * 9);
+  int* id_of = reinterpret_cast<int*>(own); float* prob_of = reinterpret_cast<float*>(id_of + top16);
+  unsigned short* table = reinterpret_cast<unsigned short*>(prob_of + top16); uint8_t* look = reinterpret_cast<uint8_t*>(table + TEACHER_TABLE);
   const long row = (long)blockIdx.x * TEACHER_WARPS + warp;
   if (row >= p.rows) return;
   const float w = p.weight ? __ldg(p.weight + row) : 1.f;
   Teacher out{0.f, 0.f, 0.f, 0.f};
   if (w != 0.f) {
     const T* logits = static_cast<const T*>(p.logits) + row * p.stride;
+    constexpr int E = 4;
+    int id[E]; float t[E];
+    auto load = [&](int k0) {
+#pragma unroll
+      for (int e = 0; e < E; e++) { const int k = k0 + 32 * e + lane; id[e] = -1; t[e] = -INFINITY; if (k < p.top) id[e] = teacher_entry(p, row, k, t[e]); }
+    };
     MaxSum v{-INFINITY, 0.f};
-    for (int k = lane; k < p.top; k += 32) { float t; teacher_entry(p, row, k, t); v = join(v, MaxSum{t, t == -INFINITY ? 0.f : 1.f}, c); }
+    for (int k0 = 0; k0 < p.top; k0 += 32 * E) {
+      load(k0);
+#pragma unroll
+      for (int e = 0; e < E; e++) v = join(v, MaxSum{t[e], t[e] == -INFINITY ? 0.f : 1.f}, c);
+    }
     v = warp_join(v, c);
     const bool some = !(v.m == -INFINITY && v.s == 0.f); const Norm n = norm_of(v);
     float d = 0.f, r = -INFINITY, weight = 0.f;                      // d: relative to this lane's r so far; weight: the probability that it holds
-    for (int k = lane; k < p.top; k += 32) {
-      float t; const int id = teacher_entry(p, row, k, t);
-      const float pk = !some || t == -INFINITY ? 0.f : exp2f((t - n.m) * c - n.l), s = id >= 0 ? to_f32(logits[id]) : 0.f;
-      if (pk != 0.f) {                                               // (an entry without weight says nothing, whatever the student has there)
-        if (s > r) { if (weight != 0.f) d += weight * (s - r); r = s; }      // sum of p (r - s) moves with r
-        d += pk * ((t - n.m) - (s - (r == -INFINITY ? 0.f : r))); weight += pk;
-      }
-      if constexpr (GRAD) {
-        p.stud[row * p.top + k] = s; id_of[k] = id; prob_of[k] = pk; look[k] = 0;
-        if (id >= 0) table[id & (TEACHER_TABLE - 1)] = (unsigned short)k;
+    for (int k0 = 0; k0 < p.top; k0 += 32 * E) {
+      if (p.top > 32 * E) load(k0);
+      float s[E];
+#pragma unroll
+      for (int e = 0; e < E; e++) s[e] = id[e] >= 0 ? to_f32(logits[id[e]]) : 0.f;
+#pragma unroll
+      for (int e = 0; e < E; e++) {
+        const int k = k0 + 32 * e + lane;
+        const float pk = !some || t[e] == -INFINITY ? 0.f : exp2f((t[e] - n.m) * c - n.l);
+        if (pk != 0.f) {                                             // (an entry without weight says nothing, whatever the student has there)
+          if (s[e] > r) { if (weight != 0.f) d += weight * (s[e] - r); r = s[e]; }      // sum of p (r - s) moves with r
+          d += pk * ((t[e] - n.m) - (s[e] - (r == -INFINITY ? 0.f : r))); weight += pk;
+        }
+        if constexpr (GRAD) {
+          if (k < top16) { id_of[k] = k < p.top ? id[e] : -2; prob_of[k] = pk; look[k] = 0; }
+          if (k < p.top) { p.stud[row * p.top + k] = s[e]; if (id[e] >= 0) table[id[e] & (TEACHER_TABLE - 1)] = (unsigned short)k; }
+        }
       }
     }
     const float top = warp_max(r), ref = top == -INFINITY ? 0.f : top;
@@ -93,19 +110,24 @@ __global__ void __launch_bounds__(32 * TEACHER_WARPS) distill_teacher_kernel(con
     if constexpr (GRAD) {
       __syncwarp();
       for (int k = lane; k < p.top; k += 32) {
-        const int id = id_of[k];
-        if (id < 0) continue;
-        const int found = table[id & (TEACHER_TABLE - 1)];
-        if (found != k) { look[k] = 1; if (id_of[found] == id) look[found] = 1; }
+        const int i = id_of[k];
+        if (i < 0) continue;
+        const int found = table[i & (TEACHER_TABLE - 1)];
+        if (found != k) { look[k] = 1; if (id_of[found] == i) look[found] = 1; }
       }
       __syncwarp();
       for (int k = lane; k < p.top; k += 32) {
-        int id = id_of[k]; float pk = prob_of[k];
+        int i = id_of[k]; float pk = prob_of[k];
         if (look[k]) {
-          pk = 0.f;
-          for (int f = 0; f < p.top; f++) if (id_of[f] == id) { if (f < k) { id = -1; break; } pk += prob_of[f]; }
+          const int mine = i; pk = 0.f;
+          for (int f = 0; f < top16; f += 4) {
+            const int4 o = *reinterpret_cast<const int4*>(id_of + f);
+            if (o.x != mine && o.y != mine && o.z != mine && o.w != mine) continue;
+            const int q[4] = {o.x, o.y, o.z, o.w};
+            for (int l = 0; l < 4; l++) if (q[l] == mine) { if (f + l < k) i = -1; pk += prob_of[f + l]; }
+          }
         }
-        p.id[row * p.top + k] = id; p.prob[row * p.top + k] = pk;
+        p.id[row * p.top + k] = i; p.prob[row * p.top + k] = pk;
       }
     }
   }
@@ -115,120 +137,163 @@ __global__ void __launch_bounds__(32 * TEACHER_WARPS) distill_teacher_kernel(con
 __device__ __forceinline__ float distill_loss(const Teacher& t, Norm n, float tau) { return t.w != 0.f ? t.w * tau * (t.d + (n.m - t.r) + tau * 0.69314718055994531f * (n.l - t.l)) : 0.f; }
 // q - p where the teacher has entries of row r, over what is there, for ids in [lo, hi)
 template <class T>
-__device__ __forceinline__ void distill_entries(const DistillParams& p, long r, float w, Norm n, float c, long lo, long hi) {
-  if (w == 0.f) return;
+__device__ __forceinline__ void distill_entry(const DistillParams& p, T* out, int id, float prob, float stud, float w, Norm n, float c, long lo, long hi) {
+  if (id >= 0 && id >= lo && id < hi) out[id] = from_f32<T>(w * p.temperature * (ex2((stud - n.m) * c - n.l) - prob));
+}
+template <class T>
+__device__ __forceinline__ void distill_entries(const DistillParams& p, long r, int first, float w, Norm n, float c, long lo, long hi) {
   T* out = static_cast<T*>(p.dlogits) + r * p.dstride;
-  for (int e = threadIdx.x; e < p.top; e += blockDim.x) {
-    const int id = p.id[r * p.top + e];
-    if (id >= lo && id < hi && id >= 0) out[id] = from_f32<T>(w * p.temperature * (ex2((p.stud[r * p.top + e] - n.m) * c - n.l) - p.prob[r * p.top + e]));
-  }
+  for (int e = first + threadIdx.x; e < p.top; e += blockDim.x) { const long i = r * p.top + e; distill_entry<T>(p, out, p.id[i], p.prob[i], p.stud[i], w, n, c, lo, hi); }
 }
 
 // Elements of a row from the 16-byte boundary at or before its first one.
 template <class T> __device__ __forceinline__ int row_lead(const T* row) { return (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T)); }
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
+// Largest element of a piece (a NaN counts as none)
+template <class T> __device__ __forceinline__ float piece_max(const uint4& u) {
+  if constexpr (sizeof(T) == 4) return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)), fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
+  else {
+    using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    auto as = [](uint32_t v) { return *reinterpret_cast<const T2*>(&v); };
+    const T2 m = __hmax2(__hmax2(as(u.x), as(u.y)), __hmax2(as(u.z), as(u.w)));
+    return fmaxf(to_f32(m.x), to_f32(m.y));
+  }
+}
 
-// NT threads of `cl` blocks on a row, `per` 16-byte pieces of it (counted from its 16-byte boundary) for each block; BUF rows of slots.
-template <class T, int NT, bool GRAD>
-__global__ void __launch_bounds__(NT, 1024 / NT) distill_kernel(const __grid_constant__ DistillParams p, int cl, int per) {
+// two floats an instruction
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r; asm("{\n.reg .b64 x, y;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nadd.rn.f32x2 x, x, y;\nmov.b64 {%0, %1}, x;\n}" : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y)); return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r; asm("{\n.reg .b64 x, y;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nmul.rn.f32x2 x, x, y;\nmov.b64 {%0, %1}, x;\n}" : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y)); return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r; asm("{\n.reg .b64 x, y, z;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nmov.b64 z, {%6, %7};\nfma.rn.f32x2 x, x, y, z;\nmov.b64 {%0, %1}, x;\n}" : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y)); return r;
+}
+// element pairs of a piece
+template <class T> __device__ __forceinline__ float2 piece_pair(const uint4& u, int i) {      // i: a constant once unrolled
+  if constexpr (sizeof(T) == 4) return i == 0 ? make_float2(__uint_as_float(u.x), __uint_as_float(u.y)) : make_float2(__uint_as_float(u.z), __uint_as_float(u.w));
+  else return unpack2(i == 0 ? u.x : i == 1 ? u.y : i == 2 ? u.z : u.w, T());
+}
+
+// `cl` blocks on a row, `per` 16-byte pieces of it (counted from its 16-byte boundary) for each.  WHOLE: every row and its gradient begin on such a boundary and fill their pieces.
+template <class T, bool GRAD, bool WHOLE>
+__global__ void __launch_bounds__(DISTILL_THREADS, 3) distill_kernel(const __grid_constant__ DistillParams p, int cl, int per) {
   namespace cg = cooperative_groups;
-  constexpr int V = Vec<T>::N, J = DISTILL_ITEMS / V, W = NT / 32, BUF = sizeof(T) == 2 ? 2 : 1;      // J pieces a thread; two rows under way where 16-bit elements leave room for them
-  op_begin();
-  extern __shared__ uint4 slots[];                                   // [BUF][J][NT]
-  __shared__ MaxSum part[2][W]; __shared__ MaxSum peers[2][8];       // (rows take turns: a warp may be a row ahead of another, never two)
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, vocab = (int)p.vocab;
+  constexpr int V = Vec<T>::N;
+  extern __shared__ uint4 slots[];                                   // [per], rounded up to whole turns of all threads: -inf behind
+  __shared__ MaxSum part[2][8 * DISTILL_THREADS / 32];               // sums of all warps of the cluster (rows take turns: a warp may be a row ahead of another, never two)
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nt = blockDim.x, warps = nt >> 5, vocab = (int)p.vocab;
   const int rank = cl > 1 ? (int)(blockIdx.x % cl) : 0; const long row0 = blockIdx.x / cl, step = gridDim.x / cl;
   const float c = 1.4426950408889634f / p.temperature;
-  const uint32_t slot0 = (uint32_t)__cvta_generic_to_shared(slots) + tid * 16;
   const int at = rank * per;                                         // this block's pieces: [at, at + per), as far as the row goes
+  pdl_launch();
+  if (cl > 1) cg::this_cluster().sync();                             // (all blocks are there before one writes into another)
   auto row_of = [&](long r) { return static_cast<const T*>(p.logits) + r * p.stride; };
-  auto weight_of = [&](long r) { return r < p.rows ? __ldg(&p.teach[r].w) : 0.f; };
-  // copies of this thread's pieces of row r into buffer b; pieces that the row does not fill are put together element by element, -inf where it has none
-  auto fetch = [&](long r, float w, int b) {
+  auto lead_of = [&](long r) { return WHOLE ? 0 : row_lead(row_of(r)); };
+  auto count = [&](int lead) { return min(per, (lead + vocab + V - 1) / V - at); };      // pieces of this block
+  const int n_whole = (per + nt - 1) / nt * nt;                      // places of all threads' turns
+  auto weight_of = [&](long r) { return r >= p.rows ? 0.f : p.weight ? __ldg(p.weight + r) : 1.f; };
+  // copies of this thread's pieces of row r; pieces that the row does not fill are put together element by element, -inf where it has none
+  const uint32_t slot0 = (uint32_t)__cvta_generic_to_shared(slots), none = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+  const uint4 nothing = make_uint4(none, none, none, none);          // -inf
+  auto fetch = [&](long r, float w) {
     if (w != 0.f) {
-      const T* row = row_of(r); const int lead = row_lead(row);
+      const T* row = row_of(r); const int lead = lead_of(r), n = count(lead);
+      for (int i = tid; i < (WHOLE ? n : n_whole); i += nt) {        // (WHOLE: what lies behind is the same for every row)
+        const int e = (at + i) * V - lead;                           // first element
+        if (!WHOLE && i >= n) slots[i] = nothing;
+        else if (WHOLE || (e >= 0 && e + V <= vocab)) cp16(slot0 + i * 16, row + e);
+        else {
+          T* q = reinterpret_cast<T*>(slots + i);
 #pragma unroll
-      for (int j = 0; j < J; j++) {
-        const int i = j * NT + tid, e = (at + i) * V - lead;         // e: first element
-        if (i < per && e < vocab) {
-          if (e >= 0 && e + V <= vocab) cp16(slot0 + (b * J + j) * NT * 16, row + e);
-          else {
-            T* q = reinterpret_cast<T*>(slots + (b * J + j) * NT + tid);
-#pragma unroll
-            for (int l = 0; l < V; l++) q[l] = e + l >= 0 && e + l < vocab ? row[e + l] : from_f32<T>(-INFINITY);
-          }
+          for (int l = 0; l < V; l++) q[l] = e + l >= 0 && e + l < vocab ? row[e + l] : from_f32<T>(-INFINITY);
         }
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
 
-  for (int b = 0; b < BUF; b++) fetch(row0 + b * step, weight_of(row0 + b * step), b);
-  float ahead = weight_of(row0 + BUF * step);                        // weight of the row that is fetched next
-  int b = 0, par = 0; long done = -1; float done_w = 0.f; Norm done_n{0.f, 0.f};
-  for (long r = row0; r < p.rows; r += step) {
-    const T* row = row_of(r); const int lead = row_lead(row);
-    const Teacher t = p.teach[r]; const bool on = t.w != 0.f;
-    if constexpr (BUF == 1) asm volatile("cp.async.wait_group 0;" ::: "memory"); else asm volatile("cp.async.wait_group 1;" ::: "memory");
-    float x[DISTILL_ITEMS]; float m = -INFINITY;
+  if (WHOLE) for (int i = tid; i < n_whole; i += nt) if (i >= count(0)) slots[i] = nothing;
+  float w_now = weight_of(row0); fetch(row0, w_now);
+  pdl_wait();                                                        // for the teacher's launch
+  int turn = 0; long done = -1; float done_w = 0.f; Norm done_n{0.f, 0.f};
+  for (long r = row0; r < p.rows; r += step, turn ^= 1) {
+    const Teacher t = p.teach[r]; const float w_next = weight_of(r + step); const int lead = lead_of(r), n = count(lead); const bool on = t.w != 0.f;
+    // the entries of the row before, one a thread
+    int id = -1; float prob = 0.f, stud = 0.f;
+    if constexpr (GRAD) { if (done_w != 0.f && tid < p.top) { const long i = done * p.top + tid; id = p.id[i]; prob = p.prob[i]; stud = p.stud[i]; } }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    float m = -INFINITY, s = 0.f;
+    if (w_now != 0.f) {
+      float2 sum = make_float2(0.f, 0.f);
+#pragma unroll 2
+      for (int i = tid; i < n_whole; i += nt) {
+        const uint4 u = slots[i];
+        const float top = fmaxf(m, piece_max<T>(u));
+        if (top > m) { const float g = ex2((m - top) * c); sum = mul2(sum, make_float2(g, g)); m = top; }      // (rarely behind the first pieces)
+        const float ref = m == -INFINITY ? 0.f : m; const float2 r2 = make_float2(-ref, -ref), c2 = make_float2(c, c);
 #pragma unroll
-    for (int j = 0; j < J; j++) {
-      float v[V]; const int i = j * NT + tid;
-      if (on && i < per && (at + i) * V - lead < vocab) unpack<T>(slots[(b * J + j) * NT + tid], v);
-      else {
-#pragma unroll
-        for (int l = 0; l < V; l++) v[l] = -INFINITY;
+        for (int l = 0; l < V / 2; l++) { const float2 x = mul2(add2(piece_pair<T>(u, l), r2), c2); sum = add2(sum, make_float2(ex2(x.x), ex2(x.y))); }
       }
-#pragma unroll
-      for (int l = 0; l < V; l++) { x[j * V + l] = v[l]; m = fmaxf(m, v[l]); }
+      s = sum.x + sum.y;
     }
-    fetch(r + BUF * step, ahead, b);                                 // (the values have been read: m depends on them all)
-    ahead = weight_of(r + (BUF + 1) * step);
-    m = warp_max(m);
-    const float ref = m == -INFINITY ? 0.f : m;
-    float s = 0.f;
-#pragma unroll
-    for (int j = 0; j < DISTILL_ITEMS; j++) { x[j] = ex2((x[j] - ref) * c); s += x[j]; }
-    s = warp_sum(s);
-    if (lane == 0) part[par][warp] = MaxSum{m, s};
-    __syncthreads();
     auto meet = [&](MaxSum v) {
       const float top = warp_max(v.m), to = top == -INFINITY ? 0.f : top;
       return MaxSum{top, warp_sum(v.s * ex2((v.m - to) * c))};
     };
-    MaxSum v = meet(lane < W ? part[par][lane] : MaxSum{-INFINITY, 0.f});
-    if (cl > 1) {
+    MaxSum v = meet(MaxSum{m, s});
+    if (cl == 1) {
+      if (lane == 0) part[turn][warp] = v;
+      __syncthreads();
+    } else {
       cg::cluster_group cluster = cg::this_cluster();
-      if (tid < cl) *cluster.map_shared_rank(&peers[par][rank], tid) = v;
+      if (lane < cl) *cluster.map_shared_rank(&part[turn][rank * warps + warp], lane) = v;
       cluster.sync();
-      v = meet(lane < cl ? peers[par][lane] : MaxSum{-INFINITY, 0.f});
     }
-    const Norm n = norm_of(v);
-    if (tid == 0 && rank == 0) p.loss[r] = distill_loss(t, n, p.temperature);
+    v = MaxSum{-INFINITY, 0.f};
+    for (int k = lane; k < cl * warps; k += 32) v = join(v, part[turn][k], c);
+    const Norm nm = norm_of(meet(v));
+    if (tid == 0 && rank == 0) p.loss[r] = distill_loss(t, nm, p.temperature);
     if constexpr (GRAD) {
-      const float f = !on || (m == -INFINITY && n.m > -INFINITY) ? 0.f : t.w * p.temperature * ex2((m - n.m) * c - n.l);
-      T* out = static_cast<T*>(p.dlogits) + r * p.dstride; const bool same = row_lead(out) == lead;
-#pragma unroll
-      for (int j = 0; j < J; j++) {
-        const int i = j * NT + tid, e = (at + i) * V - lead;
-        if (i >= per || e >= vocab) continue;
-        float y[V];
-#pragma unroll
-        for (int l = 0; l < V; l++) y[l] = on ? x[j * V + l] * f : 0.f;
-        if (same && e >= 0 && e + V <= vocab) *reinterpret_cast<uint4*>(out + e) = pack<T>(y);
+      const float f = t.w * p.temperature;
+      T* out = static_cast<T*>(p.dlogits) + r * p.dstride; const bool same = WHOLE || row_lead(out) == lead;
+      auto put = [&](int i, const float (&y)[V]) {
+        const int e = (at + i) * V - lead;
+        if (WHOLE || (same && e >= 0 && e + V <= vocab)) *reinterpret_cast<uint4*>(out + e) = pack<T>(y);
         else {
 #pragma unroll
           for (int l = 0; l < V; l++) if (e + l >= 0 && e + l < vocab) out[e + l] = from_f32<T>(y[l]);
         }
+      };
+      if (on) {
+        const float2 m2 = make_float2(-nm.m, -nm.m), c2 = make_float2(c, c), l2 = make_float2(-nm.l, -nm.l), f2 = make_float2(f, f);
+#pragma unroll 2
+        for (int i = tid; i < n; i += nt) {
+          const uint4 u = slots[i]; float y[V];
+#pragma unroll
+          for (int l = 0; l < V / 2; l++) { const float2 x = fma2(add2(piece_pair<T>(u, l), m2), c2, l2), q = mul2(make_float2(ex2(x.x), ex2(x.y)), f2); y[2 * l] = q.x; y[2 * l + 1] = q.y; }
+          put(i, y);
+        }
+      } else {
+        float y[V] = {};
+        for (int i = tid; i < n; i += nt) put(i, y);
       }
-      if (done >= 0) { const int l0 = row_lead(row_of(done)); distill_entries<T>(p, done, done_w, done_n, c, (long)at * V - l0, (long)(at + per) * V - l0); }
-      done = r; done_w = t.w; done_n = n;
     }
-    par ^= 1; if (++b == BUF) b = 0;
+    fetch(r + step, w_next);                                         // (this thread has read its pieces)
+    w_now = w_next;
+    if constexpr (GRAD) {
+      if (done_w != 0.f) {
+        const long lo = (long)at * V - lead_of(done);
+        distill_entry<T>(p, static_cast<T*>(p.dlogits) + done * p.dstride, id, prob, stud, done_w, done_n, c, lo, lo + (long)per * V);
+        distill_entries<T>(p, done, nt, done_w, done_n, c, lo, lo + (long)per * V);
+      }
+      done = r; done_w = t.w; done_n = nm;
+    }
   }
   if constexpr (GRAD) {
     __syncthreads();
-    if (done >= 0) { const int l0 = row_lead(row_of(done)); distill_entries<T>(p, done, done_w, done_n, c, (long)at * V - l0, (long)(at + per) * V - l0); }
+    if (done_w != 0.f) { const long lo = (long)at * V - lead_of(done); distill_entries<T>(p, done, 0, done_w, done_n, c, lo, lo + (long)per * V); }
   }
   if (cl > 1) cg::this_cluster().sync();                             // (no block leaves while another may still write into it)
 }
@@ -261,7 +326,7 @@ __global__ void __launch_bounds__(1024) distill_long_kernel(const __grid_constan
       T* out = static_cast<T*>(p.dlogits) + r * p.dstride;
       for (long e = tid; e < p.vocab; e += 1024) out[e] = from_f32<T>(on ? t.w * p.temperature * ex2((to_f32(row[e]) - n.m) * c - n.l) : 0.f);
       __syncthreads();
-      distill_entries<T>(p, r, t.w, n, c, 0, p.vocab);
+      if (on) distill_entries<T>(p, r, 0, t.w, n, c, 0, p.vocab);
     }
     __syncthreads();
   }
@@ -269,16 +334,18 @@ __global__ void __launch_bounds__(1024) distill_long_kernel(const __grid_constan
 
 template <class T, bool GRAD>
 inline int distill_launch(gn_ctx* ctx, const DistillParams& p, void* stream) {
-  const int sms = ctx->c.sm_count; const DistillPlan pl = distill_plan(p.rows, p.vocab, sms);
+  const int sms = ctx->c.sm_count; const DistillPlan pl = distill_plan(p.rows, p.vocab, (int)sizeof(T), sms);
   const int tsmem = teacher_smem(GRAD ? p.top : 0);
   if (tsmem > 48 * 1024) GN_TRY(op_smem("distill_teacher", distill_teacher_kernel<T, GRAD>, tsmem));
   GN_TRY(op_launch("distill_teacher", stream, distill_teacher_kernel<T, GRAD>, dim3(cdiv(p.rows, TEACHER_WARPS)), dim3(32 * TEACHER_WARPS), tsmem, 0, p));
   if (pl.cluster == 0) return op_launch("distill_long", stream, distill_long_kernel<T, GRAD>, dim3((unsigned)std::min<int64_t>(p.rows, 2L * sms)), dim3(1024), 0, 0, p);
-  const int V = 16 / (int)sizeof(T), smem = (sizeof(T) == 2 ? 2 : 1) * pl.threads * DISTILL_ITEMS * (int)sizeof(T);      // 64 KB for 512 threads
-  const int per = (int)ceil_div(ceil_div(p.vocab + V - 1, V), pl.cluster);
-  const dim3 grid((unsigned)(std::min<int64_t>(p.rows, std::max<int64_t>(1, (int64_t)sms * (1024 / pl.threads) / pl.cluster)) * pl.cluster));
-  auto go = [&](auto kernel) { if (smem > 48 * 1024) GN_TRY(op_smem("distill", kernel, smem)); return op_launch("distill", stream, kernel, grid, dim3(pl.threads), smem, pl.cluster, p, pl.cluster, per); };
-  return pl.threads == 1024 ? go(distill_kernel<T, 1024, GRAD>) : pl.threads == 512 ? go(distill_kernel<T, 512, GRAD>) : pl.threads == 256 ? go(distill_kernel<T, 256, GRAD>) : go(distill_kernel<T, 64, GRAD>);
+  constexpr int V = Vec<T>::N;
+  const bool whole = p.vocab % V == 0 && p.stride % V == 0 && aligned_to(p.logits, 16) && (!GRAD || (p.dstride % V == 0 && aligned_to(p.dlogits, 16)));
+  const int smem = (int)round_up(pl.per, pl.threads) * 16;
+  const int64_t per_sm = std::max<int64_t>(1, std::min<int64_t>({2048 / pl.threads, 32, 220 * 1024 / (smem + 3 * 1024)}));
+  const dim3 grid((unsigned)(std::min<int64_t>(p.rows, std::max<int64_t>(1, (int64_t)sms * per_sm / pl.cluster)) * pl.cluster));
+  auto go = [&](auto kernel) { if (smem > 40 * 1024) GN_TRY(op_smem("distill", kernel, smem)); return op_launch("distill", stream, kernel, grid, dim3(pl.threads), smem, pl.cluster, p, pl.cluster, pl.per); };
+  return whole ? go(distill_kernel<T, GRAD, true>) : go(distill_kernel<T, GRAD, false>);
 }
 
 }  // namespace gn

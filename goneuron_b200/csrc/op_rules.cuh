@@ -91,20 +91,18 @@ inline const char* check_distill(int dtype, int64_t rows, int64_t vocab, int top
   if (dlogits && dlogits == logits && rows > 1 && row_stride != drow_stride) return "in place, both strides have to be the same";
   return nullptr;
 }
-// A row is kept on chip: `threads` threads of each of `cluster` blocks hold DISTILL_ITEMS elements each in registers.  cluster 0: the row does not fit, and is
-// read again instead.  512 threads at most as long as eight blocks hold the row: two blocks of an SM overlap each other's barriers.  Few rows are cut further, so that they fill the
-// multiprocessors, down to a thousand elements per block.
-constexpr int DISTILL_ITEMS = 32;
-struct DistillPlan { int cluster, threads; };
-inline DistillPlan distill_plan(int64_t rows, int64_t vocab, int sms) {
-  const int64_t slack = 16;                                          // a row may begin inside a 16-byte piece, and blocks take whole pieces
-  auto fits = [&](int c, int threads) { return ceil_div(vocab, c) + slack <= (int64_t)threads * DISTILL_ITEMS; };
+// A row is kept in the shared memory of `cluster` blocks, `per` 16-byte pieces in each, some eight of them a thread.  cluster 0: it does not fit and is read again instead.  Parts of 72 KB leave room
+// for three blocks on a multiprocessor, which overlap each other's phases.  Few rows are cut further, so that they fill the multiprocessors, down to two thousand elements per block.
+constexpr int DISTILL_THREADS = 512, DISTILL_PART = 72 * 1024, DISTILL_PART_MOST = 200 * 1024;
+struct DistillPlan { int cluster, threads, per; };
+inline DistillPlan distill_plan(int64_t rows, int64_t vocab, int size, int sms) {
+  const int64_t v = 16 / size, pieces = ceil_div(vocab + v - 1, v);  // (a row may begin inside a piece)
   int c = 1;
-  while (c < 8 && !fits(c, 512)) c *= 2;
-  if (!fits(c, 1024)) return {0, 1024};
-  while (c < 8 && rows * c * 2 <= sms && vocab >= 2048L * c) c *= 2;
-  for (int threads : {64, 256, 512}) if (fits(c, threads)) return {c, threads};
-  return {c, 1024};
+  while (c < 8 && ceil_div(pieces, c) * 16 > DISTILL_PART) c *= 2;
+  if (ceil_div(pieces, c) * 16 > DISTILL_PART_MOST) return {0, 1024, 0};
+  while (c < 8 && rows * c * 2 <= sms && vocab >= 4096L * c) c *= 2;
+  const int64_t per = ceil_div(pieces, c);
+  return {c, (int)std::min<int64_t>(DISTILL_THREADS, std::max<int64_t>(64, round_up(ceil_div(per, 8), 32))), (int)per};
 }
 inline int64_t distill_workspace(int64_t rows, int top, bool gradient) { return rows * (16 + (gradient ? 12 * (int64_t)top : 0)); }
 

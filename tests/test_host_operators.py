@@ -67,13 +67,14 @@ static void distill() {
   NO(check_distill(GN_BF16, 4, 100, 8, 1.f, x, 100, ids, GN_I64, (const float*)at(258), w, l, d, 100)); NO(check_distill(GN_BF16, 4, 100, 8, 1.f, x, -1, ids, GN_I64, t, w, l, d, 100));
   NO(check_distill(GN_BF16, 4, 100, 8, 1.f, x, 100, ids, GN_I64, t, w, l, d, 99)); OK(check_distill(GN_BF16, 1, 100, 8, 1.f, x, 100, ids, GN_I64, t, w, l, d, 0));
   NO(check_distill(GN_BF16, 4, 100, 8, 1.f, x, 104, ids, GN_I64, t, w, l, x, 100)); OK(check_distill(GN_BF16, 4, 100, 8, 1.f, x, 104, ids, GN_I64, t, w, l, x, 104));
-  // a block's part of a row, wherever it begins within 16 bytes, fits its threads' registers
+  // the blocks' parts hold a row, wherever it begins within 16 bytes
   for (long rows : {1L, 24L, 149L, 100000L}) for (int v = 0; v < 22; v++) for (long vocab = std::max(1L, (1L << v) - 20 * (1 + v / 14)); vocab < (1L << v) + 20; vocab++)
     for (int size : {2, 4}) {
-      const DistillPlan p = distill_plan(rows, vocab, 148);
-      if (p.cluster == 0) { IS(vocab > 8 * 32768 - 200); continue; }
+      const DistillPlan p = distill_plan(rows, vocab, size, 148);
+      if (p.cluster == 0) { IS(vocab * size > 8L * DISTILL_PART_MOST - 200); continue; }
       const int V = 16 / size;
-      for (int lead = 0; lead < V; lead++) { const long pieces = ceil_div(vocab + V - 1, V); if (lead + vocab > pieces * V || ceil_div(pieces, p.cluster) > (long)p.threads * DISTILL_ITEMS / V) { bad++; std::printf("vocab %ld rows %ld\n", vocab, rows); } }
+      IS(p.threads >= 64 && p.threads <= DISTILL_THREADS && p.threads % 32 == 0 && p.per * 16 <= DISTILL_PART_MOST);
+      for (int lead = 0; lead < V; lead++) if (ceil_div(lead + vocab, V) > (long)p.cluster * p.per) { bad++; std::printf("vocab %ld rows %ld\n", vocab, rows); }
     }
 }
 static void embedding() {
