@@ -17,7 +17,7 @@ EXPORTS = [
     "gn_adam_set_state", "gn_train_batch", "gn_train_batch_device", "gn_forward_batch", "gn_device_alloc",
     "gn_device_free", "gn_device_upload", "gn_device_download", "gn_model_last_stats", "gn_model_set_profiling",
     "gn_op_gemm_nt", "gn_op_adam", "gn_op_layernorm", "gn_op_conv2d", "gn_op_softmax_ce", "gn_op_lstm", "gn_op_gemm_nt_static", "gn_op_attention", "gn_model_state_count", "gn_model_get_state", "gn_model_set_state",
-    "gn_op_status", "gn_op_qk_norm_rope", "gn_op_qk_norm_rope_workspace", "gn_op_qk_norm_rope_backward", "gn_op_distill", "gn_op_distill_workspace",
+    "gn_op_status", "gn_op_qk_norm_rope", "gn_op_qk_norm_rope_workspace", "gn_op_qk_norm_rope_backward", "gn_op_distill",
     "gn_op_embedding", "gn_op_embedding_workspace", "gn_op_embedding_backward",
     "gn_op_gated_ffn_saved", "gn_op_gated_ffn_workspace", "gn_op_gated_ffn", "gn_op_gated_ffn_backward",
 ]
@@ -94,8 +94,7 @@ def load():
     L.gn_op_qk_norm_rope.argtypes = qk + [heads, heads, vp]
     L.gn_op_qk_norm_rope_workspace.argtypes = [vp, i64, i, i, i, i64p]
     L.gn_op_qk_norm_rope_backward.argtypes = qk + [heads] * 4 + [vp] * 3 + [i64, vp]
-    L.gn_op_distill.argtypes = [vp, i, i64, i64, i, f, vp, i64, vp, i, vp, vp, vp, vp, i64, vp, i64, vp]
-    L.gn_op_distill_workspace.argtypes = [vp, i64, i, i, i64p]
+    L.gn_op_distill.argtypes = [vp, i, i64, i64, i, f, vp, i64, vp, i, vp, vp, vp, vp, i64, vp]
     L.gn_op_embedding.argtypes = [vp, i, i64, i64, i, f, vp, i64, vp, i, vp, i64, vp]
     L.gn_op_embedding_workspace.argtypes = [vp, i64, i64, i, i64p]
     L.gn_op_embedding_backward.argtypes = [vp, i, i64, i64, i, f, vp, i64, vp, i, vp, vp, i64, vp]

@@ -7,24 +7,21 @@
 // another before it sums; (m, sum) pairs then meet in shuffles, in shared memory and between the blocks of a cluster, and q_j = e_j 2^((m - M) c) / S.  Differences
 // come before the factor: logits at the type's lowest value stay finite.
 //
-// Bound by memory: a row is read once and its gradient written once.  One launch forms what the teacher's few entries come to, a warp a row, so that no long
-// row waits for their chain of dependent loads; the second streams the rows.  A row, or a block's part of it, lies in shared memory; every thread copies there, sums over and writes back its own
+// Bound by memory: a row is read once and its gradient written once.  A row, or a block's part of it, lies in shared memory; every thread copies there, sums over and writes back its own
 // 16-byte pieces of it, so that the only barrier of a row is the one at which the warps' sums meet, and the copies of a thread's next row are under way as soon as it has written this one.
-// Blocks of an SM (three for rows of 64 KB) overlap each other's phases.  (Rows held as exponentials in registers, 1024 threads a row: 26 instructions an element, most of them per row
-// and thread, 2.4 TB/s.)  A row of more than 72 KB is spread over a cluster of blocks, whose barrier is then the cluster's.
-// Each block writes q for all of its elements; where the teacher has entries q - p is written over it, behind the next row's barrier.
+// Blocks of an SM (three for rows of 64 KB) overlap each other's phases.  A row of more than 104 KB is spread over a cluster of blocks, whose barrier is then the cluster's.
+// One more warp of every block works on the teacher's few entries, a chain of dependent loads, one row ahead of the others (a launch of its own before this one: 58 of 162 us for 4096 rows of
+// 32000 with 64 entries, bf16).  The other warps write q everywhere; that warp writes q - p over it where the teacher has entries, behind the next row's barrier.
+// (Rows held as exponentials in registers, 64 elements a thread, which saves one of an element's two exponentials: 121 us without the teacher's part, 102 this way; the special-function units do not
+// bound it, leaving all exponentials out saves 12.)
 #pragma once
 #include "device_ops.cuh"
 
 namespace gn {
 
-// What the teacher's entries of a row come to: l as in Norm below, r the student's largest value where the teacher has probability (0 if it has none), d = sum of
-// p ((t - max t) - (s - r)); w: the row's weight, 0 where it has no entry of positive probability.
-struct alignas(16) Teacher { float l, d, r, w; };
 struct DistillParams {
   const void* logits; long stride; const void* ids; int index_type; const float* top_logits; const float* weight; float* loss; void* dlogits; long dstride;
   long rows, vocab; int top; float temperature;
-  Teacher* teach; int* id; float* prob; float* stud;                 // workspace: [rows], and [rows][top] each (the gradient's)
 };
 
 struct MaxSum { float m, s; };                                       // of values v: m >= all v (or -inf: none), s = sum of 2^((v - m) c)
@@ -40,6 +37,9 @@ __device__ __forceinline__ MaxSum warp_join(MaxSum v, float c) {
 }
 // A row's probabilities are 2^((s - m) c - l).
 struct Norm { float m, l; };
+// What the teacher's entries of a row come to: l as there, r the student's largest value where the teacher has probability (0 if it has none), d = sum of p ((t - max t) - (s - r)); w: the
+// row's weight, 0 where it has no entry of positive probability.
+struct Teacher { float l, d, r, w; };
 __device__ __forceinline__ Norm norm_of(MaxSum v) { return Norm{v.m, log2f(v.s)}; }
 
 constexpr int DISTILL_TOP = 1024;
@@ -51,99 +51,93 @@ __device__ __forceinline__ int teacher_entry(const DistillParams& p, long row, i
   t = there ? __ldg(p.top_logits + row * p.top + k) : -INFINITY;
   return there ? (int)id : -1;
 }
-// A warp a row, 128 entries of it at a time in registers.  With a gradient the entries' ids, probabilities and student values are kept for the second launch; of entries with the same id the
-// first keeps all of their probability and the others become -1.  Such entries are rare and found by a table: every entry writes its number at its id's place, and whoever finds
-// another's number there, or is found by another of the same id, looks through the row.
-constexpr int TEACHER_WARPS = 4, TEACHER_TABLE = 2048;
-inline int teacher_smem(int top) { return TEACHER_WARPS * (TEACHER_TABLE * 2 + (top + 15) / 16 * 16 * 9); }      // table, ids, probabilities, flags
+// One warp.  The entries go through shared memory, where the gradient finds their ids, probabilities and student values again; the student's values are asked for as soon as the ids are there.
+// Of entries with the same id the first keeps all of their probability and the others become -1.  They are rare and found by a table: every entry writes its number at its id's place; who
+// finds another's number there and not the same id tries a second place; where that is taken too, or the ids are the same, the row is looked through.
+constexpr int TEACHER_TABLE = 2048;
+struct TeacherRow { int* id; float *prob, *stud; };                  // [top, rounded up to 16] each
+struct TeacherSmem {                                                 // rows in turns of three, then what one row needs while it is worked on
+  uint8_t* base; int top16;
+  __device__ __forceinline__ TeacherRow row(int turn) const { int* id = reinterpret_cast<int*>(base) + turn * 3 * top16; return TeacherRow{id, reinterpret_cast<float*>(id + top16), reinterpret_cast<float*>(id + 2 * top16)}; }
+  __device__ __forceinline__ float* logit() const { return reinterpret_cast<float*>(base) + 9 * top16; }
+  __device__ __forceinline__ unsigned short* table() const { return reinterpret_cast<unsigned short*>(base + 40 * top16); }
+};
+inline int teacher_smem(int top) { return (top + 15) / 16 * 16 * 40 + 2 * TEACHER_TABLE; }
 template <class T, bool GRAD>
-__global__ void __launch_bounds__(32 * TEACHER_WARPS) distill_teacher_kernel(const __grid_constant__ DistillParams p) {
-  pdl_wait(); pdl_launch();                                          // (in this order: the launch behind fetches logits before this one has finished)
-  extern __shared__ uint4 teacher_smem_raw[];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, top16 = (p.top + 15) & ~15; const float c = 1.4426950408889634f / p.temperature;
-  uint8_t* own = reinterpret_cast<uint8_t*>(teacher_smem_raw) + warp * (TEACHER_TABLE * 2 + top16 * 9);
-  int* id_of = reinterpret_cast<int*>(own); float* prob_of = reinterpret_cast<float*>(id_of + top16);
-  unsigned short* table = reinterpret_cast<unsigned short*>(prob_of + top16); uint8_t* look = reinterpret_cast<uint8_t*>(table + TEACHER_TABLE);
-  const long row = (long)blockIdx.x * TEACHER_WARPS + warp;
-  if (row >= p.rows) return;
+__device__ __forceinline__ Teacher teacher_row(const DistillParams& p, long row, float c, int lane, const TeacherSmem& sm, const TeacherRow& to) {
   const float w = p.weight ? __ldg(p.weight + row) : 1.f;
-  Teacher out{0.f, 0.f, 0.f, 0.f};
-  if (w != 0.f) {
-    const T* logits = static_cast<const T*>(p.logits) + row * p.stride;
-    constexpr int E = 4;
-    int id[E]; float t[E];
-    auto load = [&](int k0) {
+  if (w == 0.f) return Teacher{0.f, 0.f, 0.f, 0.f};
+  const T* logits = static_cast<const T*>(p.logits) + row * p.stride; float* logit = sm.logit(); unsigned short* table = sm.table();
+  float m = -INFINITY;
+  for (int k0 = lane; k0 < sm.top16; k0 += 64) {
+    int id[2]; float t[2], s[2];
 #pragma unroll
-      for (int e = 0; e < E; e++) { const int k = k0 + 32 * e + lane; id[e] = -1; t[e] = -INFINITY; if (k < p.top) id[e] = teacher_entry(p, row, k, t[e]); }
-    };
-    MaxSum v{-INFINITY, 0.f};
-    for (int k0 = 0; k0 < p.top; k0 += 32 * E) {
-      load(k0);
+    for (int e = 0; e < 2; e++) { id[e] = -2; t[e] = -INFINITY; if (k0 + 32 * e < p.top) id[e] = teacher_entry(p, row, k0 + 32 * e, t[e]); }
 #pragma unroll
-      for (int e = 0; e < E; e++) v = join(v, MaxSum{t[e], t[e] == -INFINITY ? 0.f : 1.f}, c);
-    }
-    v = warp_join(v, c);
-    const bool some = !(v.m == -INFINITY && v.s == 0.f); const Norm n = norm_of(v);
-    float d = 0.f, r = -INFINITY, weight = 0.f;                      // d: relative to this lane's r so far; weight: the probability that it holds
-    for (int k0 = 0; k0 < p.top; k0 += 32 * E) {
-      if (p.top > 32 * E) load(k0);
-      float s[E];
+    for (int e = 0; e < 2; e++) s[e] = id[e] >= 0 ? to_f32(logits[id[e]]) : 0.f;
 #pragma unroll
-      for (int e = 0; e < E; e++) s[e] = id[e] >= 0 ? to_f32(logits[id[e]]) : 0.f;
-#pragma unroll
-      for (int e = 0; e < E; e++) {
-        const int k = k0 + 32 * e + lane;
-        const float pk = !some || t[e] == -INFINITY ? 0.f : exp2f((t[e] - n.m) * c - n.l);
-        if (pk != 0.f) {                                             // (an entry without weight says nothing, whatever the student has there)
-          if (s[e] > r) { if (weight != 0.f) d += weight * (s[e] - r); r = s[e]; }      // sum of p (r - s) moves with r
-          d += pk * ((t[e] - n.m) - (s[e] - (r == -INFINITY ? 0.f : r))); weight += pk;
-        }
-        if constexpr (GRAD) {
-          if (k < top16) { id_of[k] = k < p.top ? id[e] : -2; prob_of[k] = pk; look[k] = 0; }
-          if (k < p.top) { p.stud[row * p.top + k] = s[e]; if (id[e] >= 0) table[id[e] & (TEACHER_TABLE - 1)] = (unsigned short)k; }
-        }
-      }
-    }
-    const float top = warp_max(r), ref = top == -INFINITY ? 0.f : top;
-    if (weight != 0.f) d += weight * (ref - (r == -INFINITY ? 0.f : r));
-    out = Teacher{n.l, warp_sum(d), ref, some ? w : 0.f};
-    if constexpr (GRAD) {
-      __syncwarp();
-      for (int k = lane; k < p.top; k += 32) {
-        const int i = id_of[k];
-        if (i < 0) continue;
-        const int found = table[i & (TEACHER_TABLE - 1)];
-        if (found != k) { look[k] = 1; if (id_of[found] == i) look[found] = 1; }
-      }
-      __syncwarp();
-      for (int k = lane; k < p.top; k += 32) {
-        int i = id_of[k]; float pk = prob_of[k];
-        if (look[k]) {
-          const int mine = i; pk = 0.f;
-          for (int f = 0; f < top16; f += 4) {
-            const int4 o = *reinterpret_cast<const int4*>(id_of + f);
-            if (o.x != mine && o.y != mine && o.z != mine && o.w != mine) continue;
-            const int q[4] = {o.x, o.y, o.z, o.w};
-            for (int l = 0; l < 4; l++) if (q[l] == mine) { if (f + l < k) i = -1; pk += prob_of[f + l]; }
-          }
-        }
-        p.id[row * p.top + k] = i; p.prob[row * p.top + k] = pk;
-      }
+    for (int e = 0; e < 2; e++) {
+      const int k = k0 + 32 * e;
+      if (k < sm.top16) { to.id[k] = id[e]; logit[k] = t[e]; to.stud[k] = s[e]; if (GRAD && id[e] >= 0) table[id[e] & (TEACHER_TABLE - 1)] = (unsigned short)k; }
+      m = fmaxf(m, t[e]);
     }
   }
-  if (lane == 0) p.teach[row] = out;
+  m = warp_max(m);
+  const float ref = m == -INFINITY ? 0.f : m; float sum = 0.f, r = -INFINITY;
+  for (int k = lane; k < p.top; k += 32) {
+    const float e = exp2f((logit[k] - ref) * c);
+    sum += e; to.prob[k] = e; if (e != 0.f) r = fmaxf(r, to.stud[k]);      // (an entry without weight says nothing, whatever the student has there)
+  }
+  sum = warp_sum(sum); r = warp_max(r);
+  const bool some = sum != 0.f; const float scale = some ? 1.f / sum : 0.f; float d = 0.f;
+  if (r == -INFINITY) r = 0.f;
+  for (int k = lane; k < p.top; k += 32) { const float e = to.prob[k], pk = e * scale; if (e != 0.f) d += pk * ((logit[k] - ref) - (to.stud[k] - r)); to.prob[k] = pk; }
+  if constexpr (GRAD) {
+    __syncwarp();
+    bool lost = false, look = false;
+    for (int k = lane; k < p.top; k += 32) {
+      const int i = to.id[k], found = i >= 0 ? table[i & (TEACHER_TABLE - 1)] : k;
+      if (found != k) { lost = true; look |= to.id[found] == i; }
+    }
+    if (__any_sync(0xffffffffu, lost) && !__any_sync(0xffffffffu, look)) {
+      auto second = [](int i) { return (unsigned)i * 2654435761u >> 21; };      // (2^32 over the golden ratio: 11 bits)
+      unsigned mine = 0;                                             // this lane's entries that lost
+      for (int k = lane, j = 0; k < p.top; k += 32, j++) { const int i = to.id[k]; if (i >= 0 && table[i & (TEACHER_TABLE - 1)] != k) mine |= 1u << j; }
+      __syncwarp();
+      for (int k = lane, j = 0; k < p.top; k += 32, j++) if (mine >> j & 1) table[second(to.id[k])] = (unsigned short)k;
+      __syncwarp();
+      for (int k = lane, j = 0; k < p.top; k += 32, j++) if (mine >> j & 1) look |= table[second(to.id[k])] != k;
+    }
+    if (__any_sync(0xffffffffu, look)) {
+      // sums for the first of each id, in order; the others become -1 when all have looked
+      unsigned gone = 0;
+      for (int k = lane, j = 0; k - lane < p.top; k += 32, j++) {
+        const int i = k < p.top ? to.id[k] : -1; float pk = 0.f; bool first = true;
+        if (i >= 0)
+          for (int f = 0; f < sm.top16; f += 4) {
+            const int4 o = *reinterpret_cast<const int4*>(to.id + f);
+            if (o.x != i && o.y != i && o.z != i && o.w != i) continue;
+            const int q[4] = {o.x, o.y, o.z, o.w};
+            for (int l = 0; l < 4; l++) if (q[l] == i) { if (f + l < k) first = false; pk += to.prob[f + l]; }
+          }
+        __syncwarp();
+        if (i >= 0 && first) to.prob[k] = pk; else if (i >= 0) gone |= 1u << j;      // (an id's sum is read by nobody behind its first entry)
+        __syncwarp();
+      }
+      for (int k = lane, j = 0; k < p.top; k += 32, j++) if (gone >> j & 1) to.id[k] = -1;
+    }
+    __syncwarp();
+  }
+  return Teacher{log2f(sum), warp_sum(d), r, some ? w : 0.f};
 }
 // w T^2 sum of p (log p - log q), from p = 2^((t - max t) c - l_t) and q = 2^((s - M) c - l), as the p add up to 1
 __device__ __forceinline__ float distill_loss(const Teacher& t, Norm n, float tau) { return t.w != 0.f ? t.w * tau * (t.d + (n.m - t.r) + tau * 0.69314718055994531f * (n.l - t.l)) : 0.f; }
-// q - p where the teacher has entries of row r, over what is there, for ids in [lo, hi)
+// q - p where the teacher has entries of row r, over what is there, for ids in [lo, hi); one warp
 template <class T>
-__device__ __forceinline__ void distill_entry(const DistillParams& p, T* out, int id, float prob, float stud, float w, Norm n, float c, long lo, long hi) {
-  if (id >= 0 && id >= lo && id < hi) out[id] = from_f32<T>(w * p.temperature * (ex2((stud - n.m) * c - n.l) - prob));
-}
-template <class T>
-__device__ __forceinline__ void distill_entries(const DistillParams& p, long r, int first, float w, Norm n, float c, long lo, long hi) {
+__device__ __forceinline__ void distill_entries(const DistillParams& p, long r, const TeacherRow& of, float w, Norm n, float c, long lo, long hi, int lane) {
+  if (w == 0.f) return;
   T* out = static_cast<T*>(p.dlogits) + r * p.dstride;
-  for (int e = first + threadIdx.x; e < p.top; e += blockDim.x) { const long i = r * p.top + e; distill_entry<T>(p, out, p.id[i], p.prob[i], p.stud[i], w, n, c, lo, hi); }
+  for (int e = lane; e < p.top; e += 32) { const int id = of.id[e]; if (id >= 0 && id >= lo && id < hi) out[id] = from_f32<T>(w * p.temperature * (ex2((of.stud[e] - n.m) * c - n.l) - of.prob[e])); }
 }
 
 // Elements of a row from the 16-byte boundary at or before its first one.
@@ -178,32 +172,30 @@ template <class T> __device__ __forceinline__ float2 piece_pair(const uint4& u, 
 
 // `cl` blocks on a row, `per` 16-byte pieces of it (counted from its 16-byte boundary) for each.  WHOLE: every row and its gradient begin on such a boundary and fill their pieces.
 template <class T, bool GRAD, bool WHOLE>
-__global__ void __launch_bounds__(DISTILL_THREADS, 3) distill_kernel(const __grid_constant__ DistillParams p, int cl, int per) {
+__global__ void __launch_bounds__(DISTILL_THREADS + 32, 3) distill_kernel(const __grid_constant__ DistillParams p, int cl, int per) {
   namespace cg = cooperative_groups;
   constexpr int V = Vec<T>::N;
-  extern __shared__ uint4 slots[];                                   // [per], rounded up to whole turns of all threads: -inf behind
-  __shared__ MaxSum part[2][8 * DISTILL_THREADS / 32];               // sums of all warps of the cluster (rows take turns: a warp may be a row ahead of another, never two)
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nt = blockDim.x, warps = nt >> 5, vocab = (int)p.vocab;
+  extern __shared__ uint4 slots[];                                   // [per], then the teacher's
+  // Rows take turns with what their barrier guards, a warp may be a row ahead of another, never two: sums of all warps of the cluster; weights, which are written a row ahead.
+  __shared__ MaxSum part[2][8 * DISTILL_THREADS / 32]; __shared__ float weight_of_turn[3];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nt = blockDim.x - 32, warps = nt >> 5, vocab = (int)p.vocab;
   const int rank = cl > 1 ? (int)(blockIdx.x % cl) : 0; const long row0 = blockIdx.x / cl, step = gridDim.x / cl;
   const float c = 1.4426950408889634f / p.temperature;
   const int at = rank * per;                                         // this block's pieces: [at, at + per), as far as the row goes
-  pdl_launch();
+  op_begin();
   if (cl > 1) cg::this_cluster().sync();                             // (all blocks are there before one writes into another)
   auto row_of = [&](long r) { return static_cast<const T*>(p.logits) + r * p.stride; };
   auto lead_of = [&](long r) { return WHOLE ? 0 : row_lead(row_of(r)); };
   auto count = [&](int lead) { return min(per, (lead + vocab + V - 1) / V - at); };      // pieces of this block
-  const int n_whole = (per + nt - 1) / nt * nt;                      // places of all threads' turns
   auto weight_of = [&](long r) { return r >= p.rows ? 0.f : p.weight ? __ldg(p.weight + r) : 1.f; };
   // copies of this thread's pieces of row r; pieces that the row does not fill are put together element by element, -inf where it has none
-  const uint32_t slot0 = (uint32_t)__cvta_generic_to_shared(slots), none = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
-  const uint4 nothing = make_uint4(none, none, none, none);          // -inf
+  const uint32_t slot0 = (uint32_t)__cvta_generic_to_shared(slots);
   auto fetch = [&](long r, float w) {
     if (w != 0.f) {
       const T* row = row_of(r); const int lead = lead_of(r), n = count(lead);
-      for (int i = tid; i < (WHOLE ? n : n_whole); i += nt) {        // (WHOLE: what lies behind is the same for every row)
+      for (int i = tid; i < n; i += nt) {
         const int e = (at + i) * V - lead;                           // first element
-        if (!WHOLE && i >= n) slots[i] = nothing;
-        else if (WHOLE || (e >= 0 && e + V <= vocab)) cp16(slot0 + i * 16, row + e);
+        if (WHOLE || (e >= 0 && e + V <= vocab)) cp16(slot0 + i * 16, row + e);
         else {
           T* q = reinterpret_cast<T*>(slots + i);
 #pragma unroll
@@ -214,21 +206,50 @@ __global__ void __launch_bounds__(DISTILL_THREADS, 3) distill_kernel(const __gri
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
 
-  if (WHOLE) for (int i = tid; i < n_whole; i += nt) if (i >= count(0)) slots[i] = nothing;
+  auto barrier = [&]() { if (cl == 1) __syncthreads(); else cg::this_cluster().sync(); };
+  auto reduce = [&](MaxSum v) {
+    const float top = warp_max(v.m), to = top == -INFINITY ? 0.f : top;
+    return MaxSum{top, warp_sum(v.s * ex2((v.m - to) * c))};
+  };
+  auto meet = [&](int turn) {                                        // behind the barrier: all warps' sums
+    MaxSum v{-INFINITY, 0.f};
+    for (int k = lane; k < cl * warps; k += 32) v = join(v, part[turn][k], c);
+    return norm_of(reduce(v));
+  };
+  if (warp == warps) {                                               // the teacher's warp
+    const TeacherSmem sm{reinterpret_cast<uint8_t*>(slots + per), (p.top + 15) & ~15};
+    auto bounds = [&](long r, long& lo, long& hi) { lo = (long)at * V - lead_of(r); hi = lo + (long)per * V; };
+    Teacher now = teacher_row<T, GRAD>(p, row0, c, lane, sm, sm.row(0)); int three = 0, turn = 0; long done = -1; float done_w = 0.f; Norm done_n{0.f, 0.f};
+    if (lane == 0) weight_of_turn[0] = now.w;
+    for (long r = row0; r < p.rows; r += step, turn ^= 1) {
+      const int next = three == 2 ? 0 : three + 1, last = three == 0 ? 2 : three - 1;
+      Teacher then{0.f, 0.f, 0.f, 0.f};
+      if (r + step < p.rows) { then = teacher_row<T, GRAD>(p, r + step, c, lane, sm, sm.row(next)); if (lane == 0) weight_of_turn[next] = then.w; }
+      __syncwarp();
+      barrier();
+      const Norm nm = meet(turn);
+      if (lane == 0 && rank == 0) p.loss[r] = distill_loss(now, nm, p.temperature);
+      if constexpr (GRAD) { if (done >= 0) { long lo, hi; bounds(done, lo, hi); distill_entries<T>(p, done, sm.row(last), done_w, done_n, c, lo, hi, lane); } }
+      done = r; done_w = now.w; done_n = nm; now = then; three = next;
+    }
+    if constexpr (GRAD) {
+      __syncthreads();
+      long lo, hi; bounds(done, lo, hi); distill_entries<T>(p, done, sm.row(three == 0 ? 2 : three - 1), done_w, done_n, c, lo, hi, lane);
+    }
+    if (cl > 1) cg::this_cluster().sync();
+    return;
+  }
+
   float w_now = weight_of(row0); fetch(row0, w_now);
-  pdl_wait();                                                        // for the teacher's launch
-  int turn = 0; long done = -1; float done_w = 0.f; Norm done_n{0.f, 0.f};
+  int turn = 0, three = 0;
   for (long r = row0; r < p.rows; r += step, turn ^= 1) {
-    const Teacher t = p.teach[r]; const float w_next = weight_of(r + step); const int lead = lead_of(r), n = count(lead); const bool on = t.w != 0.f;
-    // the entries of the row before, one a thread
-    int id = -1; float prob = 0.f, stud = 0.f;
-    if constexpr (GRAD) { if (done_w != 0.f && tid < p.top) { const long i = done * p.top + tid; id = p.id[i]; prob = p.prob[i]; stud = p.stud[i]; } }
+    const float w_next = weight_of(r + step); const int lead = lead_of(r), n = count(lead);
     asm volatile("cp.async.wait_all;" ::: "memory");
     float m = -INFINITY, s = 0.f;
     if (w_now != 0.f) {
       float2 sum = make_float2(0.f, 0.f);
-#pragma unroll 2
-      for (int i = tid; i < n_whole; i += nt) {
+#pragma unroll 1
+      for (int i = tid; i < n; i += nt) {
         const uint4 u = slots[i];
         const float top = fmaxf(m, piece_max<T>(u));
         if (top > m) { const float g = ex2((m - top) * c); sum = mul2(sum, make_float2(g, g)); m = top; }      // (rarely behind the first pieces)
@@ -238,25 +259,13 @@ __global__ void __launch_bounds__(DISTILL_THREADS, 3) distill_kernel(const __gri
       }
       s = sum.x + sum.y;
     }
-    auto meet = [&](MaxSum v) {
-      const float top = warp_max(v.m), to = top == -INFINITY ? 0.f : top;
-      return MaxSum{top, warp_sum(v.s * ex2((v.m - to) * c))};
-    };
-    MaxSum v = meet(MaxSum{m, s});
-    if (cl == 1) {
-      if (lane == 0) part[turn][warp] = v;
-      __syncthreads();
-    } else {
-      cg::cluster_group cluster = cg::this_cluster();
-      if (lane < cl) *cluster.map_shared_rank(&part[turn][rank * warps + warp], lane) = v;
-      cluster.sync();
-    }
-    v = MaxSum{-INFINITY, 0.f};
-    for (int k = lane; k < cl * warps; k += 32) v = join(v, part[turn][k], c);
-    const Norm nm = norm_of(meet(v));
-    if (tid == 0 && rank == 0) p.loss[r] = distill_loss(t, nm, p.temperature);
+    const MaxSum v = reduce(MaxSum{m, s});
+    if (cl == 1) { if (lane == 0) part[turn][warp] = v; }
+    else if (lane < cl) *cg::this_cluster().map_shared_rank(&part[turn][rank * warps + warp], lane) = v;
+    __syncwarp();
+    barrier();
     if constexpr (GRAD) {
-      const float f = t.w * p.temperature;
+      const Norm nm = meet(turn); const float f = weight_of_turn[three] * p.temperature; const bool on = f != 0.f;
       T* out = static_cast<T*>(p.dlogits) + r * p.dstride; const bool same = WHOLE || row_lead(out) == lead;
       auto put = [&](int i, const float (&y)[V]) {
         const int e = (at + i) * V - lead;
@@ -268,7 +277,7 @@ __global__ void __launch_bounds__(DISTILL_THREADS, 3) distill_kernel(const __gri
       };
       if (on) {
         const float2 m2 = make_float2(-nm.m, -nm.m), c2 = make_float2(c, c), l2 = make_float2(-nm.l, -nm.l), f2 = make_float2(f, f);
-#pragma unroll 2
+#pragma unroll 1
         for (int i = tid; i < n; i += nt) {
           const uint4 u = slots[i]; float y[V];
 #pragma unroll
@@ -282,19 +291,9 @@ __global__ void __launch_bounds__(DISTILL_THREADS, 3) distill_kernel(const __gri
     }
     fetch(r + step, w_next);                                         // (this thread has read its pieces)
     w_now = w_next;
-    if constexpr (GRAD) {
-      if (done_w != 0.f) {
-        const long lo = (long)at * V - lead_of(done);
-        distill_entry<T>(p, static_cast<T*>(p.dlogits) + done * p.dstride, id, prob, stud, done_w, done_n, c, lo, lo + (long)per * V);
-        distill_entries<T>(p, done, nt, done_w, done_n, c, lo, lo + (long)per * V);
-      }
-      done = r; done_w = t.w; done_n = nm;
-    }
+    if (++three == 3) three = 0;
   }
-  if constexpr (GRAD) {
-    __syncthreads();
-    if (done_w != 0.f) { const long lo = (long)at * V - lead_of(done); distill_entries<T>(p, done, 0, done_w, done_n, c, lo, lo + (long)per * V); }
-  }
+  if constexpr (GRAD) __syncthreads();                               // (the last row is written)
   if (cl > 1) cg::this_cluster().sync();                             // (no block leaves while another may still write into it)
 }
 
@@ -302,12 +301,15 @@ __global__ void __launch_bounds__(DISTILL_THREADS, 3) distill_kernel(const __gri
 template <class T, bool GRAD>
 __global__ void __launch_bounds__(1024) distill_long_kernel(const __grid_constant__ DistillParams p) {
   op_begin();
-  __shared__ MaxSum part[32];
+  extern __shared__ uint4 slots[];
+  __shared__ MaxSum part[32]; __shared__ Teacher teach;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5; const float c = 1.4426950408889634f / p.temperature;
+  const TeacherSmem sm{reinterpret_cast<uint8_t*>(slots), (p.top + 15) & ~15};
   for (long r = blockIdx.x; r < p.rows; r += gridDim.x) {
-    const T* row = static_cast<const T*>(p.logits) + r * p.stride; const Teacher t = p.teach[r]; const bool on = t.w != 0.f;
+    const T* row = static_cast<const T*>(p.logits) + r * p.stride;
     MaxSum v{-INFINITY, 0.f};
-    if (on)
+    if (warp == 0) { const Teacher t = teacher_row<T, GRAD>(p, r, c, lane, sm, sm.row(0)); if (lane == 0) teach = t; }
+    if ((p.weight ? __ldg(p.weight + r) : 1.f) != 0.f)
       for (long e0 = tid; e0 < p.vocab; e0 += 8 * 1024) {
         float x[8]; float m = -INFINITY;
 #pragma unroll
@@ -320,13 +322,13 @@ __global__ void __launch_bounds__(1024) distill_long_kernel(const __grid_constan
     v = warp_join(v, c);
     if (lane == 0) part[warp] = v;
     __syncthreads();
-    const Norm n = norm_of(warp_join(part[lane], c));
+    const Norm n = norm_of(warp_join(part[lane], c)); const Teacher t = teach; const bool on = t.w != 0.f;
     if (tid == 0) p.loss[r] = distill_loss(t, n, p.temperature);
     if constexpr (GRAD) {
       T* out = static_cast<T*>(p.dlogits) + r * p.dstride;
       for (long e = tid; e < p.vocab; e += 1024) out[e] = from_f32<T>(on ? t.w * p.temperature * ex2((to_f32(row[e]) - n.m) * c - n.l) : 0.f);
       __syncthreads();
-      if (on) distill_entries<T>(p, r, 0, t.w, n, c, 0, p.vocab);
+      if (warp == 0) distill_entries<T>(p, r, sm.row(0), t.w, n, c, 0, p.vocab, lane);
     }
     __syncthreads();
   }
@@ -335,16 +337,13 @@ __global__ void __launch_bounds__(1024) distill_long_kernel(const __grid_constan
 template <class T, bool GRAD>
 inline int distill_launch(gn_ctx* ctx, const DistillParams& p, void* stream) {
   const int sms = ctx->c.sm_count; const DistillPlan pl = distill_plan(p.rows, p.vocab, (int)sizeof(T), sms);
-  const int tsmem = teacher_smem(GRAD ? p.top : 0);
-  if (tsmem > 48 * 1024) GN_TRY(op_smem("distill_teacher", distill_teacher_kernel<T, GRAD>, tsmem));
-  GN_TRY(op_launch("distill_teacher", stream, distill_teacher_kernel<T, GRAD>, dim3(cdiv(p.rows, TEACHER_WARPS)), dim3(32 * TEACHER_WARPS), tsmem, 0, p));
-  if (pl.cluster == 0) return op_launch("distill_long", stream, distill_long_kernel<T, GRAD>, dim3((unsigned)std::min<int64_t>(p.rows, 2L * sms)), dim3(1024), 0, 0, p);
+  const int tsmem = teacher_smem(p.top);
+  if (pl.cluster == 0) return op_launch("distill_long", stream, distill_long_kernel<T, GRAD>, dim3((unsigned)std::min<int64_t>(p.rows, 2L * sms)), dim3(1024), tsmem, 0, p);
   constexpr int V = Vec<T>::N;
   const bool whole = p.vocab % V == 0 && p.stride % V == 0 && aligned_to(p.logits, 16) && (!GRAD || (p.dstride % V == 0 && aligned_to(p.dlogits, 16)));
-  const int smem = (int)round_up(pl.per, pl.threads) * 16;
-  const int64_t per_sm = std::max<int64_t>(1, std::min<int64_t>({2048 / pl.threads, 32, 220 * 1024 / (smem + 3 * 1024)}));
+  const int smem = pl.per * 16 + tsmem; const int64_t per_sm = std::max<int64_t>(1, std::min<int64_t>({2048 / (pl.threads + 32), 32, 65536 / (40 * (pl.threads + 32)), 224 * 1024 / (smem + 3 * 1024)}));
   const dim3 grid((unsigned)(std::min<int64_t>(p.rows, std::max<int64_t>(1, (int64_t)sms * per_sm / pl.cluster)) * pl.cluster));
-  auto go = [&](auto kernel) { if (smem > 40 * 1024) GN_TRY(op_smem("distill", kernel, smem)); return op_launch("distill", stream, kernel, grid, dim3(pl.threads), smem, pl.cluster, p, pl.cluster, pl.per); };
+  auto go = [&](auto kernel) { if (smem > 40 * 1024) GN_TRY(op_smem("distill", kernel, smem)); return op_launch("distill", stream, kernel, grid, dim3(pl.threads + 32), smem, pl.cluster, p, pl.cluster, pl.per); };
   return whole ? go(distill_kernel<T, GRAD, true>) : go(distill_kernel<T, GRAD, false>);
 }
 
@@ -352,20 +351,12 @@ inline int distill_launch(gn_ctx* ctx, const DistillParams& p, void* stream) {
 
 extern "C" {
 
-int gn_op_distill_workspace(gn_ctx* ctx, int64_t rows, int top, int gradient, int64_t* bytes) {
-  using namespace gn;
-  if (!ctx || !ctx->alive || !bytes || rows < 0 || rows > OP_MAX_ROWS || top < 0 || top > DISTILL_TOP) return fail(GN_ERR_INVALID_ARG, "op_distill_workspace: bad argument");
-  *bytes = distill_workspace(rows, top, gradient != 0); return GN_OK;
-}
-
 int gn_op_distill(gn_ctx* ctx, int dtype, int64_t rows, int64_t vocab, int top, float temperature, const void* logits, int64_t row_stride, const void* top_ids, int index_type, const float* top_logits,
-                  const float* weight, float* loss, void* dlogits, int64_t drow_stride, void* workspace, int64_t workspace_bytes, void* stream) {
+                  const float* weight, float* loss, void* dlogits, int64_t drow_stride, void* stream) {
   using namespace gn;
   GN_OP_BEGIN("op_distill", check_distill(dtype, rows, vocab, top, temperature, logits, row_stride, top_ids, index_type, top_logits, weight, loss, dlogits, drow_stride));
   if (rows == 0) return GN_OK;
-  if (!workspace || !aligned_to(workspace, 16) || workspace_bytes < distill_workspace(rows, top, dlogits != nullptr)) return fail(GN_ERR_INVALID_ARG, "op_distill: the workspace is too small, null or not aligned");
-  Teacher* teach = static_cast<Teacher*>(workspace); int* id = reinterpret_cast<int*>(teach + rows); float* prob = reinterpret_cast<float*>(id + rows * top);
-  const DistillParams p{logits, (long)row_stride, top_ids, index_type, top_logits, weight, loss, dlogits, (long)drow_stride, (long)rows, (long)vocab, top, temperature, teach, id, prob, prob + rows * top};
+  const DistillParams p{logits, (long)row_stride, top_ids, index_type, top_logits, weight, loss, dlogits, (long)drow_stride, (long)rows, (long)vocab, top, temperature};
   return with_type(dtype, [&](auto t) { using T = decltype(t); return dlogits ? distill_launch<T, true>(ctx, p, stream) : distill_launch<T, false>(ctx, p, stream); });
 }
 

@@ -172,11 +172,8 @@ std::tuple<Tensor, OptTensor> distill(uint64_t handle, int index, const Tensor& 
   const int top = (int)top_ids.size(1);
   Tensor loss = empty(top_logits, {n}); OptTensor grad;
   if (gradient) grad = out ? *out : empty(logits, logits.sizes());
-  int64_t need = 0;
-  check(gn_op_distill_workspace(d.ctx, n, top, gradient, &need));
-  Tensor ws = bytes(logits, need);
   check(gn_op_distill(d.ctx, dtype_of("logits", logits), n, vocab, top, (float)temperature, ptr(logits), logits.stride(0), ptr(top_ids), wide, (float*)ptr(top_logits), (float*)ptr(row_weight), (float*)ptr(loss), ptr(grad),
-                      gradient ? grad->stride(0) : 0, ptr(ws), need, d.stream()));
+                      gradient ? grad->stride(0) : 0, d.stream()));
   return {loss, grad};
 }
 

@@ -337,10 +337,9 @@ int gn_op_qk_norm_rope_backward(gn_ctx* ctx, int dtype, int64_t tokens, int head
  * positive probability, has loss 0 and gradient 0 whatever its logits hold.  logits [rows, vocab] and dlogits (null: loss only; may be
  * logits in place) of `dtype`, rows row_stride / drow_stride elements apart; top_ids [rows, top] of index_type, top_logits float32 [rows, top],
  * dense; weight float32 [rows] (null: 1); loss float32 [rows].  top <= 1024.  An index outside [-1, vocab) counts as -1 and sets the status. */
-int gn_op_distill_workspace(gn_ctx* ctx, int64_t rows, int top, int gradient, int64_t* bytes);      /* gradient: whether dlogits is given */
 int gn_op_distill(gn_ctx* ctx, int dtype, int64_t rows, int64_t vocab, int top, float temperature,
                   const void* logits, int64_t row_stride, const void* top_ids, int index_type, const float* top_logits,
-                  const float* weight, float* loss, void* dlogits, int64_t drow_stride, void* workspace, int64_t workspace_bytes, void* stream);
+                  const float* weight, float* loss, void* dlogits, int64_t drow_stride, void* stream);
 
 /* Embedding lookup: out[i] = scale * table[ids[i]], rows of zeros where ids[i] is -1.  table [vocab, dim] and out [tokens, dim] of
  * `dtype`, rows table_stride / out_stride elements apart.  An id outside [-1, vocab) counts as -1 and sets the status. */
