@@ -2,7 +2,7 @@
 //
 //   r = 1 / sqrt(mean(x^2) + eps),  y = R (g x r);     u = R^T dy,  dx = r (g u - x r^2 mean(g u x)),  dg = sum u x r
 //
-// R turns pairs of elements by position * frequency.  The angle is formed in 64 bits, in turns, and its whole turns are dropped there, so that
+// R turns pairs of elements by position * frequency.  The angle is formed in 64 bits, as a fraction of a turn, so that
 // a far position costs no accuracy; sine and cosine of what is left are float32, once per token and pair for all heads, in shared memory.
 // Everything between reading x (and dy) and the one rounding of the result is float32.
 //
@@ -18,58 +18,76 @@ struct QkParams {
   QkHeads t[2]; long tokens; int head, rot, inter; float eps; const void* pos; int index_type; const double* freq; float* partial;
 };
 
-// cosine and sine of the angle of (token, pair)
-__device__ __forceinline__ float2 qk_turn(const QkParams& p, long token, int pair) {
-  double turns = (double)load_index(p.pos, p.index_type, token) * __ldg(p.freq + pair) * 0.15915494309189533577;      // 1 / (2 pi)
-  turns -= rint(turns);
-  float s, c; sincospif(2.f * (float)turns, &s, &c);
-  return make_float2(c, s);
+// Frequencies in turns, as 64-bit fractions of one: a position times that, in wrapping arithmetic, drops whole turns without a rounding.  (The product and the whole turns in float64 for every token
+// and pair were a fifth of the forward pass's time.)
+__device__ __forceinline__ void qk_frequencies(const QkParams& p, unsigned long long* fx) {
+  for (int i = threadIdx.x; i < p.rot >> 1; i += blockDim.x) {
+    double f = __ldg(p.freq + i) * 0.15915494309189533577;           // 1 / (2 pi)
+    f -= floor(f);
+    fx[i] = (unsigned long long)(f * 18446744073709551616.0);
+  }
 }
-// ... of n tokens from `base` on: per token the cosines of all pairs, then the sines
-__device__ __forceinline__ void qk_turns(const QkParams& p, long base, int n, float* cs) {
+// cosines and sines of the angles of n tokens from `base` on: per token the cosines of all pairs, then the sines
+__device__ __forceinline__ void qk_turns(const QkParams& p, long base, int n, const unsigned long long* fx, float* cs) {
   const int half = p.rot >> 1;
-  for (int e = threadIdx.x; e < n * half; e += blockDim.x) { const int t = e / half, i = e - t * half; const float2 v = qk_turn(p, base + t, i); cs[t * p.rot + i] = v.x; cs[t * p.rot + half + i] = v.y; }
+  for (int e = threadIdx.x; e < n * half; e += blockDim.x) {
+    const int t = e / half, i = e - t * half;
+    const int turn = (int)((unsigned long long)load_index(p.pos, p.index_type, base + t) * fx[i] >> 32);      // of 2^32, from half a turn back to half a turn on
+    float s, c; sincospif((float)turn * 4.656612873077392578125e-10f, &s, &c);      // 2^-31
+    cs[t * p.rot + i] = c; cs[t * p.rot + half + i] = s;
+  }
 }
 __device__ __forceinline__ void rotate(float& a, float& b, float c, float s) { const float u = a * c - b * s; b = a * s + b * c; a = u; }
 
 // A lane's two pieces of a row: the halves of its pairs, or two neighbours behind the rotated part (interleaved: two neighbours everywhere), with the cosines and sines of
-// their pairs and the gain of their elements.  The same for all heads of a token, so that they stay in registers while a lane goes through QkTile::HB of them.
-template <class T> struct QkLane {
-  static constexpr int V = Vec<T>::N;
+// their pairs and the gain of their elements.  The same for all heads of a token, so that they stay in registers while a lane goes through several of them.
+// FULL: halves are rotated, all of a row, and the lanes of a group are exactly a row's, so that nothing needs asking.  Arithmetic goes two elements an instruction.
+template <class T, bool FULL> struct QkLane {
+  static constexpr int V = Vec<T>::N, P = V / 2;
   int pa, pb; bool has_a, has_b, split;
-  float ga[V], gb[V], c[V], s[V];
+  float2 ga[P], gb[P], c[P], s[P];                                   // cosines and sines of pairs 2 j, 2 j + 1
   __device__ __forceinline__ QkLane(const QkParams& p, int slot) {
     const int pieces = p.head / V, turned = (p.rot >> 1) / V;
-    split = !p.inter && slot < turned;
+    split = FULL || (!p.inter && slot < turned);
     pa = split ? slot : 2 * slot; pb = split ? slot + turned : 2 * slot + 1;
-    has_a = pa < pieces; has_b = pb < pieces;
+    has_a = FULL || pa < pieces; has_b = FULL || pb < pieces;
   }
   __device__ __forceinline__ void gain(const float* g) {
+    auto at = [&](bool has, int e) { return g && has ? __ldg(reinterpret_cast<const float2*>(g + e)) : make_float2(1.f, 1.f); };
+    if (reinterpret_cast<uintptr_t>(g) & 7) {                        // (a gain need only be aligned to its type)
 #pragma unroll
-    for (int j = 0; j < V; j++) { ga[j] = g && has_a ? __ldg(g + pa * V + j) : 1.f; gb[j] = g && has_b ? __ldg(g + pb * V + j) : 1.f; }
+      for (int j = 0; j < P; j++) {
+        ga[j] = has_a ? make_float2(__ldg(g + pa * V + 2 * j), __ldg(g + pa * V + 2 * j + 1)) : make_float2(1.f, 1.f);
+        gb[j] = has_b ? make_float2(__ldg(g + pb * V + 2 * j), __ldg(g + pb * V + 2 * j + 1)) : make_float2(1.f, 1.f);
+      }
+      return;
+    }
+#pragma unroll
+    for (int j = 0; j < P; j++) { ga[j] = at(has_a, pa * V + 2 * j); gb[j] = at(has_b, pb * V + 2 * j); }
   }
   __device__ __forceinline__ void turns(const QkParams& p, const float* cs, float sign) {      // cs: the token's
     const int half = p.rot >> 1;
     if (split) {
 #pragma unroll
-      for (int j = 0; j < V; j += 4) {
-        const float4 u = *reinterpret_cast<const float4*>(cs + pa * V + j), w = *reinterpret_cast<const float4*>(cs + half + pa * V + j);
-        c[j] = u.x; c[j + 1] = u.y; c[j + 2] = u.z; c[j + 3] = u.w; s[j] = sign * w.x; s[j + 1] = sign * w.y; s[j + 2] = sign * w.z; s[j + 3] = sign * w.w;
+      for (int j = 0; j < P; j += 2) {
+        const float4 u = *reinterpret_cast<const float4*>(cs + pa * V + 2 * j), w = *reinterpret_cast<const float4*>(cs + half + pa * V + 2 * j);
+        c[j] = make_float2(u.x, u.y); c[j + 1] = make_float2(u.z, u.w); s[j] = make_float2(sign * w.x, sign * w.y); s[j + 1] = make_float2(sign * w.z, sign * w.w);
       }
     } else if (p.inter) {
+      auto at = [&](int j) { const int i = (j < P ? pa : pb) * P + j % P; return i < half ? make_float2(cs[i], sign * cs[half + i]) : make_float2(1.f, 0.f); };
 #pragma unroll
-      for (int j = 0; j < V; j++) { const int i = (j < V / 2 ? pa : pb) * (V / 2) + j % (V / 2); c[j] = i < half ? cs[i] : 1.f; s[j] = i < half ? sign * cs[half + i] : 0.f; }
+      for (int j = 0; j < P; j++) { const float2 u = at(2 * j), w = at(2 * j + 1); c[j] = make_float2(u.x, w.x); s[j] = make_float2(u.y, w.y); }
     }
   }
-  __device__ __forceinline__ void turn(const QkParams& p, float (&a)[V], float (&b)[V]) const {
+  __device__ __forceinline__ void turn(const QkParams& p, float2 (&a)[P], float2 (&b)[P]) const {
     if (split) {
 #pragma unroll
-      for (int j = 0; j < V; j++) rotate(a[j], b[j], c[j], s[j]);
+      for (int j = 0; j < P; j++) { const float2 n = make_float2(-s[j].x, -s[j].y), u = fma2(b[j], n, mul2(a[j], c[j])); b[j] = fma2(b[j], c[j], mul2(a[j], s[j])); a[j] = u; }
     } else if (p.inter) {                                            // (elements that do not turn are left alone: 0 times an infinity is none)
 #pragma unroll
-      for (int j = 0; j < V / 2; j++) {
-        if (pa * V + 2 * j < p.rot) rotate(a[2 * j], a[2 * j + 1], c[j], s[j]);
-        if (pb * V + 2 * j < p.rot) rotate(b[2 * j], b[2 * j + 1], c[V / 2 + j], s[V / 2 + j]);
+      for (int j = 0; j < P; j++) {
+        if (pa * V + 2 * j < p.rot) rotate(a[j].x, a[j].y, j & 1 ? c[j / 2].y : c[j / 2].x, j & 1 ? s[j / 2].y : s[j / 2].x);
+        if (pb * V + 2 * j < p.rot) rotate(b[j].x, b[j].y, (P + j) & 1 ? c[(P + j) / 2].y : c[(P + j) / 2].x, (P + j) & 1 ? s[(P + j) / 2].y : s[(P + j) / 2].x);
       }
     }
   }
@@ -78,118 +96,133 @@ template <class T> struct QkLane {
     if (has_a) a = reinterpret_cast<const uint4*>(row)[pa];
     if (has_b) b = reinterpret_cast<const uint4*>(row)[pb];
   }
-  __device__ __forceinline__ void store(void* row, const float (&a)[V], const float (&b)[V]) const {
-    if (has_a) reinterpret_cast<uint4*>(row)[pa] = pack<T>(a);
-    if (has_b) reinterpret_cast<uint4*>(row)[pb] = pack<T>(b);
+  __device__ __forceinline__ static void open(const uint4& u, float2 (&v)[P]) {
+    float x[V]; unpack<T>(u, x);
+#pragma unroll
+    for (int j = 0; j < P; j++) v[j] = make_float2(x[2 * j], x[2 * j + 1]);
+  }
+  __device__ __forceinline__ static uint4 shut(const float2 (&v)[P]) {
+    float x[V];
+#pragma unroll
+    for (int j = 0; j < P; j++) { x[2 * j] = v[j].x; x[2 * j + 1] = v[j].y; }
+    return pack<T>(x);
+  }
+  __device__ __forceinline__ void store(void* row, const float2 (&a)[P], const float2 (&b)[P]) const {
+    if (has_a) reinterpret_cast<uint4*>(row)[pa] = shut(a);
+    if (has_b) reinterpret_cast<uint4*>(row)[pb] = shut(b);
   }
 };
 
 constexpr int QK_THREADS = 256;
-// A group of G lanes takes HB heads of one token at a time.  Forward: four, eight 16-byte loads of a lane under way; backward two, x and dy.  (One head at a time, with the cosines read from
-// shared memory for each: 129 us forward and 236 backward for 65536 tokens of 16 + 4 heads of 64, bf16; bound by instructions, 14 an element.)
-template <class T, int G, bool BWD>
+// A group of G lanes takes HB heads of one token at a time.  (One head at a time, with the cosines read from shared memory for each: 129 us forward and 236 backward for 65536 tokens of 16 + 4 heads of
+// 64, bf16; one element an instruction: 79 and 131.)
+template <class T, int G, bool BWD, bool FULL>
 __global__ void __launch_bounds__(QK_THREADS, QK_PER_SM) qk_vec_kernel(const __grid_constant__ QkParams p) {
-  constexpr int V = Vec<T>::N, GROUPS = QK_THREADS / G, HB = BWD ? QK_HEADS_BWD : QK_HEADS_FWD;
+  using Lane = QkLane<T, FULL>;
+  constexpr int V = Vec<T>::N, P = V / 2, GROUPS = QK_THREADS / G, HB = BWD ? QK_HEADS_BWD : QK_HEADS_FWD;
   op_begin();
   extern __shared__ float4 qk_smem[];
-  float* cs = reinterpret_cast<float*>(qk_smem);
+  unsigned long long* fx = reinterpret_cast<unsigned long long*>(qk_smem); float* cs = reinterpret_cast<float*>(fx) + ((p.rot + 3) & ~3);
   __shared__ float red[BWD ? QK_THREADS / 32 * G * 2 * V : 1];
   const int slot = threadIdx.x % G, g0 = threadIdx.x / G;
-  QkLane<T> lane(p, slot);
+  Lane lane(p, slot);
   const int kind = blockIdx.y; const QkHeads& h = p.t[kind];
   if (h.heads == 0) return;
-  {
-    const int per_token = (h.heads + HB - 1) / HB;
-    lane.gain(h.gain);
-    float acc[BWD ? 2 * V : 1];
-    if constexpr (BWD) {
+  const int per_token = (h.heads + HB - 1) / HB;
+  lane.gain(h.gain);
+  float2 acc[BWD ? 2 * P : 1];
+  if constexpr (BWD) {
 #pragma unroll
-      for (int j = 0; j < 2 * V; j++) acc[j] = 0.f;
-    }
-    for (long base = (long)blockIdx.x * h.per_block; base < p.tokens; base += (long)gridDim.x * h.per_block) {
-      const int n = (int)min((long)h.per_block, p.tokens - base), items = n * per_token;
-      for (int i0 = 0; i0 < items; i0 += GROUPS) {                   // (the same count for a whole block: barriers and shuffles want all of it)
-        const int i = i0 + g0; const bool on = i < items;
-        const int t = on ? i / per_token : 0, h0 = on ? (i - t * per_token) * HB : 0, heads = on ? min(HB, h.heads - h0) : 0;
-        const long tok = base + t;
-        const T* x = static_cast<const T*>(h.in) + tok * h.in_t + h0 * h.in_h;
-        uint4 ua[HB], ub[HB], wa[BWD ? HB : 1], wb[BWD ? HB : 1];
+    for (int j = 0; j < 2 * P; j++) acc[j] = make_float2(0.f, 0.f);
+  }
+  const float inv = 1.f / p.head;
+  qk_frequencies(p, fx);                                             // (seen behind the loop's first barrier)
+  for (long base = (long)blockIdx.x * h.per_block; base < p.tokens; base += (long)gridDim.x * h.per_block) {
+    const int n = (int)min((long)h.per_block, p.tokens - base), items = n * per_token;
+    int t0 = g0 / per_token, hb0 = g0 - t0 * per_token;              // (token, block of heads) of this group's item
+    for (int i0 = 0; i0 < items; i0 += GROUPS) {                     // (the same count for a whole block: barriers and shuffles want all of it)
+      if (i0 > 0) { const int i = i0 + g0; t0 = i / per_token; hb0 = i - t0 * per_token; }
+      const bool on = t0 < n; const int t = on ? t0 : 0, h0 = on ? hb0 * HB : 0, heads = on ? min(HB, h.heads - h0) : 0;
+      const long tok = base + t;
+      const T* x = static_cast<const T*>(h.in) + tok * h.in_t + h0 * h.in_h;
+      uint4 ua[HB], ub[HB], wa[BWD ? HB : 1], wb[BWD ? HB : 1];
+#pragma unroll
+      for (int q = 0; q < HB; q++) {
+        ua[q] = ub[q] = make_uint4(0, 0, 0, 0);
+        if (q < heads) lane.load(x + q * h.in_h, ua[q], ub[q]);
+      }
+      if constexpr (BWD) {
+        const T* d = static_cast<const T*>(h.dy) + tok * h.dy_t + h0 * h.dy_h;
 #pragma unroll
         for (int q = 0; q < HB; q++) {
-          ua[q] = ub[q] = make_uint4(0, 0, 0, 0);
-          if (q < heads) lane.load(x + q * h.in_h, ua[q], ub[q]);
+          wa[q] = wb[q] = make_uint4(0, 0, 0, 0);
+          if (q < heads) lane.load(d + q * h.dy_h, wa[q], wb[q]);
         }
-        if constexpr (BWD) {
-          const T* d = static_cast<const T*>(h.dy) + tok * h.dy_t + h0 * h.dy_h;
+      }
+      if (i0 == 0) {                                                 // under the loads
+        __syncthreads();
+        qk_turns(p, base, n, fx, cs);
+        __syncthreads();
+      }
+      lane.turns(p, cs + t * p.rot, BWD ? -1.f : 1.f);
+      T* o = static_cast<T*>(h.out) + tok * h.out_t + h0 * h.out_h;
 #pragma unroll
-          for (int q = 0; q < HB; q++) {
-            wa[q] = wb[q] = make_uint4(0, 0, 0, 0);
-            if (q < heads) lane.load(d + q * h.dy_h, wa[q], wb[q]);
+      for (int q = 0; q < HB; q++) {
+        float2 a[P], b[P]; Lane::open(ua[q], a); Lane::open(ub[q], b);
+        float2 s2 = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int j = 0; j < P; j++) { s2 = fma2(a[j], a[j], s2); s2 = fma2(b[j], b[j], s2); }
+        float ss = s2.x + s2.y;
+        if constexpr (!BWD) {
+#pragma unroll
+          for (int m = G / 2; m > 0; m >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
+          const float rs = rsqrtf(fmaf(ss, inv, p.eps)); const float2 r2 = make_float2(rs, rs);
+#pragma unroll
+          for (int j = 0; j < P; j++) { a[j] = mul2(a[j], lane.ga[j]); b[j] = mul2(b[j], lane.gb[j]); }
+          lane.turn(p, a, b);
+#pragma unroll
+          for (int j = 0; j < P; j++) { a[j] = mul2(a[j], r2); b[j] = mul2(b[j], r2); }
+          if (q < heads) lane.store(o + q * h.out_h, a, b);
+        } else {
+          float2 ya[P], yb[P]; Lane::open(wa[q], ya); Lane::open(wb[q], yb);
+          lane.turn(p, ya, yb);
+          float2 x2 = make_float2(0.f, 0.f);
+#pragma unroll
+          for (int j = 0; j < P; j++) { x2 = fma2(mul2(ya[j], lane.ga[j]), a[j], x2); x2 = fma2(mul2(yb[j], lane.gb[j]), b[j], x2); }
+          float sx = x2.x + x2.y;
+#pragma unroll
+          for (int m = G / 2; m > 0; m >>= 1) { ss += __shfl_xor_sync(0xffffffffu, ss, m); sx += __shfl_xor_sync(0xffffffffu, sx, m); }
+          const float rs = rsqrtf(fmaf(ss, inv, p.eps)), m = -rs * rs * (sx * inv); const float2 r2 = make_float2(rs, rs), m2 = make_float2(m, m);
+#pragma unroll
+          for (int j = 0; j < P; j++) {
+            acc[j] = fma2(ya[j], mul2(a[j], r2), acc[j]); acc[P + j] = fma2(yb[j], mul2(b[j], r2), acc[P + j]);      // (rows that are not there have zeros)
+            ya[j] = mul2(r2, fma2(a[j], m2, mul2(ya[j], lane.ga[j]))); yb[j] = mul2(r2, fma2(b[j], m2, mul2(yb[j], lane.gb[j])));
           }
-        }
-        if (i0 == 0) {                                               // under the loads
-          __syncthreads();
-          qk_turns(p, base, n, cs);
-          __syncthreads();
-        }
-        lane.turns(p, cs + t * p.rot, BWD ? -1.f : 1.f);
-        T* o = static_cast<T*>(h.out) + tok * h.out_t + h0 * h.out_h;
-#pragma unroll
-        for (int q = 0; q < HB; q++) {
-          float a[V], b[V]; unpack<T>(ua[q], a); unpack<T>(ub[q], b);
-          float ss = 0.f;
-#pragma unroll
-          for (int j = 0; j < V; j++) { ss = fmaf(a[j], a[j], ss); ss = fmaf(b[j], b[j], ss); }
-          if constexpr (!BWD) {
-#pragma unroll
-            for (int m = G / 2; m > 0; m >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
-            const float rs = rsqrtf(ss / p.head + p.eps);
-#pragma unroll
-            for (int j = 0; j < V; j++) { a[j] *= lane.ga[j]; b[j] *= lane.gb[j]; }
-            lane.turn(p, a, b);
-#pragma unroll
-            for (int j = 0; j < V; j++) { a[j] *= rs; b[j] *= rs; }
-            if (q < heads) lane.store(o + q * h.out_h, a, b);
-          } else {
-            float ya[V], yb[V]; unpack<T>(wa[q], ya); unpack<T>(wb[q], yb);
-            lane.turn(p, ya, yb);
-            float sx = 0.f;
-#pragma unroll
-            for (int j = 0; j < V; j++) { sx = fmaf(ya[j] * lane.ga[j], a[j], sx); sx = fmaf(yb[j] * lane.gb[j], b[j], sx); }
-#pragma unroll
-            for (int m = G / 2; m > 0; m >>= 1) { ss += __shfl_xor_sync(0xffffffffu, ss, m); sx += __shfl_xor_sync(0xffffffffu, sx, m); }
-            const float rs = rsqrtf(ss / p.head + p.eps), m = rs * rs * (sx / p.head);
-#pragma unroll
-            for (int j = 0; j < V; j++) {
-              acc[j] = fmaf(ya[j], a[j] * rs, acc[j]); acc[V + j] = fmaf(yb[j], b[j] * rs, acc[V + j]);      // (rows that are not there have zeros)
-              ya[j] = rs * fmaf(-a[j], m, ya[j] * lane.ga[j]); yb[j] = rs * fmaf(-b[j], m, yb[j] * lane.gb[j]);
-            }
-            if (q < heads) lane.store(o + q * h.out_h, ya, yb);
-          }
+          if (q < heads) lane.store(o + q * h.out_h, ya, yb);
         }
       }
     }
-    if constexpr (BWD) {
-      if (!p.partial) return;
+  }
+  if constexpr (BWD) {
+    if (!p.partial) return;
 #pragma unroll
-      for (int m = 16; m >= G; m >>= 1) {
+    for (int m = 16; m >= G; m >>= 1) {
 #pragma unroll
-        for (int j = 0; j < 2 * V; j++) acc[j] += __shfl_xor_sync(0xffffffffu, acc[j], m);
-      }
-      const int warp = threadIdx.x >> 5;
-      __syncthreads();
-      if ((threadIdx.x & 31) < G) {
+      for (int j = 0; j < 2 * P; j++) { acc[j].x += __shfl_xor_sync(0xffffffffu, acc[j].x, m); acc[j].y += __shfl_xor_sync(0xffffffffu, acc[j].y, m); }
+    }
+    const int warp = threadIdx.x >> 5;
+    __syncthreads();
+    if ((threadIdx.x & 31) < G) {
 #pragma unroll
-        for (int j = 0; j < 2 * V; j++) red[(warp * G + slot) * 2 * V + j] = acc[j];
-      }
-      __syncthreads();
-      float* out = p.partial + ((long)blockIdx.x * 2 + kind) * p.head;
-      for (int e = threadIdx.x; e < G * 2 * V; e += QK_THREADS) {
-        const int j = e % (2 * V); const QkLane<T> of(p, e / (2 * V)); const int piece = j < V ? of.pa : of.pb;
-        float v = 0.f;
-        for (int w = 0; w < QK_THREADS / 32; w++) v += red[w * G * 2 * V + e];
-        if (piece * V < p.head) out[piece * V + j % V] = v;
-      }
+      for (int j = 0; j < 2 * P; j++) { red[(warp * G + slot) * 2 * V + 2 * j] = acc[j].x; red[(warp * G + slot) * 2 * V + 2 * j + 1] = acc[j].y; }
+    }
+    __syncthreads();
+    float* out = p.partial + ((long)blockIdx.x * 2 + kind) * p.head;
+    for (int e = threadIdx.x; e < G * 2 * V; e += QK_THREADS) {
+      const int j = e % (2 * V); const Lane of(p, e / (2 * V)); const int piece = j < V ? of.pa : of.pb;
+      float v = 0.f;
+      for (int w = 0; w < QK_THREADS / 32; w++) v += red[w * G * 2 * V + e];
+      if (piece * V < p.head) out[piece * V + j % V] = v;
     }
   }
 }
@@ -200,10 +233,11 @@ template <class T, bool BWD>
 __global__ void __launch_bounds__(32 * QK_ROW_WARPS) qk_rows_kernel(const __grid_constant__ QkParams p) {
   op_begin();
   extern __shared__ float4 qk_smem[];
-  float* cs = reinterpret_cast<float*>(qk_smem);
+  unsigned long long* fx = reinterpret_cast<unsigned long long*>(qk_smem); float* cs = reinterpret_cast<float*>(fx) + ((p.rot + 3) & ~3);
   const int half = p.rot >> 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int kind = blockIdx.y; const QkHeads& h = p.t[kind];
   if (h.heads == 0) return;
+  qk_frequencies(p, fx);
   float* acc = cs + h.per_block * p.rot + warp * p.head;             // this warp's share of the gain's gradient; an element belongs to one lane
   {
     auto first = [&](int i) { return p.inter ? 2 * i : i; };
@@ -216,7 +250,7 @@ __global__ void __launch_bounds__(32 * QK_ROW_WARPS) qk_rows_kernel(const __grid
     for (long base = (long)blockIdx.x * h.per_block; base < p.tokens; base += (long)gridDim.x * h.per_block) {
       const int n = (int)min((long)h.per_block, p.tokens - base), rows = n * h.heads;
       __syncthreads();
-      qk_turns(p, base, n, cs);
+      qk_turns(p, base, n, fx, cs);
       __syncthreads();
       for (int r = warp; r < rows; r += QK_ROW_WARPS) {
         const int t = r / h.heads, hd = r - t * h.heads;
@@ -285,6 +319,11 @@ __global__ void __launch_bounds__(1024) qk_gain_kernel(const float* __restrict__
   if (lane == 0 && out < 2 * head) { float* d = out < head ? dq : dk; if (d) d[out < head ? out : out - head] = v; }
 }
 
+template <class T, int G, bool BWD>
+inline int qk_launch_vec(const QkParams& p, dim3 grid, size_t turns, void* stream) {
+  const bool full = !p.inter && p.rot == p.head && p.head == 2 * G * Vec<T>::N;
+  return op_launch("qk_vec", stream, full ? qk_vec_kernel<T, G, BWD, true> : qk_vec_kernel<T, G, BWD, false>, grid, dim3(QK_THREADS), turns, 0, p);
+}
 // Sets the tokens of a block and launches; *blocks: partial sums that the gradient of a gain leaves.
 template <class T, bool BWD>
 inline int qk_launch(QkParams p, int group, int sms, void* stream, unsigned* blocks) {
@@ -295,14 +334,14 @@ inline int qk_launch(QkParams p, int group, int sms, void* stream, unsigned* blo
   }
   *blocks = (unsigned)n;
   const dim3 grid((unsigned)n, p.t[1].heads ? 2 : 1);
-  const size_t turns = (size_t)most * p.rot * sizeof(float);         // at most 32 KB
+  const size_t turns = ((size_t)most * p.rot + ((p.rot + 3) & ~3)) * sizeof(float);      // at most 36 KB
   switch (group) {
     case 0: return op_launch("qk_rows", stream, qk_rows_kernel<T, BWD>, grid, dim3(32 * QK_ROW_WARPS), turns + (BWD ? (size_t)QK_ROW_WARPS * p.head * sizeof(float) : 0), 0, p);
-    case 2: return op_launch("qk_vec", stream, qk_vec_kernel<T, 2, BWD>, grid, dim3(QK_THREADS), turns, 0, p);
-    case 4: return op_launch("qk_vec", stream, qk_vec_kernel<T, 4, BWD>, grid, dim3(QK_THREADS), turns, 0, p);
-    case 8: return op_launch("qk_vec", stream, qk_vec_kernel<T, 8, BWD>, grid, dim3(QK_THREADS), turns, 0, p);
-    case 16: return op_launch("qk_vec", stream, qk_vec_kernel<T, 16, BWD>, grid, dim3(QK_THREADS), turns, 0, p);
-    default: return op_launch("qk_vec", stream, qk_vec_kernel<T, 32, BWD>, grid, dim3(QK_THREADS), turns, 0, p);
+    case 2: return qk_launch_vec<T, 2, BWD>(p, grid, turns, stream);
+    case 4: return qk_launch_vec<T, 4, BWD>(p, grid, turns, stream);
+    case 8: return qk_launch_vec<T, 8, BWD>(p, grid, turns, stream);
+    case 16: return qk_launch_vec<T, 16, BWD>(p, grid, turns, stream);
+    default: return qk_launch_vec<T, 32, BWD>(p, grid, turns, stream);
   }
 }
 inline QkHeads qk_heads(const gn_heads* x, const gn_heads* dy, const gn_heads* out, const float* gain) {
