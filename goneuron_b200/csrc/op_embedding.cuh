@@ -36,7 +36,7 @@ __global__ void __launch_bounds__(256) embedding_kernel(const T* __restrict__ ta
           float v[Vec<T>::N]; unpack<T>(u[j], v);
 #pragma unroll
           for (int k = 0; k < Vec<T>::N; k++) v[k] = there ? v[k] * scale : 0.f;
-          if (e0 + 32 * j < n) reinterpret_cast<uint4*>(dst)[e0 + 32 * j] = pack<T>(v);
+          if (e0 + 32 * j < n) __stcs(reinterpret_cast<uint4*>(dst) + e0 + 32 * j, pack<T>(v));      // (the table's rows are read again, these are not)
         }
       }
     }
@@ -116,7 +116,7 @@ constexpr int SORT_SMALL_SMEM = (SORT_SMALL_THREADS / 32 * 256 + 2 * SORT_SMALL)
 // moves its tokens there.  FIRST: keys come from the ids and places are the tokens' own.
 constexpr int SORT_THREADS = 256;
 template <bool FIRST>
-__global__ void __launch_bounds__(SORT_THREADS) sort_count_kernel(const void* __restrict__ ids, int index_type, const unsigned* __restrict__ keys, long tokens, long vocab, int shift, unsigned* __restrict__ hist) {
+__global__ void __launch_bounds__(SORT_THREADS) sort_count_kernel(const void* __restrict__ ids, int index_type, const unsigned* __restrict__ keys, long tokens, long vocab, int shift, bool by_tile, unsigned* __restrict__ hist) {
   op_begin();
   __shared__ unsigned cnt[256];
   cnt[threadIdx.x] = 0;
@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_count_kernel(const void* __
     if (i < tokens) atomicAdd(&cnt[((FIRST ? token_key(ids, index_type, i, vocab) : __ldg(keys + i)) >> shift) & 255], 1u);
   }
   __syncthreads();
-  hist[(long)threadIdx.x * gridDim.x + blockIdx.x] = cnt[threadIdx.x];      // digit by digit
+  hist[by_tile ? blockIdx.x * 256L + threadIdx.x : (long)threadIdx.x * gridDim.x + blockIdx.x] = cnt[threadIdx.x];      // digit by digit for the scan
 }
 // In place: every count becomes the sum of those before it.  One block.
 __global__ void __launch_bounds__(1024) sort_scan_kernel(unsigned* __restrict__ hist, long n) {
@@ -158,7 +158,8 @@ __global__ void __launch_bounds__(1024) sort_scan_kernel(unsigned* __restrict__ 
     __syncthreads();
   }
 }
-template <bool FIRST>
+// SCAN: the counts are as sort_count_kernel left them, and every tile adds up what lies before its own (few tiles: a launch less a pass).
+template <bool FIRST, bool SCAN>
 __global__ void __launch_bounds__(SORT_THREADS) sort_move_kernel(const void* __restrict__ ids, int index_type, const unsigned* __restrict__ keys, const int* __restrict__ order, long tokens, long vocab, int shift,
                                                                  const unsigned* __restrict__ hist, unsigned* __restrict__ keys_out, int* __restrict__ order_out) {
   constexpr int W = SORT_THREADS / 32, PER = SORT_TILE / SORT_THREADS;      // rows of 32 places of a warp
@@ -178,7 +179,20 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_move_kernel(const void* __r
 #pragma unroll
   for (int j = 0; j < PER; j++) if (first + j * 32 + lane < tokens) atomicAdd(&cnt[warp * 256 + ((key[j] >> shift) & 255)], 1u);
   __syncthreads();
-  unsigned at0 = __ldg(hist + (long)tid * gridDim.x + blockIdx.x);   // thread = digit
+  unsigned at0;                                                      // thread = digit: where this tile's begin
+  if constexpr (SCAN) {
+    __shared__ unsigned sums[W];
+    unsigned before = 0, total = 0;
+#pragma unroll 32
+    for (int t = 0; t < (int)gridDim.x; t++) { const unsigned c = __ldg(hist + t * 256 + tid); if (t < (int)blockIdx.x) before += c; total += c; }
+    unsigned s = total;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) { const unsigned u = __shfl_up_sync(0xffffffffu, s, o); if (lane >= o) s += u; }
+    if (lane == 31) sums[warp] = s;
+    __syncthreads();
+    for (int w = 0; w < warp; w++) s += sums[w];
+    at0 = s - total + before;
+  } else at0 = __ldg(hist + (long)tid * gridDim.x + blockIdx.x);
 #pragma unroll
   for (int w = 0; w < W; w++) { const unsigned c = cnt[w * 256 + tid]; cnt[w * 256 + tid] = at0; at0 += c; }
   __syncthreads();
@@ -269,52 +283,66 @@ __global__ void __launch_bounds__(EMB_THREADS) embedding_sum_kernel(const T* __r
     }
   }
 }
-// A run that goes on over the end of the piece where it began: that piece's last sum, then the first sums of the pieces behind it up to the one where the run ends.
-// Most blocks find no such run and leave after three independent loads.  (Looking the run's end up by bisection, and 32 columns of a block at a time: 127 us of a gradient over
-// 131072 tokens whose other launches take 100.)  Four threads a column, each a run of neighbouring pieces, added in order; V columns of a thread.
-constexpr int JOIN_COLS = 64;
+// A run that goes on over the end of the piece where it began: that piece's last sum, then the first sums of the pieces behind it up to the one where the run ends.  Most runs end in the next piece:
+// two warps look at a piece and add a run's parts, V columns a lane, in order; a run of more than JOIN_LONG pieces is left to the whole block, a quarter of its pieces to each two warps.  (A block for every
+// piece: 18 us for 131072 tokens of 1024; looking the run's end up by bisection and 32 columns at a time: 127.)
+constexpr int JOIN_COLS = 64, JOIN_GROUPS = 4, JOIN_LONG = 32;
 template <int V>
-__global__ void __launch_bounds__(4 * JOIN_COLS) embedding_join_kernel(const unsigned* __restrict__ keys, long tokens, long vocab, int dim, int chunk, long chunks, const float* __restrict__ partial, float* __restrict__ dtable) {
+__global__ void __launch_bounds__(JOIN_GROUPS * JOIN_COLS) embedding_join_kernel(const unsigned* __restrict__ keys, long tokens, long vocab, int dim, int chunk, long chunks, const float* __restrict__ partial, float* __restrict__ dtable) {
   op_begin();
-  __shared__ float red[3][JOIN_COLS * V];
-  __shared__ int found;
-  const long c = blockIdx.x, end = (c + 1) * chunk;                  // (a last piece has nothing behind it: the launch leaves it out)
-  const unsigned key = __ldg(keys + end - 1), next = __ldg(keys + end), begin = __ldg(keys + c * chunk), before = c > 0 ? __ldg(keys + c * chunk - 1) : 0xffffffffu;
-  if (key >= (unsigned)vocab || next != key || (begin == key && before == key)) return;      // no row, no run over the end, or one that began before
-  long m = 1;                                                        // pieces behind this one that begin within the run
-  for (long i0 = c + 1;; i0 += blockDim.x) {
-    if (threadIdx.x == 0) found = 0x7fffffff;
-    __syncthreads();
-    const long i = i0 + threadIdx.x;
-    if (i >= chunks || __ldg(keys + i * chunk) != key) atomicMin(&found, (int)threadIdx.x);
-    __syncthreads();
-    const int f = found;
-    __syncthreads();
-    if (f != 0x7fffffff) { m = i0 + f - c - 1; break; }
+  __shared__ float red[JOIN_GROUPS - 1][JOIN_COLS * V];
+  __shared__ long length[JOIN_GROUPS]; __shared__ unsigned key_of[JOIN_GROUPS];
+  const int w = threadIdx.x / JOIN_COLS, lane = threadIdx.x % JOIN_COLS; const long col = ((long)blockIdx.y * JOIN_COLS + lane) * V; const bool in = col < dim;
+  const long c0 = (long)blockIdx.x * JOIN_GROUPS, c = c0 + w;
+  long m = 0;                                                        // pieces behind this one that begin within a run which began here
+  unsigned key = 0;
+  if (c + 1 < chunks) {                                              // (a last piece has nothing behind it)
+    key = __ldg(keys + (c + 1) * chunk - 1);
+    const unsigned next = __ldg(keys + (c + 1) * chunk), begin = __ldg(keys + c * chunk), before = c > 0 ? __ldg(keys + c * chunk - 1) : 0xffffffffu;
+    if (key < (unsigned)vocab && next == key && !(begin == key && before == key))
+      for (long i0 = c + 2;; i0 += 32) {                             // the first piece behind that does not begin within the run
+        const long i = i0 + (threadIdx.x & 31);
+        const unsigned other = __ballot_sync(0xffffffffu, i >= chunks || __ldg(keys + i * chunk) != key);
+        if (other) { m = i0 + __ffs(other) - 1 - c - 1; break; }
+      }
   }
-  const int w = threadIdx.x / JOIN_COLS, lane = threadIdx.x % JOIN_COLS; const long per = (m + 3) / 4, col = ((long)blockIdx.y * JOIN_COLS + lane) * V; const bool in = col < dim;
-  float v[V];
-#pragma unroll
-  for (int j = 0; j < V; j++) v[j] = 0.f;
-  auto add = [&](const float* row) {
+  auto add = [&](float (&v)[V], const float* row) {
     if constexpr (V == 1) v[0] += __ldg(row + col);
     else { const float4 u = __ldg(reinterpret_cast<const float4*>(row + col)); v[0] += u.x; v[1] += u.y; v[2] += u.z; v[3] += u.w; }
   };
-  if (in) {
-    if (w == 0) add(partial + (2 * c + 1) * dim);
-#pragma unroll 8
-    for (long i = w * per; i < min(m, (w + 1) * per); i++) add(partial + 2 * (c + 1 + i) * dim);
-  }
-  if (w > 0) {
-#pragma unroll
-    for (int j = 0; j < V; j++) red[w - 1][lane * V + j] = v[j];
-  }
-  __syncthreads();
-  if (w == 0 && in) {
-    float* out = dtable + (long)key * dim + col;
-#pragma unroll
-    for (int j = 0; j < V; j++) { for (int i = 0; i < 3; i++) v[j] += red[i][lane * V + j]; }
+  auto put = [&](const float (&v)[V], unsigned k) {
+    float* out = dtable + (long)k * dim + col;
     if constexpr (V == 1) *out = v[0]; else *reinterpret_cast<float4*>(out) = make_float4(v[0], v[1], v[2], v[3]);
+  };
+  if (m > 0 && m <= JOIN_LONG && in) {
+    float v[V] = {};
+    add(v, partial + (2 * c + 1) * dim);
+#pragma unroll 4
+    for (long i = 0; i < m; i++) add(v, partial + 2 * (c + 1 + i) * dim);
+    put(v, key);
+  }
+  if (lane == 0) { length[w] = m; key_of[w] = key; }
+  if (!__syncthreads_or(m > JOIN_LONG)) return;
+  for (int g = 0; g < JOIN_GROUPS; g++) {
+    const long n = length[g], p = c0 + g, per = (n + JOIN_GROUPS - 1) / JOIN_GROUPS;
+    if (n <= JOIN_LONG) continue;
+    float v[V] = {};
+    if (in) {
+      if (w == 0) add(v, partial + (2 * p + 1) * dim);
+#pragma unroll 8
+      for (long i = w * per; i < min(n, (w + 1) * per); i++) add(v, partial + 2 * (p + 1 + i) * dim);
+    }
+    if (w > 0) {
+#pragma unroll
+      for (int j = 0; j < V; j++) red[w - 1][lane * V + j] = v[j];
+    }
+    __syncthreads();
+    if (w == 0 && in) {
+#pragma unroll
+      for (int j = 0; j < V; j++) for (int i = 0; i < JOIN_GROUPS - 1; i++) v[j] += red[i][lane * V + j];
+      put(v, key_of[g]);
+    }
+    __syncthreads();
   }
 }
 
@@ -330,8 +358,8 @@ inline int embedding_sums(const EmbeddingPlan& pl, const void* dout, long stride
   else GN_TRY(op_launch("embedding_sum", stream, embedding_sum_kernel<T, 1>, grid, dim3(EMB_THREADS), 0, 0, static_cast<const T*>(dout), stride, keys, order, tokens, vocab, dim, scale, pl.chunk, (long)pl.chunks, dtable, partial));
   if (pl.chunks < 2) return GN_OK;
   const bool vec4 = dim % 4 == 0 && aligned_to(dtable, 16);
-  const dim3 join((unsigned)(pl.chunks - 1), (unsigned)ceil_div(dim, JOIN_COLS * (vec4 ? 4 : 1)));
-  return op_launch("embedding_join", stream, vec4 ? embedding_join_kernel<4> : embedding_join_kernel<1>, join, dim3(4 * JOIN_COLS), 0, 0, keys, tokens, vocab, dim, pl.chunk, (long)pl.chunks, (const float*)partial, dtable);
+  const dim3 join((unsigned)ceil_div(pl.chunks - 1, JOIN_GROUPS), (unsigned)ceil_div(dim, JOIN_COLS * (vec4 ? 4 : 1)));
+  return op_launch("embedding_join", stream, vec4 ? embedding_join_kernel<4> : embedding_join_kernel<1>, join, dim3(JOIN_GROUPS * JOIN_COLS), 0, 0, keys, tokens, vocab, dim, pl.chunk, (long)pl.chunks, (const float*)partial, dtable);
 }
 
 }  // namespace gn
@@ -379,10 +407,10 @@ int gn_op_embedding_backward(gn_ctx* ctx, int dtype, int64_t tokens, int64_t voc
       const bool to_first = (pl.passes - pass) % 2 == 1;
       const unsigned* kin = u(to_first ? pl.keys2 : pl.keys); const int* vin = (const int*)u(to_first ? pl.order2 : pl.order);
       unsigned* kout = u(to_first ? pl.keys : pl.keys2); int* vout = (int*)u(to_first ? pl.order : pl.order2);
-      const int shift = pass * SORT_BITS;
-      GN_TRY(op_launch("sort_count", stream, pass == 0 ? sort_count_kernel<true> : sort_count_kernel<false>, grid, block, 0, 0, ids, index_type, kin, (long)tokens, (long)vocab, shift, u(pl.hist)));
-      GN_TRY(op_launch("sort_scan", stream, sort_scan_kernel, dim3(1), dim3(1024), 0, 0, u(pl.hist), (long)(pl.tiles << SORT_BITS)));
-      GN_TRY(op_launch("sort_move", stream, pass == 0 ? sort_move_kernel<true> : sort_move_kernel<false>, grid, block, 0, 0, ids, index_type, kin, vin, (long)tokens, (long)vocab, shift, (const unsigned*)u(pl.hist), kout, vout));
+      const int shift = pass * SORT_BITS; const bool scan = pl.tiles <= SORT_SCAN_TILES;
+      GN_TRY(op_launch("sort_count", stream, pass == 0 ? sort_count_kernel<true> : sort_count_kernel<false>, grid, block, 0, 0, ids, index_type, kin, (long)tokens, (long)vocab, shift, scan, u(pl.hist)));
+      if (!scan) GN_TRY(op_launch("sort_scan", stream, sort_scan_kernel, dim3(1), dim3(1024), 0, 0, u(pl.hist), (long)(pl.tiles << SORT_BITS)));
+      GN_TRY(op_launch("sort_move", stream, pass == 0 ? (scan ? sort_move_kernel<true, true> : sort_move_kernel<true, false>) : scan ? sort_move_kernel<false, true> : sort_move_kernel<false, false>, grid, block, 0, 0, ids, index_type, kin, vin, (long)tokens, (long)vocab, shift, (const unsigned*)u(pl.hist), kout, vout));
     }
   }
   return with_type(dtype, [&](auto t) { using T = decltype(t); return embedding_sums<T>(pl, dout, (long)dout_stride, ws, (long)tokens, (long)vocab, dim, scale, dtable, stream); });

@@ -122,7 +122,7 @@ inline const char* check_embedding(int dtype, int64_t tokens, int64_t vocab, int
 }
 // The tokens' order by id, then sums of it in pieces of `chunk` neighbouring places.  Up to SORT_SMALL tokens one block sorts them in shared memory; above, passes of
 // 8 bits over tiles of SORT_TILE tokens.
-constexpr int SORT_SMALL = 8192, SORT_TILE = 2048, SORT_BITS = 8;
+constexpr int SORT_SMALL = 8192, SORT_TILE = 2048, SORT_BITS = 8, SORT_SCAN_TILES = 128;      // SCAN_TILES: up to so many tiles add up the others' counts themselves
 struct EmbeddingPlan {
   bool small; int bits, passes, chunk; int64_t tiles, chunks;
   int64_t keys, order, keys2, order2, hist, partial, bytes;          // places in the workspace, in bytes

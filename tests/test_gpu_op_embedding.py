@@ -30,11 +30,11 @@ def _check(dev, ids, vocab, dim, type, scale, dout=None):
     d = ops.embedding_backward(dev, dout, ids, vocab, scale=scale)
     rows = dout.reshape(-1, dim).double()[there] * scale
     want, size = (torch.zeros(vocab, dim, dtype=torch.float64, device="cuda").index_add_(0, flat[there], r) for r in (rows, rows.abs()))
-    # a row's sum: the additions of a piece of 4 to 64 places (as embedding_plan cuts them), then those of a quarter of the pieces, and four more; two products
+    # a row's sum: the additions of a piece of 4 to 64 places (as embedding_plan cuts them), then those of up to 32 pieces or a quarter of them all, and four more; two products
     chunk = 4
     while chunk < 64 and flat.numel() > chunk * 8 * 148:
         chunk *= 2
-    longest = chunk + flat.numel() / chunk / 4 + 8
+    longest = chunk + max(32, flat.numel() / chunk / 4) + 8
     assert_near(d, want, 2.0 ** -24 * longest * size, "dtable")
     assert torch.equal(d, ops.embedding_backward(dev, dout, ids, vocab, scale=scale))
     return out, d
@@ -42,7 +42,7 @@ def _check(dev, ids, vocab, dim, type, scale, dout=None):
 
 @pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("tokens,vocab,dim", [(1, 1, 1), (1, 50000, 64), (2, 3, 8), (31, 17, 300), (33, 255, 64), (1000, 256, 24), (1024, 257, 33), (4737, 700, 40), (8192, 65535, 16), (8193, 65536, 16),
-                                              (20000, 5, 1032), (30001, 300, 12), (70000, 32000, 8)])
+                                              (20000, 5, 1032), (30001, 300, 12), (70000, 32000, 8), (262144, 4000, 8), (262145, 70000, 8)])
 def test_against_float64(dev, type, tokens, vocab, dim):
     gen = torch.Generator("cuda").manual_seed(tokens)
     ids = (torch.rand(tokens, device="cuda", generator=gen) ** 2 * vocab).long().clamp_(max=vocab - 1)
