@@ -51,6 +51,10 @@ inline const char* check_qk(const QkArgs& a) {
   if (const char* e = check_heads(a, a.q, a.q->heads, false)) return e;
   return a.k ? check_heads(a, a.k, a.k->heads, false) : nullptr;
 }
+// In place, a row has to be written where it was read.
+inline const char* check_in_place(const gn_heads* in, const gn_heads* out) {
+  return in && out && in->data && in->data == out->data && (in->token_stride != out->token_stride || in->head_stride != out->head_stride) ? "in place, both tensors' strides have to be the same" : nullptr;
+}
 // Groups of lanes: a lane has two 16-byte pieces of a row, and a row's lanes are neighbours, 2 to 32 of them.  0: the row goes element by element
 // (sizes, strides or pointers that 16-byte pieces do not fit, pairs that end inside one, rows of more than 64 pieces).
 inline int qk_group(int dtype, int head_size, int rotated, bool interleaved, const gn_heads* const* t, int n) {

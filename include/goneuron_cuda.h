@@ -315,7 +315,7 @@ typedef struct gn_heads {
  * R turning the pair (x[i], x[i + rotated/2]) -- interleaved: (x[2i], x[2i + 1]) -- of the first `rotated` elements by
  * position * frequencies[i]; the others stay.  The angle is formed and reduced in 64 bits.  q, k -> q_out, k_out of the same
  * heads (in place where pointer and strides are the same); k and k_out may both be null.  gain_q, gain_k: float32 [head_size],
- * null for 1.  positions: [tokens] of index_type; frequencies: float64 [rotated / 2]; both may be null where rotated is 0.
+ * null for 1.  positions: [tokens] of index_type; frequencies: float64 [rotated / 2], finite; both may be null where rotated is 0.
  * head_size <= 1024; rotated even, <= head_size.  The rotation is that of TransformerBlock with useRoPE (transformer.go:212-236). */
 int gn_op_qk_norm_rope(gn_ctx* ctx, int dtype, int64_t tokens, int head_size, int rotated, int interleaved, float eps,
                        const gn_heads* q, const gn_heads* k, const float* gain_q, const float* gain_k,

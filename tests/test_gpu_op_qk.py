@@ -182,3 +182,20 @@ def test_no_tokens(dev):
     assert qo.shape == q.shape and ko.shape == q.shape
     dq, dk, dgq, dgk = ops.qk_norm_rope_backward(dev, q, q, q, q, g, g, pos, _freq(64))
     assert float(dgq.abs().sum()) == 0 and float(dgk.abs().sum()) == 0
+
+
+def test_gains_anywhere_and_one_missing(dev):
+    """Gains that begin 4 bytes after an 8-byte boundary; a gain for the keys alone."""
+    gen = torch.Generator("cuda").manual_seed(6)
+    q, k = (torch.randn(50, h, 64, device="cuda", generator=gen).bfloat16() for h in (3, 2))
+    gains = torch.rand(130, device="cuda", generator=gen)
+    pos = torch.arange(50, device="cuda")
+    _check(dev, q, k, gains[1:65], gains[65:129], pos, _freq(64), False)
+    _check(dev, q, k, None, gains[65:129], pos, _freq(64), True)
+
+
+def test_in_place_with_other_strides_is_refused(dev):
+    from goneuron_b200 import _lib, operators as ops
+    wide = torch.randn(20, 8, 64, device="cuda")
+    with pytest.raises(_lib.GoNeuronCudaError):
+        ops.qk_norm_rope(dev, wide[:, :2], None, out=(wide.view(40, 4, 64)[:20, :2], None))

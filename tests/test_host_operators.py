@@ -42,6 +42,7 @@ static void qk() {
   r = q; r.token_stride = -512; NO(check_qk(b));
   r = q; r.token_stride = 0; OK(check_qk(b)); NO(check_heads(b, &r, 8, true));      // one row for all: as an input only
   r = q; r.head_stride = 63; NO(check_heads(b, &r, 8, true));
+  gn_heads same = q, moved = q; moved.token_stride = 1024; OK(check_in_place(&q, &same)); NO(check_in_place(&q, &moved)); OK(check_in_place(nullptr, &q)); OK(check_in_place(&q, &k));
   NO(check_heads(a, &k, 8, true)); NO(check_heads(a, nullptr, 8, true));
   const gn_heads* all[] = {&q, &k, nullptr};
   IS(qk_group(GN_F16, 64, 64, false, all, 3) == 4); IS(qk_group(GN_F32, 64, 64, false, all, 3) == 8); IS(qk_group(GN_F16, 512, 512, false, all, 3) == 32);
