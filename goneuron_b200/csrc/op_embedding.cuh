@@ -67,50 +67,25 @@ struct TileDigit {
   }
 };
 
-// Few tokens: one block, everything in shared memory.
-constexpr int SORT_SMALL_THREADS = 1024;
-__global__ void __launch_bounds__(SORT_SMALL_THREADS) sort_small_kernel(const void* __restrict__ ids, int index_type, int tokens, long vocab, int passes, unsigned* __restrict__ keys, int* __restrict__ order) {
+// Few tokens: a token's place is the number of keys below its own, and of equal ones before it.  A warp counts for one token at a time, all keys in every block's shared memory: 9 million comparisons for
+// 3001 tokens, spread over all multiprocessors.  (One block that sorted them in shared memory took 10 us.)
+constexpr int RANK_THREADS = 1024;
+__global__ void __launch_bounds__(RANK_THREADS) sort_rank_kernel(const void* __restrict__ ids, int index_type, int tokens, long vocab, unsigned* __restrict__ keys, int* __restrict__ order) {
   op_begin();
-  extern __shared__ unsigned sort_smem[];
-  constexpr int W = SORT_SMALL_THREADS / 32;
-  unsigned* cnt = sort_smem;                                         // [W][256]
-  unsigned* k0 = cnt + W * 256; unsigned* k1 = k0 + SORT_SMALL;      // key and place, in and out
-  unsigned short* p0 = reinterpret_cast<unsigned short*>(k1 + SORT_SMALL); unsigned short* p1 = p0 + SORT_SMALL;
-  __shared__ unsigned sums[8];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  for (int i = tid; i < tokens; i += SORT_SMALL_THREADS) { k0[i] = token_key(ids, index_type, i, vocab); p0[i] = (unsigned short)i; }
-  const int per = ((tokens + 31) / 32 + W - 1) / W, first = warp * per * 32, last = min(tokens, first + per * 32);
-  for (int pass = 0; pass < passes; pass++) {
-    const int shift = pass * SORT_BITS;
-    for (int e = tid; e < W * 256; e += SORT_SMALL_THREADS) cnt[e] = 0;
-    __syncthreads();
-    for (int i = first + lane; i < last; i += 32) atomicAdd(&cnt[warp * 256 + ((k0[i] >> shift) & 255)], 1u);
-    __syncthreads();
-    if (tid < 256) {                                                 // thread = digit: running count over the warps, then over the digits
-      unsigned n = 0;
-      for (int w = 0; w < W; w++) { const unsigned c = cnt[w * 256 + tid]; cnt[w * 256 + tid] = n; n += c; }
-      unsigned s = n;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) { const unsigned u = __shfl_up_sync(0xffffffffu, s, o); if (lane >= o) s += u; }
-      if (lane == 31) sums[warp] = s;
-      __syncwarp();
-      asm volatile("bar.sync 1, 256;" ::: "memory");
-      for (int w = 0; w < warp; w++) s += sums[w];
-      s -= n;
-      for (int w = 0; w < W; w++) cnt[w * 256 + tid] += s;
+  __shared__ __align__(16) unsigned all[SORT_SMALL];
+  const int lane = threadIdx.x & 31, padded = (tokens + 127) & ~127;
+  for (int i = threadIdx.x; i < padded; i += RANK_THREADS) all[i] = i < tokens ? token_key(ids, index_type, i, vocab) : 0xffffffffu;
+  __syncthreads();
+  for (int i = blockIdx.x * (RANK_THREADS / 32) + (threadIdx.x >> 5); i < tokens; i += gridDim.x * (RANK_THREADS / 32)) {
+    const unsigned key = all[i]; int n = 0;
+    for (int j0 = lane * 4; j0 < padded; j0 += 128) {
+      const uint4 k = *reinterpret_cast<const uint4*>(all + j0);
+      n += (k.x < key + (j0 < i)) + (k.y < key + (j0 + 1 < i)) + (k.z < key + (j0 + 2 < i)) + (k.w < key + (j0 + 3 < i));      // (keys are below 2^31)
     }
-    __syncthreads();
-    for (int i0 = first; i0 < last; i0 += 32) {
-      const int i = i0 + lane; const bool on = i < last;
-      const unsigned key = on ? k0[i] : 0, at = TileDigit::place(cnt + warp * 256, (key >> shift) & 255, on, lane);
-      if (on) { k1[at] = key; p1[at] = p0[i]; }
-    }
-    __syncthreads();
-    unsigned* k = k0; k0 = k1; k1 = k; unsigned short* p = p0; p0 = p1; p1 = p;
+    n = __reduce_add_sync(0xffffffffu, n);
+    if (lane == 0) { keys[n] = key; order[n] = i; }
   }
-  for (int i = tid; i < tokens; i += SORT_SMALL_THREADS) { keys[i] = k0[i]; order[i] = p0[i]; }
 }
-constexpr int SORT_SMALL_SMEM = (SORT_SMALL_THREADS / 32 * 256 + 2 * SORT_SMALL) * 4 + 2 * SORT_SMALL * 2;
 
 // Many tokens: per pass the digits of every tile are counted, the counts of all tiles become places (digit by digit, within a digit tile by tile), and every tile
 // moves its tokens there.  FIRST: keys come from the ids and places are the tokens' own.
@@ -399,8 +374,8 @@ int gn_op_embedding_backward(gn_ctx* ctx, int dtype, int64_t tokens, int64_t voc
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   auto u = [&](int64_t at) { return reinterpret_cast<unsigned*>(ws + at); };
   if (pl.small) {
-    GN_TRY(op_smem("sort_small", sort_small_kernel, SORT_SMALL_SMEM));
-    GN_TRY(op_launch("sort_small", stream, sort_small_kernel, dim3(1), dim3(SORT_SMALL_THREADS), SORT_SMALL_SMEM, 0, ids, index_type, (int)tokens, (long)vocab, pl.passes, u(pl.keys), (int*)u(pl.order)));
+    const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div(tokens, RANK_THREADS / 32), (int64_t)ctx->c.sm_count);
+    GN_TRY(op_launch("sort_rank", stream, sort_rank_kernel, dim3(blocks), dim3(RANK_THREADS), 0, 0, ids, index_type, (int)tokens, (long)vocab, u(pl.keys), (int*)u(pl.order)));
   } else {
     const dim3 grid((unsigned)pl.tiles), block(SORT_THREADS);
     for (int pass = 0; pass < pl.passes; pass++) {                   // the last pass writes `keys` and `order`

@@ -124,7 +124,7 @@ inline const char* check_embedding(int dtype, int64_t tokens, int64_t vocab, int
   if (in_stride < 0 || (out_rows > 1 && out_stride < dim)) return "rows overlap, or a stride is negative";
   return nullptr;
 }
-// The tokens' order by id, then sums of it in pieces of `chunk` neighbouring places.  Up to SORT_SMALL tokens one block sorts them in shared memory; above, passes of
+// The tokens' order by id, then sums of it in pieces of `chunk` neighbouring places.  Up to SORT_SMALL tokens places are counted directly; above, passes of
 // 8 bits over tiles of SORT_TILE tokens.
 constexpr int SORT_SMALL = 8192, SORT_TILE = 2048, SORT_BITS = 8, SORT_SCAN_TILES = 128;      // SCAN_TILES: up to so many tiles add up the others' counts themselves
 struct EmbeddingPlan {
