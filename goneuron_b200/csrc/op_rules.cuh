@@ -34,7 +34,15 @@ inline const char* check_heads(const QkArgs& a, const gn_heads* h, int heads, bo
   if (a.tokens && heads && !h->data) return "a data pointer is null";
   if (const char* e = check_dtype(a.dtype, h->data)) return e;
   if (h->token_stride < 0 || h->head_stride < 0) return "a stride is negative";
-  if (written && ((a.tokens > 1 && h->token_stride < a.head_size) || (heads > 1 && h->head_stride < a.head_size))) return "an output's rows overlap";
+  if (written) {                                                     // rows lie side by side within the smaller stride, and all of those within the larger one
+    const bool many_t = a.tokens > 1, many_h = heads > 1;
+    if ((many_t && h->token_stride < a.head_size) || (many_h && h->head_stride < a.head_size)) return "an output's rows overlap";
+    if (many_t && many_h) {
+      const bool tokens_inside = h->token_stride < h->head_stride;
+      const int64_t inner = tokens_inside ? h->token_stride : h->head_stride, n = tokens_inside ? a.tokens : heads, outer = tokens_inside ? h->head_stride : h->token_stride;
+      if ((outer - a.head_size) / inner < n - 1) return "an output's rows overlap";
+    }
+  }
   return nullptr;
 }
 inline const char* check_qk(const QkArgs& a) {

@@ -42,6 +42,12 @@ static void qk() {
   r = q; r.token_stride = -512; NO(check_qk(b));
   r = q; r.token_stride = 0; OK(check_qk(b)); NO(check_heads(b, &r, 8, true));      // one row for all: as an input only
   r = q; r.head_stride = 63; NO(check_heads(b, &r, 8, true));
+  // heads of a token that reach into the next one's, either way round; side by side, with room between, or as a part of wider rows is fine
+  r = q; r.token_stride = 64; NO(check_heads(a, &r, 8, true)); OK(check_heads(a, &r, 8, false)); r.token_stride = 511; NO(check_heads(a, &r, 8, true)); r.token_stride = 512; OK(check_heads(a, &r, 8, true));
+  r.token_stride = 64; r.head_stride = 639; NO(check_heads(a, &r, 8, true)); r.head_stride = 640; OK(check_heads(a, &r, 8, true)); r.token_stride = 66; r.head_stride = 657; NO(check_heads(a, &r, 8, true));
+  r.head_stride = 658; OK(check_heads(a, &r, 8, true)); r.token_stride = 1024; r.head_stride = 128; OK(check_heads(a, &r, 8, true)); r.token_stride = 960; OK(check_heads(a, &r, 8, true));
+  r.token_stride = r.head_stride = INT64_MAX; NO(check_heads(a, &r, 8, true));
+  b = a; b.tokens = 1; r = q; r.token_stride = 0; OK(check_heads(b, &r, 8, true)); b = a;
   gn_heads same = q, moved = q; moved.token_stride = 1024; OK(check_in_place(&q, &same)); NO(check_in_place(&q, &moved)); OK(check_in_place(nullptr, &q)); OK(check_in_place(&q, &k));
   NO(check_heads(a, &k, 8, true)); NO(check_heads(a, nullptr, 8, true));
   const gn_heads* all[] = {&q, &k, nullptr};
