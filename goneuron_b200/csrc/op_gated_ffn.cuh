@@ -9,7 +9,7 @@
 // block's shared memory and TMA writes as much, the 128 bytes a cycle that there are.  (A block by itself, 128 x 256: 12 + 12 KB, the main loop at 62 % of the MMA rate, 1327 TFLOP/s
 // at K = 4096.)
 //   - Forward: a tile's B operand is 128 rows of Wg followed by 128 of Wu, one 256-wide MMA for both projections, and a thread of the epilogue has g and u of the same elements:
-//     activation and product are formed there and only h is written (and, for the gradient, g and u in float32).
+//     activation and product are formed there and only h is written (and, for the gradient, g and u).
 //   - dh is not written: its epilogue reads g and u, and writes dg and du.
 //   - dx is one product over 2 ff indices, the first half of them from (dg, Wg), the second from (du, Wu).
 //   - The three weight gradients are one launch.
@@ -63,7 +63,7 @@ template <int act> __device__ __forceinline__ void fg_act_grad(float g, float& a
   if constexpr (act == GN_ACT_SILU) { const float p = fg_sigmoid(g); a = g * p; da = p * (1.f + g * (1.f - p)); }
   else if constexpr (act == GN_ACT_GELU) {                                     // (1 + tanh z) / 2 = sigmoid(2 z) = p, 1 - tanh^2 z = 4 p (1 - p)
     const float p = fg_sigmoid(g * fmaf(0.07135481627f * g, g, 1.5957691216057308f));
-    a = g * p; da = p + g * 2.f * p * (1.f - p) * fmaf(0.10703222440890925f * g, g, 0.7978845608028654f);
+    a = g * p; da = p + g * 2.f * p * (1.f - p) * fminf(fmaf(0.10703222440890925f * g, g, 0.7978845608028654f), 3e38f);      // (far out 0 times a square that may not be finite)
   } else { a = fmaxf(g, 0.f); da = g > 0.f ? 1.f : 0.f; }
 }
 

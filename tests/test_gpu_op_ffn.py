@@ -99,6 +99,27 @@ def test_special_values(dev, bad):
             assert not rows[7] and rows.sum() >= 38 and all(rows[i] for i in range(40) if i not in (7, 9))
 
 
+def test_gates_whose_square_is_not_finite(dev):
+    """Gates of some 2^80, finite in bfloat16 though their square is not in float32: every activation is relu there, and relu's results are those of gates of about 1 times powers of two, bit for bit."""
+    from goneuron_b200 import operators as ops
+    x, wg, wu, wd, dy = _case(40, 128, 256, "bf16", 8)
+    up, down = 2.0 ** 40, 2.0 ** -40
+
+    def run(x, wg, wu, wd, act):
+        y, saved = ops.gated_ffn(dev, x, wg, wu, wd, act, save=True)
+        return [y, ops.gated_ffn(dev, x[:5], wg, wu, wd, act), *ops.gated_ffn_backward(dev, dy, x, wg, wu, wd, saved, act)]
+    _check(dev, x, wg, wu, wd, dy, "relu")
+    want = [v * k for v, k in zip(run(x, wg, wu, wd, "relu"), (up, up, 1.0, 1.0, up * up, up * up))]
+    for act in ACT:
+        got = run(x * up, wg * up, wu * down, wd * down, act)
+        for v, r in zip(got, want):
+            assert torch.isfinite(v).all()
+            if act == "relu":
+                assert torch.equal(v, r)
+            else:                                        # h, dg, du and the result may be rounded to the neighbouring number, 2^-7 off: the quotient in the sigmoid has some 2^-22
+                assert (v.double() - r.double()).norm() <= 2 * 2.0 ** -7 * r.double().norm()
+
+
 def test_views_and_batches(dev):
     x, wg, wu, wd, dy = _case(60, 96, 200, "f16", 6)
     wide = torch.randn(60, 400, device="cuda").half()
