@@ -1,6 +1,9 @@
 """The operators on device memory as they would be used together: a training step of a one-layer student (embedding, norm and rotation of queries and keys, attention by torch, gated feed-forward block,
 distillation from a teacher's top logits) against float64 autograd; the same model answering token by token; from two threads at once; with gradients left out."""
 import ctypes as C
+import os
+import subprocess
+import sys
 import threading
 
 import pytest
@@ -211,6 +214,66 @@ def test_gradients_that_are_not_wanted(dev):
     g = torch.ones(64, device="cuda")
     *_, dgk = ops.qk_norm_rope_backward(dev, q, k, q, k, None, g)
     assert ops.qk_norm_rope_backward(dev, q, k, q, k, None, g)[2] is None and torch.equal(dgk, ops.qk_norm_rope_backward(dev, q, k, q, k, g, g)[3])
+
+
+def test_captured_branches(dev):
+    """Two branches of a captured graph, each with kernels of these operators, joined by one that reads both: kernels placed under their predecessors wait for both branches."""
+    from goneuron_b200 import operators as ops
+    w, gen = _weights(6)
+    ids, pos, *_ = _batch(gen)
+    q = torch.randn(150, H, E, device="cuda", generator=gen).half()
+
+    def step(side):
+        main = torch.cuda.current_stream()
+        x = ops.embedding(dev, w["table"], ids, scale=D ** 0.5)
+        if side:
+            side.wait_stream(main)
+        with torch.cuda.stream(side or main):
+            a = ops.qk_norm_rope(dev, q, None, w["gq"], None, pos, FREQ())[0]
+            a = ops.gated_ffn(dev, a.reshape(150, D), w["wg"], w["wu"], w["wd"])
+        y = ops.gated_ffn(dev, x, w["wg"], w["wu"], w["wd"])
+        if side:
+            main.wait_stream(side)
+        return ops.qk_norm_rope(dev, a.view(150, H, E), y.view(150, H, E), None, None, pos, FREQ())
+    want = step(None)
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(side)
+    for i in range(5):
+        for t in got:
+            t.fill_(7.0)
+        graph.replay()
+        assert all(torch.equal(x, y) for x, y in zip(got, want)), i
+    ops.check(dev)
+
+
+FIRST = """
+import torch
+from goneuron_b200 import operators as ops
+from goneuron_b200.sequential import Device
+dev = Device(0)
+r = lambda *s: torch.randn(*s, device="cuda").half()
+x, wg, wu, wd, q, table, logits = r(40, 64), r(128, 64), r(128, 64), r(64, 128), r(40, 4, 64), r(90, 64), r(40, 500)
+ids, top = torch.randint(0, 90, (40,), device="cuda"), torch.randn(40, 5, device="cuda")
+def step():
+    y, saved = ops.gated_ffn(dev, x, wg, wu, wd, save=True)
+    return [y, ops.gated_ffn(dev, x[:1], wg, wu, wd), *ops.gated_ffn_backward(dev, x, x, wg, wu, wd, saved), ops.qk_norm_rope(dev, q, None)[0], ops.embedding(dev, table, ids),
+            ops.embedding_backward(dev, x, ids, 90), *ops.distill_loss_grad(dev, logits, ids[:, None].expand(40, 5).contiguous(), top)]
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = step()
+graph.replay()
+want = step()
+ops.check(dev)
+assert all(torch.equal(a, b) for a, b in zip(got, want))
+print("the same")
+"""
+
+
+def test_first_calls_of_a_process_are_captured():
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", FIRST], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "the same" in r.stdout, r.stderr[-2000:]
 
 
 def test_status_is_not_read_while_capturing(dev):
