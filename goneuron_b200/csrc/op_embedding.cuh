@@ -67,23 +67,31 @@ struct TileDigit {
   }
 };
 
-// Few tokens: a token's place is the number of keys below its own, and of equal ones before it.  A warp counts for one token at a time, all keys in every block's shared memory: 9 million comparisons for
-// 3001 tokens, spread over all multiprocessors.  (One block that sorted them in shared memory took 10 us.)
-constexpr int RANK_THREADS = 1024;
+// Few tokens: a token's place is the number of keys below its own, and of equal ones before it.  A warp counts for four neighbouring tokens at a time, all keys in every block's shared memory: 9
+// million comparisons for 3001 tokens, spread over all multiprocessors.  (One block that sorted them in shared memory took 10 us.)
+constexpr int RANK_THREADS = 1024, RANK_TOKENS = 4;
 __global__ void __launch_bounds__(RANK_THREADS) sort_rank_kernel(const void* __restrict__ ids, int index_type, int tokens, long vocab, unsigned* __restrict__ keys, int* __restrict__ order) {
   op_begin();
   __shared__ __align__(16) unsigned all[SORT_SMALL];
   const int lane = threadIdx.x & 31, padded = (tokens + 127) & ~127;
   for (int i = threadIdx.x; i < padded; i += RANK_THREADS) all[i] = i < tokens ? token_key(ids, index_type, i, vocab) : 0xffffffffu;
   __syncthreads();
-  for (int i = blockIdx.x * (RANK_THREADS / 32) + (threadIdx.x >> 5); i < tokens; i += gridDim.x * (RANK_THREADS / 32)) {
-    const unsigned key = all[i]; int n = 0;
-    for (int j0 = lane * 4; j0 < padded; j0 += 128) {
-      const uint4 k = *reinterpret_cast<const uint4*>(all + j0);
-      n += (k.x < key + (j0 < i)) + (k.y < key + (j0 + 1 < i)) + (k.z < key + (j0 + 2 < i)) + (k.w < key + (j0 + 3 < i));      // (keys are below 2^31)
+  for (int i = ((threadIdx.x >> 5) * gridDim.x + blockIdx.x) * RANK_TOKENS; i < tokens; i += gridDim.x * (RANK_THREADS / 32) * RANK_TOKENS) {
+    const uint4 own = *reinterpret_cast<const uint4*>(all + i); const unsigned key[RANK_TOKENS] = {own.x, own.y, own.z, own.w};
+    int n[RANK_TOKENS] = {};
+#pragma unroll 2
+    for (int j = lane * 4; j < padded; j += 128) {
+      const uint4 k = *reinterpret_cast<const uint4*>(all + j); const unsigned before = j < i;      // (four keys all before the four tokens, all behind them or they themselves; keys are below 2^31)
+#pragma unroll
+      for (int t = 0; t < RANK_TOKENS; t++) { const unsigned to = key[t] + before; n[t] += (k.x < to) + (k.y < to) + (k.z < to) + (k.w < to); }
     }
-    n = __reduce_add_sync(0xffffffffu, n);
-    if (lane == 0) { keys[n] = key; order[n] = i; }
+#pragma unroll
+    for (int t = 0; t < RANK_TOKENS; t++) {
+      n[t] = __reduce_add_sync(0xffffffffu, n[t]);
+#pragma unroll
+      for (int e = 0; e < t; e++) n[t] += key[e] == key[t];
+      if (lane == t && i + t < tokens) { keys[n[t]] = key[t]; order[n[t]] = i + t; }
+    }
   }
 }
 
@@ -374,7 +382,7 @@ int gn_op_embedding_backward(gn_ctx* ctx, int dtype, int64_t tokens, int64_t voc
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   auto u = [&](int64_t at) { return reinterpret_cast<unsigned*>(ws + at); };
   if (pl.small) {
-    const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div(tokens, RANK_THREADS / 32), (int64_t)ctx->c.sm_count);
+    const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div(tokens, RANK_TOKENS), (int64_t)ctx->c.sm_count);
     GN_TRY(op_launch("sort_rank", stream, sort_rank_kernel, dim3(blocks), dim3(RANK_THREADS), 0, 0, ids, index_type, (int)tokens, (long)vocab, u(pl.keys), (int*)u(pl.order)));
   } else {
     const dim3 grid((unsigned)pl.tiles), block(SORT_THREADS);

@@ -132,9 +132,10 @@ inline const char* check_embedding(int dtype, int64_t tokens, int64_t vocab, int
   if (in_stride < 0 || (out_rows > 1 && out_stride < dim)) return "rows overlap, or a stride is negative";
   return nullptr;
 }
-// The tokens' order by id, then sums of it in pieces of `chunk` neighbouring places.  Up to SORT_SMALL tokens places are counted directly; above, passes of
-// 8 bits over tiles of SORT_TILE tokens.
-constexpr int SORT_SMALL = 8192, SORT_TILE = 2048, SORT_BITS = 8, SORT_SCAN_TILES = 128;      // SCAN_TILES: up to so many tiles add up the others' counts themselves
+// The tokens' order by id, then sums of it in pieces of `chunk` neighbouring places.  Up to SORT_SMALL tokens places are counted directly, with the
+// square of the tokens' number; above, passes of 8 bits over tiles of SORT_TILE tokens (gradient of 300 elements and 5000 ids, f32: counted, 17 us for
+// 4500 tokens, 22 for 6000, 30 for 8192; in passes 29 for 8192).
+constexpr int SORT_SMALL = 7168, SORT_TILE = 2048, SORT_BITS = 8, SORT_SCAN_TILES = 128;      // SCAN_TILES: up to so many tiles add up the others' counts themselves
 struct EmbeddingPlan {
   bool small; int bits, passes, chunk; int64_t tiles, chunks;
   int64_t keys, order, keys2, order2, hist, partial, bytes;          // places in the workspace, in bytes

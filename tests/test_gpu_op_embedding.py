@@ -52,6 +52,16 @@ def test_against_float64(dev, type, tokens, vocab, dim):
         _check(dev, ids.int(), vocab, dim, type, 1.0)
 
 
+@pytest.mark.parametrize("tokens", [5, 127, 128, 129, 130, 131, 4097, 7165, 7167, 7168, 7169])
+def test_places_of_equal_ids(dev, tokens):
+    """Token counts on either side of those at which places are found another way, many tokens of an id: a sum is that of every one of its tokens, once."""
+    gen = torch.Generator("cuda").manual_seed(tokens)
+    ids = torch.randint(-1, 40, (tokens,), device="cuda", generator=gen)
+    _check(dev, ids, 40, 8, "f32", 1.0)
+    _check(dev, ids.sort(descending=True).values, 40, 8, "f16", 1.0)
+    _check(dev, torch.arange(tokens, device="cuda").flip(0), tokens, 8, "bf16", 1.0)
+
+
 @pytest.mark.parametrize("tokens", [64, 5000, 40000])
 def test_orders_that_cross_pieces(dev, tokens):
     """One token everywhere, runs of every length, nothing but padding, a token at the last row."""
