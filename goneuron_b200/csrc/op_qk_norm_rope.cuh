@@ -6,7 +6,8 @@
 // a far position costs no accuracy; sine and cosine of what is left are float32, once per token and pair for all heads, in shared memory.
 // Everything between reading x (and dy) and the one rounding of the result is float32.
 //
-// Bound by memory: a row is read once and written once.  A lane holds two 16-byte pieces of a row, the two halves of its pairs, so that a rotation stays
+// Bound by memory: a row is read once and written once.  A lane holds two pieces of a row, of 16 bytes (or 8: 32768 tokens of 16 + 4 heads of 80, 40 of them rotated, bf16: 81 us forward and 131
+// backward, element by element 643 and 1310, then with 8 warps an SM), the two halves of its pairs, so that a rotation stays
 // within the lane and the sums over a row are shuffles among its 2 to 32 lanes.
 #pragma once
 #include "device_ops.cuh"
@@ -41,9 +42,10 @@ __device__ __forceinline__ void rotate(float& a, float& b, float c, float s) { c
 
 // A lane's two pieces of a row: the halves of its pairs, or two neighbours behind the rotated part (interleaved: two neighbours everywhere), with the cosines and sines of
 // their pairs and the gain of their elements.  The same for all heads of a token, so that they stay in registers while a lane goes through several of them.
-// FULL: halves are rotated, all of a row, and the lanes of a group are exactly a row's, so that nothing needs asking.  Arithmetic goes two elements an instruction.
-template <class T, bool FULL> struct QkLane {
-  static constexpr int V = Vec<T>::N, P = V / 2;
+// V: elements of a piece, of 16 or 8 bytes.  FULL: halves are rotated, all of a row, and the lanes of a group are exactly a row's, so that nothing needs asking.  Arithmetic goes two elements an instruction.
+template <class T, int V, bool FULL> struct QkLane {
+  static constexpr int P = V / 2;
+  using Piece = typename std::conditional<V * sizeof(T) == 16, uint4, uint2>::type;
   int pa, pb; bool has_a, has_b, split;
   float2 ga[P], gb[P], c[P], s[P];                                   // cosines and sines of pairs 2 j, 2 j + 1
   __device__ __forceinline__ QkLane(const QkParams& p, int slot) {
@@ -91,35 +93,41 @@ template <class T, bool FULL> struct QkLane {
       }
     }
   }
-  __device__ __forceinline__ void load(const void* row, uint4& a, uint4& b) const {
-    a = make_uint4(0, 0, 0, 0); b = a;
-    if (has_a) a = reinterpret_cast<const uint4*>(row)[pa];
-    if (has_b) b = reinterpret_cast<const uint4*>(row)[pb];
+  __device__ __forceinline__ void load(const void* row, Piece& a, Piece& b) const {
+    a = Piece{}; b = a;
+    if (has_a) a = reinterpret_cast<const Piece*>(row)[pa];
+    if (has_b) b = reinterpret_cast<const Piece*>(row)[pb];
   }
-  __device__ __forceinline__ static void open(const uint4& u, float2 (&v)[P]) {
-    float x[V]; unpack<T>(u, x);
+  __device__ __forceinline__ static void open(const Piece& u, float2 (&v)[P]) {
+    if constexpr (sizeof(Piece) == 8) { v[0] = unpack2(u.x, T()); v[1] = unpack2(u.y, T()); }
+    else {
+      float x[V]; unpack<T>(u, x);
 #pragma unroll
-    for (int j = 0; j < P; j++) v[j] = make_float2(x[2 * j], x[2 * j + 1]);
+      for (int j = 0; j < P; j++) v[j] = make_float2(x[2 * j], x[2 * j + 1]);
+    }
   }
-  __device__ __forceinline__ static uint4 shut(const float2 (&v)[P]) {
-    float x[V];
+  __device__ __forceinline__ static Piece shut(const float2 (&v)[P]) {
+    if constexpr (sizeof(Piece) == 8) return make_uint2(pack2(v[0].x, v[0].y, T()), pack2(v[1].x, v[1].y, T()));
+    else {
+      float x[V];
 #pragma unroll
-    for (int j = 0; j < P; j++) { x[2 * j] = v[j].x; x[2 * j + 1] = v[j].y; }
-    return pack<T>(x);
+      for (int j = 0; j < P; j++) { x[2 * j] = v[j].x; x[2 * j + 1] = v[j].y; }
+      return pack<T>(x);
+    }
   }
   __device__ __forceinline__ void store(void* row, const float2 (&a)[P], const float2 (&b)[P]) const {
-    if (has_a) reinterpret_cast<uint4*>(row)[pa] = shut(a);
-    if (has_b) reinterpret_cast<uint4*>(row)[pb] = shut(b);
+    if (has_a) reinterpret_cast<Piece*>(row)[pa] = shut(a);
+    if (has_b) reinterpret_cast<Piece*>(row)[pb] = shut(b);
   }
 };
 
 constexpr int QK_THREADS = 256;
 // A group of G lanes takes HB heads of one token at a time.  (One head at a time, with the cosines read from shared memory for each: 129 us forward and 236 backward for 65536 tokens of 16 + 4 heads of
 // 64, bf16; one element an instruction: 79 and 131.)
-template <class T, int G, bool BWD, bool FULL>
+template <class T, int V, int G, bool BWD, bool FULL>
 __global__ void __launch_bounds__(QK_THREADS, QK_PER_SM) qk_vec_kernel(const __grid_constant__ QkParams p) {
-  using Lane = QkLane<T, FULL>;
-  constexpr int V = Vec<T>::N, P = V / 2, GROUPS = QK_THREADS / G, HB = BWD ? QK_HEADS_BWD : QK_HEADS_FWD;
+  using Lane = QkLane<T, V, FULL>; using Piece = typename Lane::Piece;
+  constexpr int P = V / 2, GROUPS = QK_THREADS / G, HB = BWD ? QK_HEADS_BWD : QK_HEADS_FWD;
   op_begin();
   extern __shared__ float4 qk_smem[];
   unsigned long long* fx = reinterpret_cast<unsigned long long*>(qk_smem); float* cs = reinterpret_cast<float*>(fx) + ((p.rot + 3) & ~3);
@@ -145,17 +153,17 @@ __global__ void __launch_bounds__(QK_THREADS, QK_PER_SM) qk_vec_kernel(const __g
       const bool on = t0 < n; const int t = on ? t0 : 0, h0 = on ? hb0 * HB : 0, heads = on ? min(HB, h.heads - h0) : 0;
       const long tok = base + t;
       const T* x = static_cast<const T*>(h.in) + tok * h.in_t + h0 * h.in_h;
-      uint4 ua[HB], ub[HB], wa[BWD ? HB : 1], wb[BWD ? HB : 1];
+      Piece ua[HB], ub[HB], wa[BWD ? HB : 1], wb[BWD ? HB : 1];
 #pragma unroll
       for (int q = 0; q < HB; q++) {
-        ua[q] = ub[q] = make_uint4(0, 0, 0, 0);
+        ua[q] = ub[q] = Piece{};
         if (q < heads) lane.load(x + q * h.in_h, ua[q], ub[q]);
       }
       if constexpr (BWD) {
         const T* d = static_cast<const T*>(h.dy) + tok * h.dy_t + h0 * h.dy_h;
 #pragma unroll
         for (int q = 0; q < HB; q++) {
-          wa[q] = wb[q] = make_uint4(0, 0, 0, 0);
+          wa[q] = wb[q] = Piece{};
           if (q < heads) lane.load(d + q * h.dy_h, wa[q], wb[q]);
         }
       }
@@ -227,10 +235,10 @@ __global__ void __launch_bounds__(QK_THREADS, QK_PER_SM) qk_vec_kernel(const __g
   }
 }
 
-// Rows that 16-byte pieces do not fit: a warp per row, an element (or a pair) per lane at a time.
-constexpr int QK_ROW_WARPS = 4;
+// Rows that no pieces fit: a warp per row, an element (or a pair) per lane at a time.  Bound by the latency of a row's loads and sums one after another, so that 32 warps an SM are under way
+// (32768 tokens of 16 + 4 heads of 66, bf16: 344 us forward, 496 backward; with 8 warps 697 and 1323).
 template <class T, bool BWD>
-__global__ void __launch_bounds__(32 * QK_ROW_WARPS) qk_rows_kernel(const __grid_constant__ QkParams p) {
+__global__ void __launch_bounds__(32 * QK_ROW_WARPS, QK_PER_SM) qk_rows_kernel(const __grid_constant__ QkParams p) {
   op_begin();
   extern __shared__ float4 qk_smem[];
   unsigned long long* fx = reinterpret_cast<unsigned long long*>(qk_smem); float* cs = reinterpret_cast<float*>(fx) + ((p.rot + 3) & ~3);
@@ -320,13 +328,18 @@ __global__ void __launch_bounds__(1024) qk_gain_kernel(const float* __restrict__
 }
 
 template <class T, int G, bool BWD>
-inline int qk_launch_vec(const QkParams& p, dim3 grid, size_t turns, void* stream) {
-  const bool full = !p.inter && p.rot == p.head && p.head == 2 * G * Vec<T>::N;
-  return op_launch("qk_vec", stream, full ? qk_vec_kernel<T, G, BWD, true> : qk_vec_kernel<T, G, BWD, false>, grid, dim3(QK_THREADS), turns, 0, p);
+inline int qk_launch_vec(const QkParams& p, int piece, dim3 grid, size_t turns, void* stream) {
+  constexpr int V = Vec<T>::N;
+  if constexpr (sizeof(T) == 2) { if (piece == 8) return op_launch("qk_vec", stream, qk_vec_kernel<T, 4, G, BWD, false>, grid, dim3(QK_THREADS), turns, 0, p); }
+  const bool full = !p.inter && p.rot == p.head && p.head == 2 * G * V;
+  return op_launch("qk_vec", stream, full ? qk_vec_kernel<T, V, G, BWD, true> : qk_vec_kernel<T, V, G, BWD, false>, grid, dim3(QK_THREADS), turns, 0, p);
 }
 // Sets the tokens of a block and launches; *blocks: partial sums that the gradient of a gain leaves.
 template <class T, bool BWD>
-inline int qk_launch(QkParams p, int group, int sms, void* stream, unsigned* blocks) {
+inline int qk_launch(QkParams p, const gn_heads* const* all, int n_all, int sms, void* stream, unsigned* blocks) {
+  constexpr int dtype = sizeof(T) == 4 ? GN_F32 : GN_F16;            // (only its size counts here)
+  int piece = 16, group = qk_group(dtype, p.head, p.rot, p.inter, all, n_all);
+  if (group == 0 && sizeof(T) == 2) { piece = 8; group = qk_group(dtype, p.head, p.rot, p.inter, all, n_all, 8); }
   int most = 0; int64_t n = 1;
   for (QkHeads& h : p.t) {
     h.per_block = qk_tokens(p.tokens, sms, group, h.heads, BWD ? QK_HEADS_BWD : QK_HEADS_FWD, p.rot);
@@ -336,12 +349,16 @@ inline int qk_launch(QkParams p, int group, int sms, void* stream, unsigned* blo
   const dim3 grid((unsigned)n, p.t[1].heads ? 2 : 1);
   const size_t turns = ((size_t)most * p.rot + ((p.rot + 3) & ~3)) * sizeof(float);      // at most 36 KB
   switch (group) {
-    case 0: return op_launch("qk_rows", stream, qk_rows_kernel<T, BWD>, grid, dim3(32 * QK_ROW_WARPS), turns + (BWD ? (size_t)QK_ROW_WARPS * p.head * sizeof(float) : 0), 0, p);
-    case 2: return qk_launch_vec<T, 2, BWD>(p, grid, turns, stream);
-    case 4: return qk_launch_vec<T, 4, BWD>(p, grid, turns, stream);
-    case 8: return qk_launch_vec<T, 8, BWD>(p, grid, turns, stream);
-    case 16: return qk_launch_vec<T, 16, BWD>(p, grid, turns, stream);
-    default: return qk_launch_vec<T, 32, BWD>(p, grid, turns, stream);
+    case 0: {
+      const size_t smem = turns + (BWD ? (size_t)QK_ROW_WARPS * p.head * sizeof(float) : 0);      // at most 100 KB
+      if (smem > 40 * 1024) GN_TRY(op_smem("qk_rows", qk_rows_kernel<T, BWD>, (int)smem));
+      return op_launch("qk_rows", stream, qk_rows_kernel<T, BWD>, grid, dim3(32 * QK_ROW_WARPS), smem, 0, p);
+    }
+    case 2: return qk_launch_vec<T, 2, BWD>(p, piece, grid, turns, stream);
+    case 4: return qk_launch_vec<T, 4, BWD>(p, piece, grid, turns, stream);
+    case 8: return qk_launch_vec<T, 8, BWD>(p, piece, grid, turns, stream);
+    case 16: return qk_launch_vec<T, 16, BWD>(p, piece, grid, turns, stream);
+    default: return qk_launch_vec<T, 32, BWD>(p, piece, grid, turns, stream);
   }
 }
 inline QkHeads qk_heads(const gn_heads* x, const gn_heads* dy, const gn_heads* out, const float* gain) {
@@ -371,9 +388,8 @@ int gn_op_qk_norm_rope(gn_ctx* ctx, int dtype, int64_t tokens, int head_size, in
   if (tokens == 0 || q->heads + (k ? k->heads : 0) == 0) return GN_OK;
   const int sms = ctx->c.sm_count; const gn_heads* all[] = {q, k, q_out, k ? k_out : nullptr};
   QkParams p{{qk_heads(q, nullptr, q_out, gain_q), qk_heads(k, nullptr, k_out, gain_k)}, tokens, head_size, rotated, interleaved != 0, eps, positions, index_type, frequencies, nullptr};
-  const int group = qk_group(dtype, head_size, rotated, interleaved != 0, all, 4);
   unsigned blocks = 0;
-  return with_type(dtype, [&](auto t) { using T = decltype(t); return qk_launch<T, false>(p, group, sms, stream, &blocks); });
+  return with_type(dtype, [&](auto t) { using T = decltype(t); return qk_launch<T, false>(p, all, 4, sms, stream, &blocks); });
 }
 
 int gn_op_qk_norm_rope_workspace(gn_ctx* ctx, int64_t tokens, int q_heads, int k_heads, int head_size, int64_t* bytes) {
@@ -407,9 +423,8 @@ int gn_op_qk_norm_rope_backward(gn_ctx* ctx, int dtype, int64_t tokens, int head
   if (gains && (!workspace || !aligned_to(workspace, 16) || workspace_bytes < qk_workspace(tokens, head_size, sms))) return fail(GN_ERR_INVALID_ARG, "op_qk_norm_rope_backward: the workspace is too small, null or not aligned");
   const gn_heads* all[] = {q, k, dq_out, k ? dk_out : nullptr, dq, k ? dk : nullptr};
   QkParams p{{qk_heads(q, dq_out, dq, gain_q), qk_heads(k, dk_out, dk, gain_k)}, tokens, head_size, rotated, interleaved != 0, eps, positions, index_type, frequencies, gains ? (float*)workspace : nullptr};
-  const int group = qk_group(dtype, head_size, rotated, interleaved != 0, all, 6);
   unsigned blocks = 0;
-  if (p.t[0].heads + p.t[1].heads) GN_TRY(with_type(dtype, [&](auto t) { using T = decltype(t); return qk_launch<T, true>(p, group, sms, stream, &blocks); }));
+  if (p.t[0].heads + p.t[1].heads) GN_TRY(with_type(dtype, [&](auto t) { using T = decltype(t); return qk_launch<T, true>(p, all, 6, sms, stream, &blocks); }));
   // a tensor of no heads has left no partial sums
   if (dgain_q && !p.t[0].heads) { GN_CUDA(cudaMemsetAsync(dgain_q, 0, 4L * head_size, (cudaStream_t)stream)); dgain_q = nullptr; }
   if (dgain_k && !p.t[1].heads) { GN_CUDA(cudaMemsetAsync(dgain_k, 0, 4L * head_size, (cudaStream_t)stream)); dgain_k = nullptr; }

@@ -63,22 +63,23 @@ inline const char* check_qk(const QkArgs& a) {
 inline const char* check_in_place(const gn_heads* in, const gn_heads* out) {
   return in && out && in->data && in->data == out->data && (in->token_stride != out->token_stride || in->head_stride != out->head_stride) ? "in place, both tensors' strides have to be the same" : nullptr;
 }
-// Groups of lanes: a lane has two 16-byte pieces of a row, and a row's lanes are neighbours, 2 to 32 of them.  0: the row goes element by element
-// (sizes, strides or pointers that 16-byte pieces do not fit, pairs that end inside one, rows of more than 64 pieces).
-inline int qk_group(int dtype, int head_size, int rotated, bool interleaved, const gn_heads* const* t, int n) {
-  const int vec = 16 / dtype_size(dtype), pieces = head_size / vec;
+// Groups of lanes: a lane has two pieces of a row, 16 bytes each, or 8 where 16 do not fit and the type has 16 bits; a row's lanes are neighbours, 2 to 32 of them.  0: the
+// pieces do not fit (sizes, strides or pointers, pairs that end inside one, rows of more than 64 pieces); a row that neither fits goes element by element.
+inline int qk_group(int dtype, int head_size, int rotated, bool interleaved, const gn_heads* const* t, int n, int piece = 16) {
+  const int vec = piece / dtype_size(dtype), pieces = head_size / vec;
   if (head_size % vec || pieces > 64 || (!interleaved && rotated % (2 * vec))) return 0;
   for (int i = 0; i < n; i++)
-    if (t[i] && (!aligned_to(t[i]->data, 16) || t[i]->token_stride % vec || t[i]->head_stride % vec)) return 0;
+    if (t[i] && (!aligned_to(t[i]->data, piece) || t[i]->token_stride % vec || t[i]->head_stride % vec)) return 0;
   int g = 2;
   while (2 * g < pieces) g *= 2;
   return g;
 }
 // Work of the queries and of the keys goes to blocks of their own.  A block takes as many tokens at a time as its groups of lanes fill, where that leaves work for all blocks, and at most
 // 32 KB of cosines and sines.
+constexpr int QK_ROW_WARPS = 16;                                      // of a block that goes element by element, a row each
 constexpr int QK_PER_SM = 2, QK_HEADS_FWD = 4, QK_HEADS_BWD = 2;     // heads of a token that a group of lanes takes at a time
 inline int qk_tokens(int64_t tokens, int sms, int group, int heads, int heads_at_a_time, int rotated) {
-  const int64_t per_token = group ? std::max<int64_t>(1, ceil_div(heads, heads_at_a_time)) : heads, groups = group ? 256 / group : 4;
+  const int64_t per_token = group ? std::max<int64_t>(1, ceil_div(heads, heads_at_a_time)) : heads, groups = group ? 256 / group : QK_ROW_WARPS;
   int64_t n = std::max<int64_t>(1, groups / std::max<int64_t>(1, per_token));
   n = std::min(n, std::max<int64_t>(1, ceil_div(tokens, (int64_t)sms * QK_PER_SM)));
   return (int)std::min<int64_t>(n, rotated ? std::max(1, 8192 / rotated) : 256);

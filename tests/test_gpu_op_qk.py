@@ -95,6 +95,21 @@ def test_against_float64(dev, type, tokens, heads, kv, size, rotated, interleave
     _check(dev, q, k, gq, gk, pos if rotated else None, _freq(rotated), interleaved)
 
 
+@pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("tokens,heads,kv,size,rotated,interleaved,room", [
+    (333, 6, 2, 80, 40, False, 0), (1, 6, 2, 80, 40, False, 0), (2100, 2, 1, 80, 40, False, 0), (100, 4, 3, 72, 24, False, 0), (50, 3, 2, 12, 8, False, 0), (50, 3, 2, 4, 4, True, 0), (40, 2, 1, 252, 248, False, 0),
+    (40, 2, 1, 252, 250, True, 0), (60, 5, 2, 64, 64, False, 4), (60, 5, 2, 64, 64, True, 4), (60, 5, 2, 64, 64, False, 2), (60, 5, 2, 64, 48, False, 1), (1500, 3, 2, 66, 66, False, 0), (20, 1, 1, 1024, 1024, False, 1),
+    (3, 40, 1, 260, 256, False, 4)])
+def test_pieces_of_every_width(dev, type, tokens, heads, kv, size, rotated, interleaved, room):
+    """Rows that fit pieces of 16 bytes, of 8 or none, by their size, by where the rotated part's halves end, or by the room between heads."""
+    gen = torch.Generator("cuda").manual_seed(tokens + size + room)
+    t = TYPES[type]
+    q, k = (torch.randn(tokens, h, size + room, device="cuda", generator=gen).mul(2).to(t)[:, :, :size] for h in (heads, kv))
+    gq, gk = (1 + 0.3 * torch.randn(size, device="cuda", generator=gen) for _ in range(2))
+    pos = torch.randint(0, 4096, (tokens,), device="cuda", generator=gen)
+    _check(dev, q, k, gq, gk, pos, _freq(rotated), interleaved)
+
+
 @pytest.mark.parametrize("type", ["f32", "bf16"])
 def test_views_batches_and_missing_parts(dev, type):
     """Views of a fused projection (aligned for 16-byte accesses and not), a batch, 32-bit positions, no gains, no keys, broadcast gradients."""

@@ -55,6 +55,8 @@ static void qk() {
   IS(qk_group(GN_F16, 65, 64, false, all, 3) == 0); IS(qk_group(GN_F16, 64, 24, false, all, 3) == 0); IS(qk_group(GN_F16, 64, 24, true, all, 3) == 4); IS(qk_group(GN_F16, 1024, 0, false, all, 3) == 0);
   gn_heads odd = q; odd.token_stride = 513; all[0] = &odd; IS(qk_group(GN_F16, 64, 64, false, all, 3) == 0);
   odd = q; odd.data = at(4098); IS(qk_group(GN_F16, 64, 64, false, all, 3) == 0);
+  all[0] = &q; IS(qk_group(GN_F16, 80, 40, false, all, 3) == 0 && qk_group(GN_F16, 80, 40, false, all, 3, 8) == 16); IS(qk_group(GN_BF16, 80, 44, false, all, 3, 8) == 0); IS(qk_group(GN_BF16, 260, 0, false, all, 3, 8) == 0);
+  odd = q; odd.token_stride = 516; all[0] = &odd; IS(qk_group(GN_F16, 64, 64, false, all, 3) == 0 && qk_group(GN_F16, 64, 64, false, all, 3, 8) == 8); odd.data = at(4100); IS(qk_group(GN_F16, 64, 64, false, all, 3, 8) == 0);
   for (long n : {1L, 7L, 1184L, 65536L, 2000000000L}) for (int sms : {1, 148}) for (int group : {0, 4, 32}) for (int heads : {0, 1, 5, 300}) for (int rot : {0, 64, 1024}) {
     const int t = qk_tokens(n, sms, group, heads, QK_HEADS_BWD, rot); const long blocks = qk_blocks(n, sms, t);
     IS(t >= 1 && (long)t * rot * 4 <= 32768); IS(blocks >= 1 && blocks <= (long)sms * QK_PER_SM && blocks <= n); IS(qk_workspace(n, 128, sms) >= blocks * 1024);
