@@ -67,6 +67,18 @@ def test_against_float64(dev, type, rows, vocab, top):
         _check(dev, logits, ids.int(), t, 2.5)
 
 
+@pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("vocab", [106485, 106496, 106501, 128000, 180225, 212981, 212993, 250000, 360449])
+def test_rows_over_four_and_eight_blocks(dev, type, vocab):
+    """More rows than fill the multiprocessors at once, lengths on either side of those at which a row is cut into more parts."""
+    logits, ids, t, gen = _case(60, vocab, 70, type, vocab)
+    ids[:, 5] = ids[:, 4]                                # the same index twice
+    weight = torch.rand(60, device="cuda", generator=gen) + 0.1
+    weight[3] = 0
+    _check(dev, logits, ids, t, 2.0, weight)
+    _check(dev, logits.clone(), ids, t, 2.0, weight, out=torch.empty(60, vocab + 3, device="cuda", dtype=logits.dtype)[:, 1:vocab + 1])
+
+
 @pytest.mark.parametrize("type", ["f32", "bf16"])
 @pytest.mark.parametrize("vocab", [777, 40000, 270000])
 def test_entries_and_rows_that_say_nothing(dev, type, vocab):
