@@ -16,7 +16,8 @@
 // g and u are kept as the upper 24 bits of their float32 values, in the order in which the tensor memory hands them to a warp (blocks of 32 rows x 16 columns), so that both epilogues move
 // them with whole 128-byte lines.  In 16 bits their rounding would add to those of dg and du and the error of dx be 1.7 times that of its own rounding instead of 1.4; the last 8 bits of
 // float32 would be a quarter of what the epilogue of dh, which memory bounds, has to read.
-// h, dg and du are rounded to 16 bits because the tensor cores read them as operands.
+// h, dg and du are rounded to 16 bits because the tensor cores read them as operands: y, dx and the weights' gradients have some 1.4 times the error of their own rounding, and of one to four tokens,
+// whose sums few large terms make up, 1.2 to 1.7 times.
 // Few output tiles: the contraction is cut into slices whose float32 sums a second launch adds in order.
 //
 // Waits are bounded as in the contraction engine: a wait that gives up sets the status word, every role of the block leaves its loops, copies and MMAs in flight are waited for
@@ -357,7 +358,10 @@ template <> __device__ __forceinline__ void mma_16x8x16<__half>(float (&d)[4], u
 template <> __device__ __forceinline__ void mma_16x8x16<__nv_bfloat16>(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};" : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-constexpr int FEW_WARPS = 8, FEW_TOKENS = 16;
+constexpr int FEW_WARPS = 8;
+// Up to eight tokens h is kept as the sum of two 16-bit numbers, a plane of `tokens` rows for each, and the second launch multiplies by both.  Rounded to 16 bits it would make the error of y some 1.4
+// times that of its own rounding, and up to 1.7 for a single token, where few terms make up the sum.  (One token, 1024 x 4096, bf16: 9.2 -> 9.9 us.  For 9 to 16 tokens, whose
+// errors average out, it would be 10 to 25 % and is not done.)
 // GATE: out[t][n] = act(x w0^T) (x w1^T), else x w0^T.  n in blocks of 16, `cl` blocks of a cluster share the contraction.  NB: blocks of eight tokens.
 template <class T, bool GATE, int NB, int ACT>
 __global__ void __launch_bounds__(32 * FEW_WARPS) fg_few_kernel(const T* x, long x_stride, const T* __restrict__ w0, const T* __restrict__ w1, int tokens, int N, int K, T* __restrict__ out, long out_stride, int cl) {
@@ -371,7 +375,8 @@ __global__ void __launch_bounds__(32 * FEW_WARPS) fg_few_kernel(const T* x, long
   const uint4 zero = make_uint4(0, 0, 0, 0);
   constexpr int U = NB == 1 ? 4 : 2;                                 // steps of 32 indices under way
   const int steps = (K + 31) / 32, parts = FEW_WARPS * cl, part = rank * FEW_WARPS + warp, s_end = (int)((long)steps * (part + 1) / parts);
-  uint4 a[U][MATS][2], b[U][NB];
+  constexpr int PARTS = !GATE && NB == 1 ? 2 : 1;
+  uint4 a[U][MATS][2], b[U][NB][PARTS];
   auto weights = [&](int s0) {
 #pragma unroll
     for (int i = 0; i < U; i++) {
@@ -390,17 +395,23 @@ __global__ void __launch_bounds__(32 * FEW_WARPS) fg_few_kernel(const T* x, long
     for (int i = 0; i < U; i++) {
       const int k = (s0 + i) * 32 + q * 8; const bool in = s0 + i < s_end && k < K;
 #pragma unroll
-      for (int j = 0; j < NB; j++) { const int t = 8 * j + g; b[i][j] = in && t < tokens ? *reinterpret_cast<const uint4*>(x + t * x_stride + k) : zero; }
+      for (int j = 0; j < NB; j++) {
+        const int t = 8 * j + g;
+#pragma unroll
+        for (int e = 0; e < PARTS; e++) b[i][j][e] = in && t < tokens ? *reinterpret_cast<const uint4*>(x + (t + e * tokens) * x_stride + k) : zero;
+      }
     }
 #pragma unroll
     for (int i = 0; i < U; i++)
 #pragma unroll
       for (int m = 0; m < MATS; m++)
 #pragma unroll
-        for (int j = 0; j < NB; j++) {
-          mma_16x8x16<T>(d[m][j], a[i][m][0].x, a[i][m][1].x, a[i][m][0].y, a[i][m][1].y, b[i][j].x, b[i][j].y);
-          mma_16x8x16<T>(d[m][j], a[i][m][0].z, a[i][m][1].z, a[i][m][0].w, a[i][m][1].w, b[i][j].z, b[i][j].w);
-        }
+        for (int j = 0; j < NB; j++)
+#pragma unroll
+          for (int e = 0; e < PARTS; e++) {
+            mma_16x8x16<T>(d[m][j], a[i][m][0].x, a[i][m][1].x, a[i][m][0].y, a[i][m][1].y, b[i][j][e].x, b[i][j][e].y);
+            mma_16x8x16<T>(d[m][j], a[i][m][0].z, a[i][m][1].z, a[i][m][0].w, a[i][m][1].w, b[i][j][e].z, b[i][j][e].w);
+          }
     if (s0 + U < s_end) weights(s0 + U);
   }
 #pragma unroll
@@ -425,7 +436,11 @@ __global__ void __launch_bounds__(32 * FEW_WARPS) fg_few_kernel(const T* x, long
         v[m] = sums[m * NB * 128 + e];
         for (int r = 1; r < cl; r++) v[m] += cg::this_cluster().map_shared_rank(sums, r)[m * NB * 128 + e];
       }
-      if (n < N && t < tokens) { if constexpr (GATE) out[t * out_stride + n] = from_f32<T>(fg_act<ACT>(v[0]) * v[1]); else out[t * out_stride + n] = from_f32<T>(v[0]); }
+      if (n < N && t < tokens) {
+        const float y = GATE ? fg_act<ACT>(v[0]) * v[MATS - 1] : v[0]; const T hi = from_f32<T>(y);
+        out[t * out_stride + n] = hi;
+        if constexpr (GATE && NB == 1) { const float r = y - to_f32(hi); out[(t + tokens) * out_stride + n] = from_f32<T>(isinf(to_f32(hi)) ? 0.f : r); }      // (what 16 bits cannot hold is infinite by itself)
+      }
     }
   if (cl > 1) cg::this_cluster().sync();                             // (the others' sums have been read)
 }
@@ -482,12 +497,12 @@ template <class T, int ACT>
 inline int ffn_forward(gn_ctx* ctx, int64_t M, int D, int F, const void* x, int64_t xs, const void* wg, const void* wu, const void* wd, void* y, int64_t ys, uint8_t* saved, uint8_t* ws, void* stream) {
   const FfnPlan& pl = ffn_plan(M, D, F, ctx->c.sm_count);
   void* h = saved ? saved + pl.saved_h : ws + pl.fwd_h;
-  if (!saved && M <= FEW_TOKENS) {
+  if (!saved && M <= FFN_FEW_TOKENS) {
     auto few = [&](auto kernel, const void* in, int64_t in_s, const void* a, const void* b, int N, int K, void* out, int64_t os) {
       const int cl = ffn_few_cluster(N, K, ctx->c.sm_count);
       return op_launch("gated_ffn_few", stream, kernel, dim3((unsigned)(ceil_div(N, 16) * cl)), dim3(32 * FEW_WARPS), 0, cl, static_cast<const T*>(in), (long)in_s, static_cast<const T*>(a), static_cast<const T*>(b), (int)M, N, K, static_cast<T*>(out), (long)os, cl);
     };
-    if (M <= 8) { GN_TRY(few(fg_few_kernel<T, true, 1, ACT>, x, xs, wg, wu, F, D, h, F)); return few(fg_few_kernel<T, false, 1, GN_ACT_LINEAR>, h, F, wd, nullptr, D, F, y, ys); }
+    if (M <= FFN_FEW_TOKENS / 2) { GN_TRY(few(fg_few_kernel<T, true, 1, ACT>, x, xs, wg, wu, F, D, h, F)); return few(fg_few_kernel<T, false, 1, GN_ACT_LINEAR>, h, F, wd, nullptr, D, F, y, ys); }
     GN_TRY(few(fg_few_kernel<T, true, 2, ACT>, x, xs, wg, wu, F, D, h, F)); return few(fg_few_kernel<T, false, 2, GN_ACT_LINEAR>, h, F, wd, nullptr, D, F, y, ys);
   }
   const FgMatrix none{};

@@ -209,14 +209,15 @@ inline int64_t ffn_partial(std::initializer_list<FfnShape> shapes, const FfnCut&
   for (const FfnShape& s : shapes) tiles += ceil_div(s.M, 256) * ceil_div(s.N, c.bn);
   return c.splits > 1 ? tiles * c.splits * 256 * c.bn * 4 : 0;
 }
+constexpr int FFN_FEW_TOKENS = 16;                                   // up to so many, without a gradient, go through kernels of their own, up to half of that in blocks of eight
 // Places, in bytes, in what the forward pass saves (g and u in blocks of 32 x 16, 24 bits each, then h) and in the workspaces.
 struct FfnPlan { FfnCut y, dx, dw; int64_t saved_h, saved, fwd_h, fwd_partial, fwd, bwd_dg, bwd_du, bwd_partial, bwd; };
 inline FfnPlan ffn_make_plan(int64_t M, int64_t D, int64_t F, int sms) {
   FfnPlan p{};
   const int64_t kf = ceil_div(F, 64), h = round_up(2 * M * F, 256);
   p.y = ffn_cut({{M, D}}, kf, sms); p.dx = ffn_cut({{M, D}}, 2 * kf, sms); p.dw = ffn_cut({{F, D}, {F, D}, {D, F}}, std::max<int64_t>(1, ceil_div(M, 64)), sms);
-  p.saved_h = ceil_div(M, 32) * ceil_div(F, 16) * 3072; p.saved = p.saved_h + h;
-  p.fwd_h = 0; p.fwd_partial = h; p.fwd = h + ffn_partial({{M, D}}, p.y);
+  p.saved_h = ceil_div(M, 32) * ceil_div(F, 16) * (32 * 16 * 6); p.saved = p.saved_h + h;
+  p.fwd_h = 0; p.fwd_partial = M <= FFN_FEW_TOKENS / 2 ? round_up(4 * M * F, 256) : h; p.fwd = p.fwd_partial + ffn_partial({{M, D}}, p.y);      // (few tokens: two planes)
   p.bwd_dg = 0; p.bwd_du = h; p.bwd_partial = 2 * h; p.bwd = 2 * h + std::max(ffn_partial({{M, D}}, p.dx), ffn_partial({{F, D}, {F, D}, {D, F}}, p.dw));
   return p;
 }

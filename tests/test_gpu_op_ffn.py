@@ -99,6 +99,35 @@ def test_special_values(dev, bad):
             assert not rows[7] and rows.sum() >= 38 and all(rows[i] for i in range(40) if i not in (7, 9))
 
 
+@pytest.mark.parametrize("type", ["f16", "bf16"])
+@pytest.mark.parametrize("m,d,f,act", [(1, 8, 8, "silu"), (1, 1024, 4096, "silu"), (3, 264, 520, "gelu"), (8, 64, 128, "relu"), (7, 1032, 72, "silu"), (8, 512, 2048, "gelu")])
+def test_few_tokens_are_rounded_once(dev, type, m, d, f, act):
+    """Up to 8 tokens without a gradient: h enters the second product as two 16-bit numbers, half a step of half a step off; y has its own rounding and no other."""
+    from goneuron_b200 import operators as ops
+    x, wg, wu, wd, _ = _case(m, d, f, type, m + f)
+    X, G, U, D = (v.double() for v in (x, wg, wu, wd))
+    g, u = X @ G.T, X @ U.T
+    h = ACT[act](g) * u
+    rel, small = rounding(x.dtype)
+    a, da = ACT[act](g).abs(), torch.autograd.functional.jvp(ACT[act], (g,), (torch.ones_like(g),))[1].abs()
+    eh = rel * rel * h.abs() + small + _accumulated(d) * (da * u.abs() * (X.abs() @ G.abs().T) + a * (X.abs() @ U.abs().T)) + 2.0 ** -19 * h.abs()
+    _near(ops.gated_ffn(dev, x, wg, wu, wd, act), h @ D.T, eh @ D.abs().T + _accumulated(2 * f) * (h.abs() @ D.abs().T), "y")
+
+
+@pytest.mark.parametrize("type", ["f16", "bf16"])
+def test_few_tokens_whose_h_is_not_finite(dev, type):
+    """A product beyond the type's range, or not finite itself, makes its row's outputs not finite and no other row's, with an h of one infinity the same infinity."""
+    from goneuron_b200 import operators as ops
+    x, wg, wu, wd, _ = _case(5, 64, 64, type, 9)
+    x[:, 0], wg[:], wu[:] = 1, 0, 0
+    x[2, 0] = 3e4 if type == "f16" else 3e38
+    wg[7, 0], wu[7, 0] = 3, 2                            # h[:, 7] = 6 x^2, the others 0
+    y = ops.gated_ffn(dev, x, wg, wu, wd, "relu")
+    rows = torch.isfinite(y).all(1)
+    assert not rows[2] and rows.sum() == 4 and torch.equal(y[2][wd[:, 7] != 0], (wd[:, 7][wd[:, 7] != 0].float() * torch.inf).to(y.dtype))
+    assert torch.equal(y[0], (6 * wd[:, 7].double()).to(y.dtype))
+
+
 def test_gates_whose_square_is_not_finite(dev):
     """Gates of some 2^80, finite in bfloat16 though their square is not in float32: every activation is relu there, and relu's results are those of gates of about 1 times powers of two, bit for bit."""
     from goneuron_b200 import operators as ops
