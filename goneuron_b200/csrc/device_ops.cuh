@@ -42,6 +42,8 @@ inline int op_launch(const char* what, void* stream, void (*kernel)(P...), dim3 
   if (e != cudaSuccess) { cudaGetLastError(); return fail(GN_ERR_CUDA, "kernel launch failed (%s): %s", what, cudaGetErrorString(e)); }
   return GN_OK;
 }
+// The kernel's limit of dynamic shared memory on this GPU.  It belongs to the kernel and not to a launch: every call that needs it sets the most that any call may ask for, so that no thread lowers it between
+// another one's setting it and launching.
 template <class K> inline int op_smem(const char* what, K kernel, int bytes) {
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   return e == cudaSuccess ? GN_OK : fail(GN_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));

@@ -42,7 +42,6 @@ struct Norm { float m, l; };
 struct Teacher { float l, d, r, w; };
 __device__ __forceinline__ Norm norm_of(MaxSum v) { return Norm{v.m, log2f(v.s)}; }
 
-constexpr int DISTILL_TOP = 1024;
 // id (-1: none) and logit of entry k
 __device__ __forceinline__ int teacher_entry(const DistillParams& p, long row, int k, float& t) {
   const int64_t id = load_index(p.ids, p.index_type, row * p.top + k);
@@ -54,7 +53,6 @@ __device__ __forceinline__ int teacher_entry(const DistillParams& p, long row, i
 // One warp.  The entries go through shared memory, where the gradient finds their ids, probabilities and student values again; the student's values are asked for as soon as the ids are there.
 // Of entries with the same id the first keeps all of their probability and the others become -1.  They are rare and found by a table: every entry writes its number at its id's place; who
 // finds another's number there and not the same id tries a second place; where that is taken too, or the ids are the same, the row is looked through.
-constexpr int TEACHER_TABLE = 2048;
 struct TeacherRow { int* id; float *prob, *stud; };                  // [top, rounded up to 16] each
 struct TeacherSmem {                                                 // rows in turns of three, then what one row needs while it is worked on
   uint8_t* base; int top16;
@@ -62,7 +60,6 @@ struct TeacherSmem {                                                 // rows in 
   __device__ __forceinline__ float* logit() const { return reinterpret_cast<float*>(base) + 9 * top16; }
   __device__ __forceinline__ unsigned short* table() const { return reinterpret_cast<unsigned short*>(base + 40 * top16); }
 };
-inline int teacher_smem(int top) { return (top + 15) / 16 * 16 * 40 + 2 * TEACHER_TABLE; }
 template <class T, bool GRAD>
 __device__ __forceinline__ Teacher teacher_row(const DistillParams& p, long row, float c, int lane, const TeacherSmem& sm, const TeacherRow& to) {
   const float w = p.weight ? __ldg(p.weight + row) : 1.f;
@@ -333,7 +330,7 @@ inline int distill_launch(gn_ctx* ctx, const DistillParams& p, void* stream) {
   const bool whole = p.vocab % V == 0 && p.stride % V == 0 && aligned_to(p.logits, 16) && (!GRAD || (p.dstride % V == 0 && aligned_to(p.dlogits, 16)));
   const int smem = pl.per * 16 + tsmem; const int64_t per_sm = std::max<int64_t>(1, std::min<int64_t>({2048 / (pl.threads + 32), 32, 65536 / (40 * (pl.threads + 32)), 224 * 1024 / (smem + 3 * 1024)}));
   const dim3 grid((unsigned)(std::min<int64_t>(p.rows, std::max<int64_t>(1, (int64_t)sms * per_sm / pl.cluster)) * pl.cluster));
-  auto go = [&](auto kernel) { if (smem > 40 * 1024) GN_TRY(op_smem("distill", kernel, smem)); return op_launch("distill", stream, kernel, grid, dim3(pl.threads + 32), smem, pl.cluster, p, pl.cluster, pl.per); };
+  auto go = [&](auto kernel) { if (smem > 40 * 1024) GN_TRY(op_smem("distill", kernel, DISTILL_SMEM_MOST)); return op_launch("distill", stream, kernel, grid, dim3(pl.threads + 32), smem, pl.cluster, p, pl.cluster, pl.per); };
   return whole ? go(distill_kernel<T, GRAD, true>) : go(distill_kernel<T, GRAD, false>);
 }
 

@@ -350,8 +350,8 @@ inline int qk_launch(QkParams p, const gn_heads* const* all, int n_all, int sms,
   const size_t turns = ((size_t)most * p.rot + ((p.rot + 3) & ~3)) * sizeof(float);      // at most 36 KB
   switch (group) {
     case 0: {
-      const size_t smem = turns + (BWD ? (size_t)QK_ROW_WARPS * p.head * sizeof(float) : 0);      // at most 100 KB
-      if (smem > 40 * 1024) GN_TRY(op_smem("qk_rows", qk_rows_kernel<T, BWD>, (int)smem));
+      const size_t smem = turns + (BWD ? (size_t)QK_ROW_WARPS * p.head * sizeof(float) : 0);      // at most QK_ROWS_SMEM_MOST
+      if (smem > 40 * 1024) GN_TRY(op_smem("qk_rows", qk_rows_kernel<T, BWD>, QK_ROWS_SMEM_MOST));
       return op_launch("qk_rows", stream, qk_rows_kernel<T, BWD>, grid, dim3(32 * QK_ROW_WARPS), smem, 0, p);
     }
     case 2: return qk_launch_vec<T, 2, BWD>(p, piece, grid, turns, stream);

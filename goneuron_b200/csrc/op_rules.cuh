@@ -84,16 +84,23 @@ inline int qk_tokens(int64_t tokens, int sms, int group, int heads, int heads_at
   n = std::min(n, std::max<int64_t>(1, ceil_div(tokens, (int64_t)sms * QK_PER_SM)));
   return (int)std::min<int64_t>(n, rotated ? std::max(1, 8192 / rotated) : 256);
 }
+// Shared memory of a block that goes element by element, at most: cosines and sines, frequencies, a row of sums for every warp.
+constexpr int QK_ROWS_SMEM_MOST = (8192 + 1024 + QK_ROW_WARPS * 1024) * 4;
 // All blocks are resident at once, so that a gradient leaves no more partial sums than those.
 inline int64_t qk_blocks(int64_t tokens, int sms, int tokens_at_a_time) { return std::max<int64_t>(1, std::min<int64_t>(ceil_div(tokens, tokens_at_a_time), (int64_t)sms * QK_PER_SM)); }
 inline int64_t qk_workspace(int64_t tokens, int head_size, int sms) { return qk_blocks(tokens, sms, 1) * 2 * head_size * 4; }
 
 // ------------------------------------------------------------------ distillation
+constexpr int DISTILL_THREADS = 480, DISTILL_PART = 104 * 1024, DISTILL_PART_MOST = 176 * 1024;
+// Beside its part of a row a block has the teacher's entries in shared memory: three rows of them, what one row needs while it is worked on, and a table of ids.
+constexpr int DISTILL_TOP = 1024, TEACHER_TABLE = 2048;
+constexpr int teacher_smem(int top) { return (top + 15) / 16 * 16 * 40 + 2 * TEACHER_TABLE; }
+constexpr int DISTILL_SMEM_MOST = DISTILL_PART_MOST + teacher_smem(DISTILL_TOP);
 inline const char* check_distill(int dtype, int64_t rows, int64_t vocab, int top, float temperature, const void* logits, int64_t row_stride, const void* top_ids, int index_type,
                                  const float* top_logits, const float* weight, const float* loss, const void* dlogits, int64_t drow_stride) {
   if (rows < 0 || rows > OP_MAX_ROWS) return "rows out of range";
   if (vocab < 1 || vocab > OP_MAX_ROWS) return "vocab out of range";
-  if (top < 0 || top > 1024) return "top is not in [0, 1024]";
+  if (top < 0 || top > DISTILL_TOP) return "top is not in [0, 1024]";
   if (!(temperature > 0.f) || std::isinf(temperature)) return "temperature is not positive and finite";
   if (rows && (!logits || !loss || (top && (!top_ids || !top_logits)))) return "a data pointer is null";
   if (const char* e = check_dtype(dtype, logits)) return e;
@@ -109,7 +116,6 @@ inline const char* check_distill(int dtype, int64_t rows, int64_t vocab, int top
 // row (515 rows of 100003, f16: one block 66 us, two 61, four 80; 2000 rows of 130000, bf16: two 291, four 330), and four again only where their parts leave room for two on a multiprocessor
 // (512 rows of 128000, f32: four 216 us, eight 166; of 250000, bf16: 256 and 180).  Few rows are cut further, so that they fill the multiprocessors, down to two
 // thousand elements per block.
-constexpr int DISTILL_THREADS = 480, DISTILL_PART = 104 * 1024, DISTILL_PART_MOST = 176 * 1024;
 struct DistillPlan { int cluster, threads, per; };
 inline DistillPlan distill_plan(int64_t rows, int64_t vocab, int size, int sms) {
   const int64_t v = 16 / size, pieces = ceil_div(vocab + v - 1, v);  // (a row may begin inside a piece)
