@@ -200,7 +200,8 @@ __global__ void __launch_bounds__(QK_THREADS, QK_PER_SM) qk_vec_kernel(const __g
           float sx = x2.x + x2.y;
 #pragma unroll
           for (int m = G / 2; m > 0; m >>= 1) { ss += __shfl_xor_sync(0xffffffffu, ss, m); sx += __shfl_xor_sync(0xffffffffu, sx, m); }
-          const float rs = rsqrtf(fmaf(ss, inv, p.eps)), m = -rs * rs * (sx * inv); const float2 r2 = make_float2(rs, rs), m2 = make_float2(m, m);
+          const float rs = q < heads ? rsqrtf(fmaf(ss, inv, p.eps)) : 0.f, m = -rs * rs * (sx * inv);      // (a row that is not there has zeros: with eps = 0 its root would be infinite)
+          const float2 r2 = make_float2(rs, rs), m2 = make_float2(m, m);
 #pragma unroll
           for (int j = 0; j < P; j++) {
             acc[j] = fma2(ya[j], mul2(a[j], r2), acc[j]); acc[P + j] = fma2(yb[j], mul2(b[j], r2), acc[P + j]);      // (rows that are not there have zeros)
