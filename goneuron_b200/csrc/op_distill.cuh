@@ -47,7 +47,7 @@ __device__ __forceinline__ int teacher_entry(const DistillParams& p, long row, i
   const int64_t id = load_index(p.ids, p.index_type, row * p.top + k);
   const bool there = id >= 0 && id < p.vocab;
   if (!there && id != -1) op_report(OP_BAD_INDEX);
-  t = there ? __ldg(p.top_logits + row * p.top + k) : -INFINITY;
+  t = there ? ld(p.top_logits + row * p.top + k) : -INFINITY;
   return there ? (int)id : -1;
 }
 // One warp.  The entries go through shared memory, where the gradient finds their ids, probabilities and student values again; the student's values are asked for as soon as the ids are there.
@@ -62,7 +62,7 @@ struct TeacherSmem {                                                 // rows in 
 };
 template <class T, bool GRAD>
 __device__ __forceinline__ Teacher teacher_row(const DistillParams& p, long row, float c, int lane, const TeacherSmem& sm, const TeacherRow& to) {
-  const float w = p.weight ? __ldg(p.weight + row) : 1.f;
+  const float w = p.weight ? ld(p.weight + row) : 1.f;
   if (w == 0.f) return Teacher{0.f, 0.f, 0.f, 0.f};
   const T* logits = static_cast<const T*>(p.logits) + row * p.stride; float* logit = sm.logit(); unsigned short* table = sm.table();
   float m = -INFINITY;
@@ -174,7 +174,7 @@ __global__ void __launch_bounds__(DISTILL_THREADS + 32, 3) distill_kernel(const 
   auto row_of = [&](long r) { return static_cast<const T*>(p.logits) + r * p.stride; };
   auto lead_of = [&](long r) { return WHOLE ? 0 : row_lead(row_of(r)); };
   auto count = [&](int lead) { return min(per, (lead + vocab + V - 1) / V - at); };      // pieces of this block
-  auto weight_of = [&](long r) { return r >= p.rows ? 0.f : p.weight ? __ldg(p.weight + r) : 1.f; };
+  auto weight_of = [&](long r) { return r >= p.rows ? 0.f : p.weight ? ld(p.weight + r) : 1.f; };
   // copies of this thread's pieces of row r; pieces that the row does not fill are put together element by element, -inf where it has none
   const uint32_t slot0 = (uint32_t)__cvta_generic_to_shared(slots);
   auto fetch = [&](long r, float w) {
@@ -296,7 +296,7 @@ __global__ void __launch_bounds__(1024) distill_long_kernel(const __grid_constan
     const T* row = static_cast<const T*>(p.logits) + r * p.stride;
     MaxSum v{-INFINITY, 0.f};
     if (warp == 0) { const Teacher t = teacher_row<T, GRAD>(p, r, c, lane, sm, sm.row(0)); if (lane == 0) teach = t; }
-    if ((p.weight ? __ldg(p.weight + r) : 1.f) != 0.f)
+    if ((p.weight ? ld(p.weight + r) : 1.f) != 0.f)
       for (long e0 = tid; e0 < p.vocab; e0 += 8 * 1024) {
         float x[8]; float m = -INFINITY;
 #pragma unroll

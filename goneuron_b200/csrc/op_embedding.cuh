@@ -14,8 +14,8 @@ namespace gn {
 // ------------------------------------------------------------------ lookup
 // A warp per token.  V: elements of an access (16 bytes, or one where sizes, strides or pointers do not allow that).
 template <class T, int V>
-__global__ void __launch_bounds__(256) embedding_kernel(const T* __restrict__ table, long table_stride, const void* __restrict__ ids, int index_type, long tokens, long vocab, int dim, float scale,
-                                                        T* __restrict__ out, long out_stride) {
+__global__ void __launch_bounds__(256) embedding_kernel(const T* table, long table_stride, const void* ids, int index_type, long tokens, long vocab, int dim, float scale,
+                                                        T* out, long out_stride) {
   op_begin();
   const int lane = threadIdx.x & 31; const long warps = (long)gridDim.x * 8;
   for (long i = (long)blockIdx.x * 8 + (threadIdx.x >> 5); i < tokens; i += warps) {
@@ -30,7 +30,7 @@ __global__ void __launch_bounds__(256) embedding_kernel(const T* __restrict__ ta
       for (int e0 = lane; e0 < n; e0 += 32 * U) {
         uint4 u[U];
 #pragma unroll
-        for (int j = 0; j < U; j++) { u[j] = make_uint4(0, 0, 0, 0); if (there && e0 + 32 * j < n) u[j] = __ldg(reinterpret_cast<const uint4*>(src) + e0 + 32 * j); }
+        for (int j = 0; j < U; j++) { u[j] = make_uint4(0, 0, 0, 0); if (there && e0 + 32 * j < n) u[j] = ld(reinterpret_cast<const uint4*>(src) + e0 + 32 * j); }
 #pragma unroll
         for (int j = 0; j < U; j++) {
           float v[Vec<T>::N]; unpack<T>(u[j], v);
@@ -70,7 +70,7 @@ struct TileDigit {
 // Few tokens: a token's place is the number of keys below its own, and of equal ones before it.  A warp counts for four neighbouring tokens at a time, all keys in every block's shared memory: 9
 // million comparisons for 3001 tokens, spread over all multiprocessors.  (One block that sorted them in shared memory took 10 us.)
 constexpr int RANK_THREADS = 1024, RANK_TOKENS = 4;
-__global__ void __launch_bounds__(RANK_THREADS) sort_rank_kernel(const void* __restrict__ ids, int index_type, int tokens, long vocab, unsigned* __restrict__ keys, int* __restrict__ order) {
+__global__ void __launch_bounds__(RANK_THREADS) sort_rank_kernel(const void* ids, int index_type, int tokens, long vocab, unsigned* keys, int* order) {
   op_begin();
   __shared__ __align__(16) unsigned all[SORT_SMALL];
   const int lane = threadIdx.x & 31, padded = (tokens + 127) & ~127;
@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(RANK_THREADS) sort_rank_kernel(const void* __r
 // moves its tokens there.  FIRST: keys come from the ids and places are the tokens' own.
 constexpr int SORT_THREADS = 256;
 template <bool FIRST>
-__global__ void __launch_bounds__(SORT_THREADS) sort_count_kernel(const void* __restrict__ ids, int index_type, const unsigned* __restrict__ keys, long tokens, long vocab, int shift, bool by_tile, unsigned* __restrict__ hist) {
+__global__ void __launch_bounds__(SORT_THREADS) sort_count_kernel(const void* ids, int index_type, const unsigned* keys, long tokens, long vocab, int shift, bool by_tile, unsigned* hist) {
   op_begin();
   __shared__ unsigned cnt[256];
   cnt[threadIdx.x] = 0;
@@ -108,13 +108,13 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_count_kernel(const void* __
 #pragma unroll
   for (int j = 0; j < SORT_TILE / SORT_THREADS; j++) {
     const long i = base + j * SORT_THREADS + threadIdx.x;
-    if (i < tokens) atomicAdd(&cnt[((FIRST ? token_key(ids, index_type, i, vocab) : __ldg(keys + i)) >> shift) & 255], 1u);
+    if (i < tokens) atomicAdd(&cnt[((FIRST ? token_key(ids, index_type, i, vocab) : ld(keys + i)) >> shift) & 255], 1u);
   }
   __syncthreads();
   hist[by_tile ? blockIdx.x * 256L + threadIdx.x : (long)threadIdx.x * gridDim.x + blockIdx.x] = cnt[threadIdx.x];      // digit by digit for the scan
 }
 // In place: every count becomes the sum of those before it.  One block.
-__global__ void __launch_bounds__(1024) sort_scan_kernel(unsigned* __restrict__ hist, long n) {
+__global__ void __launch_bounds__(1024) sort_scan_kernel(unsigned* hist, long n) {
   op_begin();
   __shared__ unsigned sums[32];
   __shared__ unsigned carry;
@@ -143,8 +143,8 @@ __global__ void __launch_bounds__(1024) sort_scan_kernel(unsigned* __restrict__ 
 }
 // SCAN: the counts are as sort_count_kernel left them, and every tile adds up what lies before its own (few tiles: a launch less a pass).
 template <bool FIRST, bool SCAN>
-__global__ void __launch_bounds__(SORT_THREADS) sort_move_kernel(const void* __restrict__ ids, int index_type, const unsigned* __restrict__ keys, const int* __restrict__ order, long tokens, long vocab, int shift,
-                                                                 const unsigned* __restrict__ hist, unsigned* __restrict__ keys_out, int* __restrict__ order_out) {
+__global__ void __launch_bounds__(SORT_THREADS) sort_move_kernel(const void* ids, int index_type, const unsigned* keys, const int* order, long tokens, long vocab, int shift,
+                                                                 const unsigned* hist, unsigned* keys_out, int* order_out) {
   constexpr int W = SORT_THREADS / 32, PER = SORT_TILE / SORT_THREADS;      // rows of 32 places of a warp
   op_begin();
   __shared__ unsigned cnt[W * 256];
@@ -154,8 +154,8 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_move_kernel(const void* __r
 #pragma unroll
   for (int j = 0; j < PER; j++) {
     const long i = first + j * 32 + lane; const bool on = i < tokens;
-    key[j] = !on ? 0u : FIRST ? token_key(ids, index_type, i, vocab) : __ldg(keys + i);
-    val[j] = !on ? 0 : FIRST ? (int)i : __ldg(order + i);
+    key[j] = !on ? 0u : FIRST ? token_key(ids, index_type, i, vocab) : ld(keys + i);
+    val[j] = !on ? 0 : FIRST ? (int)i : ld(order + i);
   }
   for (int e = tid; e < W * 256; e += SORT_THREADS) cnt[e] = 0;
   __syncthreads();
@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_move_kernel(const void* __r
     __shared__ unsigned sums[W];
     unsigned before = 0, total = 0;
 #pragma unroll 32
-    for (int t = 0; t < (int)gridDim.x; t++) { const unsigned c = __ldg(hist + t * 256 + tid); if (t < (int)blockIdx.x) before += c; total += c; }
+    for (int t = 0; t < (int)gridDim.x; t++) { const unsigned c = ld(hist + t * 256 + tid); if (t < (int)blockIdx.x) before += c; total += c; }
     unsigned s = total;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) { const unsigned u = __shfl_up_sync(0xffffffffu, s, o); if (lane >= o) s += u; }
@@ -175,7 +175,7 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_move_kernel(const void* __r
     __syncthreads();
     for (int w = 0; w < warp; w++) s += sums[w];
     at0 = s - total + before;
-  } else at0 = __ldg(hist + (long)tid * gridDim.x + blockIdx.x);
+  } else at0 = ld(hist + (long)tid * gridDim.x + blockIdx.x);
 #pragma unroll
   for (int w = 0; w < W; w++) { const unsigned c = cnt[w * 256 + tid]; cnt[w * 256 + tid] = at0; at0 += c; }
   __syncthreads();
@@ -189,17 +189,17 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_move_kernel(const void* __r
 
 // ------------------------------------------------------------------ sums
 // First place of the sorted keys that is not below `key`.
-__device__ __forceinline__ long first_place(const unsigned* __restrict__ keys, long n, unsigned key) {
+__device__ __forceinline__ long first_place(const unsigned* keys, long n, unsigned key) {
   long lo = 0, hi = n;
-  while (lo < hi) { const long mid = (lo + hi) >> 1; if (__ldg(keys + mid) < key) lo = mid + 1; else hi = mid; }
+  while (lo < hi) { const long mid = (lo + hi) >> 1; if (ld(keys + mid) < key) lo = mid + 1; else hi = mid; }
   return lo;
 }
 constexpr int EMB_THREADS = 128, EMB_ZERO_ROWS = 32;
 // Columns of a block: EMB_THREADS accesses of V elements; blockIdx.y counts those.  Blocks below `chunks` sum a piece each, the others zero the rows among
 // EMB_ZERO_ROWS that no token names.
 template <class T, int V>
-__global__ void __launch_bounds__(EMB_THREADS) embedding_sum_kernel(const T* __restrict__ dout, long stride, const unsigned* __restrict__ keys, const int* __restrict__ order, long tokens, long vocab, int dim,
-                                                                    float scale, int chunk, long chunks, float* __restrict__ dtable, float* __restrict__ partial) {
+__global__ void __launch_bounds__(EMB_THREADS) embedding_sum_kernel(const T* dout, long stride, const unsigned* keys, const int* order, long tokens, long vocab, int dim,
+                                                                    float scale, int chunk, long chunks, float* dtable, float* partial) {
   op_begin();
   const long col = ((long)blockIdx.y * EMB_THREADS + threadIdx.x) * V; const bool in = col < dim;
   auto put = [&](float* row, const float (&v)[V]) {
@@ -213,7 +213,7 @@ __global__ void __launch_bounds__(EMB_THREADS) embedding_sum_kernel(const T* __r
   if (blockIdx.x >= chunks) {
     const long v0 = (blockIdx.x - chunks) * EMB_ZERO_ROWS; const int lane = threadIdx.x & 31;
     const long v = v0 + lane; bool absent = false;
-    if (v < vocab) { const long at = first_place(keys, tokens, (unsigned)v); absent = at >= tokens || __ldg(keys + at) != (unsigned)v; }
+    if (v < vocab) { const long at = first_place(keys, tokens, (unsigned)v); absent = at >= tokens || ld(keys + at) != (unsigned)v; }
     unsigned todo = __ballot_sync(0xffffffffu, absent);
     float zero[V];
 #pragma unroll
@@ -223,9 +223,9 @@ __global__ void __launch_bounds__(EMB_THREADS) embedding_sum_kernel(const T* __r
   }
   const long first = (long)blockIdx.x * chunk, last = min(tokens, first + chunk);
   __shared__ unsigned ks[64 + 2]; __shared__ int os[64];
-  for (int e = threadIdx.x; e < (int)(last - first); e += EMB_THREADS) { ks[e + 1] = __ldg(keys + first + e); os[e] = __ldg(order + first + e); }
-  if (threadIdx.x == 0) ks[0] = first > 0 ? __ldg(keys + first - 1) : 0xffffffffu;
-  if (threadIdx.x == 1) ks[last - first + 1] = last < tokens ? __ldg(keys + last) : 0xffffffffu;
+  for (int e = threadIdx.x; e < (int)(last - first); e += EMB_THREADS) { ks[e + 1] = ld(keys + first + e); os[e] = ld(order + first + e); }
+  if (threadIdx.x == 0) ks[0] = first > 0 ? ld(keys + first - 1) : 0xffffffffu;
+  if (threadIdx.x == 1) ks[last - first + 1] = last < tokens ? ld(keys + last) : 0xffffffffu;
   __syncthreads();
   const int n = (int)(last - first);
   constexpr int U = 8;                                               // rows under way
@@ -271,7 +271,7 @@ __global__ void __launch_bounds__(EMB_THREADS) embedding_sum_kernel(const T* __r
 // piece: 18 us for 131072 tokens of 1024; looking the run's end up by bisection and 32 columns at a time: 127.)
 constexpr int JOIN_COLS = 64, JOIN_GROUPS = 4, JOIN_LONG = 32;
 template <int V>
-__global__ void __launch_bounds__(JOIN_GROUPS * JOIN_COLS) embedding_join_kernel(const unsigned* __restrict__ keys, long tokens, long vocab, int dim, int chunk, long chunks, const float* __restrict__ partial, float* __restrict__ dtable) {
+__global__ void __launch_bounds__(JOIN_GROUPS * JOIN_COLS) embedding_join_kernel(const unsigned* keys, long tokens, long vocab, int dim, int chunk, long chunks, const float* partial, float* dtable) {
   op_begin();
   __shared__ float red[JOIN_GROUPS - 1][JOIN_COLS * V];
   __shared__ long length[JOIN_GROUPS]; __shared__ unsigned key_of[JOIN_GROUPS];
@@ -280,18 +280,18 @@ __global__ void __launch_bounds__(JOIN_GROUPS * JOIN_COLS) embedding_join_kernel
   long m = 0;                                                        // pieces behind this one that begin within a run which began here
   unsigned key = 0;
   if (c + 1 < chunks) {                                              // (a last piece has nothing behind it)
-    key = __ldg(keys + (c + 1) * chunk - 1);
-    const unsigned next = __ldg(keys + (c + 1) * chunk), begin = __ldg(keys + c * chunk), before = c > 0 ? __ldg(keys + c * chunk - 1) : 0xffffffffu;
+    key = ld(keys + (c + 1) * chunk - 1);
+    const unsigned next = ld(keys + (c + 1) * chunk), begin = ld(keys + c * chunk), before = c > 0 ? ld(keys + c * chunk - 1) : 0xffffffffu;
     if (key < (unsigned)vocab && next == key && !(begin == key && before == key))
       for (long i0 = c + 2;; i0 += 32) {                             // the first piece behind that does not begin within the run
         const long i = i0 + (threadIdx.x & 31);
-        const unsigned other = __ballot_sync(0xffffffffu, i >= chunks || __ldg(keys + i * chunk) != key);
+        const unsigned other = __ballot_sync(0xffffffffu, i >= chunks || ld(keys + i * chunk) != key);
         if (other) { m = i0 + __ffs(other) - 1 - c - 1; break; }
       }
   }
   auto add = [&](float (&v)[V], const float* row) {
-    if constexpr (V == 1) v[0] += __ldg(row + col);
-    else { const float4 u = __ldg(reinterpret_cast<const float4*>(row + col)); v[0] += u.x; v[1] += u.y; v[2] += u.z; v[3] += u.w; }
+    if constexpr (V == 1) v[0] += ld(row + col);
+    else { const float4 u = ld(reinterpret_cast<const float4*>(row + col)); v[0] += u.x; v[1] += u.y; v[2] += u.z; v[3] += u.w; }
   };
   auto put = [&](const float (&v)[V], unsigned k) {
     float* out = dtable + (long)k * dim + col;

@@ -364,7 +364,7 @@ constexpr int FEW_WARPS = 8;
 // errors average out, it would be 10 to 25 % and is not done.)
 // GATE: out[t][n] = act(x w0^T) (x w1^T), else x w0^T.  n in blocks of 16, `cl` blocks of a cluster share the contraction.  NB: blocks of eight tokens.
 template <class T, bool GATE, int NB, int ACT>
-__global__ void __launch_bounds__(32 * FEW_WARPS) fg_few_kernel(const T* x, long x_stride, const T* __restrict__ w0, const T* __restrict__ w1, int tokens, int N, int K, T* __restrict__ out, long out_stride, int cl) {
+__global__ void __launch_bounds__(32 * FEW_WARPS) fg_few_kernel(const T* x, long x_stride, const T* w0, const T* w1, int tokens, int N, int K, T* out, long out_stride, int cl) {
   namespace cg = cooperative_groups;
   constexpr int MATS = GATE ? 2 : 1;
   __shared__ float red[FEW_WARPS][MATS * NB][4][32];

@@ -23,7 +23,7 @@ struct QkParams {
 // and pair were a fifth of the forward pass's time.)
 __device__ __forceinline__ void qk_frequencies(const QkParams& p, unsigned long long* fx) {
   for (int i = threadIdx.x; i < p.rot >> 1; i += blockDim.x) {
-    double f = __ldg(p.freq + i) * 0.15915494309189533577;           // 1 / (2 pi)
+    double f = ld(p.freq + i) * 0.15915494309189533577;           // 1 / (2 pi)
     f -= floor(f);
     fx[i] = (unsigned long long)(f * 18446744073709551616.0);
   }
@@ -55,12 +55,12 @@ template <class T, int V, bool FULL> struct QkLane {
     has_a = FULL || pa < pieces; has_b = FULL || pb < pieces;
   }
   __device__ __forceinline__ void gain(const float* g) {
-    auto at = [&](bool has, int e) { return g && has ? __ldg(reinterpret_cast<const float2*>(g + e)) : make_float2(1.f, 1.f); };
+    auto at = [&](bool has, int e) { return g && has ? ld(reinterpret_cast<const float2*>(g + e)) : make_float2(1.f, 1.f); };
     if (reinterpret_cast<uintptr_t>(g) & 7) {                        // (a gain need only be aligned to its type)
 #pragma unroll
       for (int j = 0; j < P; j++) {
-        ga[j] = has_a ? make_float2(__ldg(g + pa * V + 2 * j), __ldg(g + pa * V + 2 * j + 1)) : make_float2(1.f, 1.f);
-        gb[j] = has_b ? make_float2(__ldg(g + pb * V + 2 * j), __ldg(g + pb * V + 2 * j + 1)) : make_float2(1.f, 1.f);
+        ga[j] = has_a ? make_float2(ld(g + pa * V + 2 * j), ld(g + pa * V + 2 * j + 1)) : make_float2(1.f, 1.f);
+        gb[j] = has_b ? make_float2(ld(g + pb * V + 2 * j), ld(g + pb * V + 2 * j + 1)) : make_float2(1.f, 1.f);
       }
       return;
     }
@@ -251,7 +251,7 @@ __global__ void __launch_bounds__(32 * QK_ROW_WARPS, QK_PER_SM) qk_rows_kernel(c
   {
     auto first = [&](int i) { return p.inter ? 2 * i : i; };
     auto second = [&](int i) { return p.inter ? 2 * i + 1 : i + half; };
-    auto gain = [&](int e) { return h.gain ? __ldg(h.gain + e) : 1.f; };
+    auto gain = [&](int e) { return h.gain ? ld(h.gain + e) : 1.f; };
     if constexpr (BWD) {
       __syncthreads();
       for (int e = threadIdx.x; e < QK_ROW_WARPS * p.head; e += blockDim.x) acc[e - warp * p.head] = 0.f;
@@ -312,14 +312,14 @@ __global__ void __launch_bounds__(32 * QK_ROW_WARPS, QK_PER_SM) qk_rows_kernel(c
 }
 
 // dgain[e] = sum of the blocks' partial sums: 32 threads a column, each a run of neighbouring blocks, in order
-__global__ void __launch_bounds__(1024) qk_gain_kernel(const float* __restrict__ partial, int blocks, int head, float* __restrict__ dq, float* __restrict__ dk) {
+__global__ void __launch_bounds__(1024) qk_gain_kernel(const float* partial, int blocks, int head, float* dq, float* dk) {
   op_begin();
   __shared__ float red[32][33];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, col = blockIdx.x * 32 + lane, per = (blocks + 31) / 32;
   float v = 0.f;
   if (col < 2 * head && (col < head ? dq : dk)) {
 #pragma unroll 8
-    for (int b = w * per; b < min(blocks, (w + 1) * per); b++) v += __ldg(partial + (long)b * 2 * head + col);
+    for (int b = w * per; b < min(blocks, (w + 1) * per); b++) v += ld(partial + (long)b * 2 * head + col);
   }
   red[w][lane] = v;
   __syncthreads();
