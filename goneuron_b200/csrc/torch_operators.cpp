@@ -79,6 +79,12 @@ Rows rows(const char* name, const Tensor& t, const Tensor* like = nullptr) {
   }
   return Rows{n, dim, stride};
 }
+// A tensor of the caller's that is written.  What autograd knows of it would not be true any more; what kept it for a backward pass notices by its version.
+void writable(const char* name, const Tensor& t) {
+  if (at::GradMode::is_enabled() && t.requires_grad()) wrong(std::string(name) + " requires a gradient and would be overwritten: call under torch.no_grad(), or give another tensor");
+  if (t.is_inference() && !c10::InferenceMode::is_enabled()) wrong(std::string(name) + " was made in inference mode and can only be written there");
+}
+void written(const Tensor& t) { t.unsafeGetTensorImpl()->bump_version(); }
 Tensor empty(const Tensor& like, at::IntArrayRef shape) { return at::empty(shape, like.options()); }
 Tensor empty(const Tensor& like, at::IntArrayRef shape, at::ScalarType type) { return at::empty(shape, like.options().dtype(type)); }
 Tensor bytes(const Tensor& like, int64_t n) { return at::empty({n}, like.options().dtype(at::kByte)); }
@@ -131,9 +137,11 @@ std::tuple<Tensor, OptTensor> qk_norm_rope(uint64_t handle, int index, const Ten
   if (q_out && k && !k_out) wrong("out: a pair of tensors is needed");
   gn_heads qo{}, ko{};
   Tensor qt = q_out ? *q_out : empty(q, q.sizes()); OptTensor kt;
-  heads_of("out[0]", qt, &qo, &q); here(a.d, "out[0]", qt);
-  if (k) { kt = k_out ? *k_out : empty(*k, k->sizes()); heads_of("out[1]", *kt, &ko, &*k); here(a.d, "out[1]", *kt); }
+  heads_of("out[0]", qt, &qo, &q); writable("out[0]", qt); here(a.d, "out[0]", qt);
+  if (k) { kt = k_out ? *k_out : empty(*k, k->sizes()); heads_of("out[1]", *kt, &ko, &*k); writable("out[1]", *kt); here(a.d, "out[1]", *kt); }
   check(gn_op_qk_norm_rope(a.d.ctx, a.dtype, a.n, (int)a.size, a.rotated, interleaved, (float)eps, &a.q, a.key(a.k), a.gain_q, a.gain_k, a.positions, a.wide, a.frequencies, &qo, a.key(ko), a.d.stream()));
+  if (q_out) written(*q_out);
+  if (k && k_out) written(*k_out);
   return {qt, kt};
 }
 
@@ -165,7 +173,7 @@ std::tuple<Tensor, OptTensor> distill(uint64_t handle, int index, const Tensor& 
   if (!top_ids.sizes().equals(top_logits.sizes())) wrong("top_ids has shape " + shape_of(top_ids) + ", top_logits " + shape_of(top_logits));
   if (top_ids.size(1) > INT32_MAX) wrong("top_ids has too many columns");
   if (row_weight) { dense("row_weight", *row_weight, at::kFloat, {n}); }
-  if (out) floating("out", *out, &logits);
+  if (out) { floating("out", *out, &logits); writable("out", *out); }
   here(d, "logits", logits); here(d, "top_ids", top_ids); here(d, "top_logits", top_logits);
   if (row_weight) here(d, "row_weight", *row_weight);
   if (out) here(d, "out", *out);
@@ -174,6 +182,7 @@ std::tuple<Tensor, OptTensor> distill(uint64_t handle, int index, const Tensor& 
   if (gradient) grad = out ? *out : empty(logits, logits.sizes());
   check(gn_op_distill(d.ctx, dtype_of("logits", logits), n, vocab, top, (float)temperature, ptr(logits), logits.stride(0), ptr(top_ids), wide, (float*)ptr(top_logits), (float*)ptr(row_weight), (float*)ptr(loss), ptr(grad),
                       gradient ? grad->stride(0) : 0, d.stream()));
+  if (out) written(*out);
   return {loss, grad};
 }
 

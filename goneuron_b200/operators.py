@@ -3,9 +3,12 @@ include/goneuron_cuda.h, which states each operator's formula and limits).
 
 They have no counterpart in the reference, whose layers are float32 on host slices.  Every function takes a `Device`
 (goneuron_b200.sequential) and tensors on that GPU; it enqueues its kernels on torch's current stream there, waits for nothing
-and can be captured into a CUDA graph.  Outputs and workspaces are torch allocations of the call; inputs' autograd history is not
-followed.  Wrong arguments raise ValueError (TypeError where a tensor is none), failures of the library GoNeuronCudaError; what
-only the kernels can find (an index out of range, a bounded wait that gave up) is kept until `check` reads it.
+and can be captured into a CUDA graph.  Outputs and workspaces are torch allocations of the call.  Inputs' autograd history is not
+followed: outputs do not require a gradient, and each operator's gradient is a call of its own.  A tensor given as `out` is
+written like any that torch changes in place: one that requires a gradient is refused outside torch.no_grad(), and a backward
+pass that has kept it raises torch's error.  Wrong arguments raise ValueError (TypeError where a tensor is none), failures of
+the library GoNeuronCudaError; what only the kernels can find (an index out of range, a bounded wait that gave up) is kept
+until `check` reads it.
 
 The functions' bodies are compiled (csrc/torch_operators.cpp)."""
 import torch  # noqa: F401  (its libraries have to be there before the module below)
