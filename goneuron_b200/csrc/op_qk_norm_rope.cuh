@@ -385,6 +385,7 @@ int gn_op_qk_norm_rope(gn_ctx* ctx, int dtype, int64_t tokens, int head_size, in
   if (!wrong && k) wrong = check_heads(a, k_out, k->heads, true);
   if (!wrong) wrong = check_in_place(q, q_out);
   if (!wrong) wrong = check_in_place(k, k_out);
+  if (!wrong && k && tokens) for (const char* e : {check_apart(q_out, k), check_apart(k_out, q), check_apart(q_out, k_out)}) if (e) wrong = e;
   GN_OP_BEGIN("op_qk_norm_rope", wrong);
   if (tokens == 0 || q->heads + (k ? k->heads : 0) == 0) return GN_OK;
   const int sms = ctx->c.sm_count; const gn_heads* all[] = {q, k, q_out, k ? k_out : nullptr};
@@ -412,6 +413,7 @@ int gn_op_qk_norm_rope_backward(gn_ctx* ctx, int dtype, int64_t tokens, int head
   if (!wrong && k) wrong = check_heads(a, dk, k->heads, true);
   if (!wrong) wrong = check_in_place(dq_out, dq);
   if (!wrong && k) wrong = check_in_place(dk_out, dk);
+  if (!wrong && k && tokens) for (const char* e : {check_apart(dq, k), check_apart(dq, dk_out), check_apart(dk, q), check_apart(dk, dq_out), check_apart(dq, dk)}) if (e) wrong = e;
   if (!wrong && (!aligned_to(dgain_q, 4) || !aligned_to(dgain_k, 4))) wrong = "a pointer is not aligned to its type";
   if (!wrong && dgain_k && !k) wrong = "dgain_k without k";
   GN_OP_BEGIN("op_qk_norm_rope_backward", wrong);

@@ -4,6 +4,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
+#include <cstdlib>
 #include <initializer_list>
 
 #include "../../include/goneuron_cuda.h"
@@ -63,6 +64,10 @@ inline const char* check_qk(const QkArgs& a) {
 inline const char* check_in_place(const gn_heads* in, const gn_heads* out) {
   return in && out && in->data && in->data == out->data && (in->token_stride != out->token_stride || in->head_stride != out->head_stride) ? "in place, both tensors' strides have to be the same" : nullptr;
 }
+// A tensor that is written may be its own input, but not the other one's, nor the other one that is written: blocks of queries and of keys do not wait for each other.
+inline const char* check_apart(const gn_heads* written, const gn_heads* other) {
+  return written && other && written->data && written->data == other->data && written->heads && other->heads ? "an output of the queries lies on a tensor of the keys, or the other way round" : nullptr;
+}
 // Groups of lanes: a lane has two pieces of a row, 16 bytes each, or 8 where 16 do not fit and the type has 16 bits; a row's lanes are neighbours, 2 to 32 of them.  0: the
 // pieces do not fit (sizes, strides or pointers, pairs that end inside one, rows of more than 64 pieces); a row that neither fits goes element by element.
 inline int qk_group(int dtype, int head_size, int rotated, bool interleaved, const gn_heads* const* t, int n, int piece = 16) {
@@ -109,6 +114,11 @@ inline const char* check_distill(int dtype, int64_t rows, int64_t vocab, int top
   if (!aligned_to(top_logits, 4) || !aligned_to(weight, 4) || !aligned_to(loss, 4)) return "a pointer is not aligned to its type";
   if (row_stride < 0 || (rows > 1 && dlogits && drow_stride < vocab)) return "rows overlap, or a stride is negative";
   if (dlogits && dlogits == logits && rows > 1 && row_stride != drow_stride) return "in place, both strides have to be the same";
+  if (dlogits && dlogits != logits && (rows == 1 || row_stride == drow_stride)) {      // rows of one may lie partly on rows of the other: those nearest to each other, t rows apart
+    const int64_t d = (int64_t)(reinterpret_cast<intptr_t>(dlogits) - reinterpret_cast<intptr_t>(logits)) / dtype_size(dtype), down = rows == 1 ? 0 : d / row_stride;
+    for (int64_t t = down - 1; t <= down + 1; t++)
+      if (std::llabs(t) < rows && std::llabs(d - t * row_stride) < vocab) return "dlogits lies partly on logits";
+  }
   return nullptr;
 }
 // A row is kept in the shared memory of `cluster` blocks, `per` 16-byte pieces in each, some eight of them a thread.  cluster 0: it does not fit and is read again instead.  Parts of up to 104 KB leave

@@ -39,7 +39,8 @@ def check(dev):
 def qk_norm_rope(dev, q, k, gain_q=None, gain_k=None, positions=None, frequencies=None, eps=1e-5, interleaved=False, out=None):
     """RMS norm of every head of q and k ([tokens, heads, size] or [batch, tokens, heads, size]; any strides of the first dimensions,
     k may be None) with gains [size] (float32), then the rotation of the pairs by positions * frequencies.  Without frequencies
-    ([rotated / 2], float64) nothing is rotated.  out: a pair of tensors for the results, q and k themselves among them."""
+    ([rotated / 2], float64) nothing is rotated.  out: a pair of tensors for the results, (q, k) themselves for in place; the queries' must not lie on the
+    keys', nor the other way round."""
     qo, ko = (None, None) if out is None else out
     return _ops.qk_norm_rope(_handle(dev), dev.device, q, k, gain_q, gain_k, positions, frequencies, eps, interleaved, qo, ko)
 
@@ -56,7 +57,8 @@ def distill_loss(dev, logits, top_ids, top_logits, temperature=1.0, row_weight=N
 
 
 def distill_loss_grad(dev, logits, top_ids, top_logits, temperature=1.0, row_weight=None, out=None):
-    """(loss, dlogits): the same with the derivative of each row's loss by its logits, which are read once.  out: a tensor for dlogits, logits among them."""
+    """(loss, dlogits): the same with the derivative of each row's loss by its logits, which are read once.  out: a tensor for dlogits, logits itself for in place, else
+    not on any part of it."""
     return _ops.distill(_handle(dev), dev.device, logits, top_ids, top_logits, temperature, row_weight, True, out)
 
 
