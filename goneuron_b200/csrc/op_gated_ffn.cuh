@@ -57,15 +57,16 @@ inline uint32_t fg_idesc(bool bf16, bool amn, bool bmn, int N) {
   return (1u << 4) | (f << 7) | (f << 10) | ((amn ? 1u : 0u) << 15) | ((bmn ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(FG_BM >> 4) << 24);
 }
 
-// act(g) u, and the factors of dh in dg and du
+// act(g) u, and the factors of dh in dg and du.  (relu lets a NaN through, which fmaxf would not.)
+__device__ __forceinline__ float fg_relu(float g) { return g < 0.f ? 0.f : g; }
 __device__ __forceinline__ float fg_sigmoid(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
-template <int act> __device__ __forceinline__ float fg_act(float g) { return act == GN_ACT_SILU ? g * fg_sigmoid(g) : act == GN_ACT_GELU ? gelu_f(g) : fmaxf(g, 0.f); }
+template <int act> __device__ __forceinline__ float fg_act(float g) { return act == GN_ACT_SILU ? g * fg_sigmoid(g) : act == GN_ACT_GELU ? gelu_f(g) : fg_relu(g); }
 template <int act> __device__ __forceinline__ void fg_act_grad(float g, float& a, float& da) {
   if constexpr (act == GN_ACT_SILU) { const float p = fg_sigmoid(g); a = g * p; da = p * (1.f + g * (1.f - p)); }
   else if constexpr (act == GN_ACT_GELU) {                                     // (1 + tanh z) / 2 = sigmoid(2 z) = p, 1 - tanh^2 z = 4 p (1 - p)
     const float p = fg_sigmoid(g * fmaf(0.07135481627f * g, g, 1.5957691216057308f));
     a = g * p; da = p + g * 2.f * p * (1.f - p) * fminf(fmaf(0.10703222440890925f * g, g, 0.7978845608028654f), 3e38f);      // (far out 0 times a square that may not be finite)
-  } else { a = fmaxf(g, 0.f); da = g > 0.f ? 1.f : 0.f; }
+  } else { a = fg_relu(g); da = g > 0.f ? 1.f : 0.f; }
 }
 
 // 16 float32 values of a lane as the upper halves of two in a word, and the bytes below of four: 48 bytes.  (What comes back repeats that byte below itself: infinities and zeros stay, and so
