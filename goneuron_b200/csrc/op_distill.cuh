@@ -323,12 +323,12 @@ __global__ void __launch_bounds__(1024) distill_long_kernel(const __grid_constan
 
 template <class T, bool GRAD>
 inline int distill_launch(gn_ctx* ctx, const DistillParams& p, void* stream) {
-  const int sms = ctx->c.sm_count; const DistillPlan pl = distill_plan(p.rows, p.vocab, (int)sizeof(T), sms);
+  const int sms = ctx->c.sm_count; const DistillPlan pl = distill_plan(p.rows, p.vocab, (int)sizeof(T), sms, p.top);
   const int tsmem = teacher_smem(p.top);
   if (pl.cluster == 0) return op_launch("distill_long", stream, distill_long_kernel<T, GRAD>, dim3((unsigned)std::min<int64_t>(p.rows, 2L * sms)), dim3(1024), tsmem, 0, p);
   constexpr int V = Vec<T>::N;
   const bool whole = p.vocab % V == 0 && p.stride % V == 0 && aligned_to(p.logits, 16) && (!GRAD || (p.dstride % V == 0 && aligned_to(p.dlogits, 16)));
-  const int smem = pl.per * 16 + tsmem; const int64_t per_sm = std::max<int64_t>(1, std::min<int64_t>({2048 / (pl.threads + 32), 32, 65536 / (40 * (pl.threads + 32)), 224 * 1024 / (smem + 3 * 1024)}));
+  const int smem = pl.per * 16 + tsmem; const int64_t per_sm = std::max<int64_t>(1, std::min<int64_t>({2048 / (pl.threads + 32), 32, 65536 / (40 * (pl.threads + 32)), DISTILL_SM_SMEM / (smem + DISTILL_FIXED)}));
   const dim3 grid((unsigned)(std::min<int64_t>(p.rows, std::max<int64_t>(1, (int64_t)sms * per_sm / pl.cluster)) * pl.cluster));
   auto go = [&](auto kernel) { if (smem > 40 * 1024) GN_TRY(op_smem("distill", kernel, DISTILL_SMEM_MOST)); return op_launch("distill", stream, kernel, grid, dim3(pl.threads + 32), smem, pl.cluster, p, pl.cluster, pl.per); };
   return whole ? go(distill_kernel<T, GRAD, true>) : go(distill_kernel<T, GRAD, false>);

@@ -121,16 +121,20 @@ inline const char* check_distill(int dtype, int64_t rows, int64_t vocab, int top
   }
   return nullptr;
 }
-// A row is kept in the shared memory of `cluster` blocks, `per` 16-byte pieces in each, some eight of them a thread.  cluster 0: it does not fit and is read again instead.  Parts of up to 104 KB leave
-// room for two blocks on a multiprocessor, which overlap each other's phases; a cluster's barrier costs more than that gives, so that four and eight blocks are taken only where two cannot hold the
-// row (515 rows of 100003, f16: one block 66 us, two 61, four 80; 2000 rows of 130000, bf16: two 291, four 330), and four again only where their parts leave room for two on a multiprocessor
+// Beside dynamic shared memory a block takes up to 2 KB of its own and 1 KB that is set apart; a multiprocessor has 228 KB.
+constexpr int DISTILL_FIXED = 3 * 1024, DISTILL_SM_SMEM = 228 * 1024;
+// A row is kept in the shared memory of `cluster` blocks, `per` 16-byte pieces in each, some eight of them a thread.  cluster 0: it does not fit and is read again instead.  Parts of up to 104 KB, less where
+// the teacher has more than 64 entries, leave room for two blocks on a multiprocessor, which overlap each other's phases (4096 rows of 50257, bf16, 256 entries: one block a row and multiprocessor 682 us, two
+// blocks a row 564; 53000 with 64 entries, two blocks a multiprocessor instead of one: 238 and 191); a cluster's barrier costs more than that gives, so that four and eight blocks are taken only where two cannot
+// hold the row (515 rows of 100003, f16: one block 66 us, two 61, four 80; 2000 rows of 130000, bf16: two 291, four 330), and four again only where their parts leave room for two on a multiprocessor
 // (512 rows of 128000, f32: four 216 us, eight 166; of 250000, bf16: 256 and 180).  Few rows are cut further, so that they fill the multiprocessors, down to two
 // thousand elements per block.
 struct DistillPlan { int cluster, threads, per; };
-inline DistillPlan distill_plan(int64_t rows, int64_t vocab, int size, int sms) {
+inline DistillPlan distill_plan(int64_t rows, int64_t vocab, int size, int sms, int top = 0) {
+  const int64_t part = std::min(DISTILL_PART, DISTILL_SM_SMEM / 2 - DISTILL_FIXED - teacher_smem(top));
   const int64_t v = 16 / size, pieces = ceil_div(vocab + v - 1, v);  // (a row may begin inside a piece)
   int c = 1;
-  while (c < 8 && ceil_div(pieces, c) * 16 > (c == 2 ? DISTILL_PART_MOST : DISTILL_PART)) c *= 2;
+  while (c < 8 && ceil_div(pieces, c) * 16 > (c == 2 ? DISTILL_PART_MOST : part)) c *= 2;
   if (ceil_div(pieces, c) * 16 > DISTILL_PART_MOST) return {0, 1024, 0};
   while (c < 8 && rows * c * 2 <= sms && vocab >= 4096L * c) c *= 2;
   const int64_t per = ceil_div(pieces, c);
