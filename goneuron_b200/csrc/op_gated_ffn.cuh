@@ -17,7 +17,8 @@
 // them with whole 128-byte lines.  In 16 bits their rounding would add to those of dg and du and the error of dx be 1.7 times that of its own rounding instead of 1.4; the last 8 bits of
 // float32 would be a quarter of what the epilogue of dh, which memory bounds, has to read.
 // h, dg and du are rounded to 16 bits because the tensor cores read them as operands: y, dx and the weights' gradients have some 1.4 times the error of their own rounding, and of one to four tokens,
-// whose sums few large terms make up, 1.2 to 1.7 times.
+// whose sums few large terms make up, 1.2 to 1.7 times.  They have that type's range as well: in float16 infinite above 65504, zero below 2^-25.  There is no scale, which would have to be known before
+// the tiles of a row are: what is too large makes its row not finite, never finite and wrong.
 // Few output tiles: the contraction is cut into slices whose float32 sums a second launch adds in order.
 //
 // Waits are bounded as in the contraction engine: a wait that gives up sets the status word, every role of the block leaves its loops, copies and MMAs in flight are waited for

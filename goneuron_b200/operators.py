@@ -81,11 +81,13 @@ def _activation(name):
 
 def gated_ffn(dev, x, w_gate, w_up, w_down, activation="silu", save=False):
     """(act(x w_gate^T) * (x w_up^T)) w_down^T for x [..., dim], w_gate and w_up [ff, dim], w_down [dim, ff]; activation "silu", "gelu" (tanh form)
-    or "relu".  save: also returns what gated_ffn_backward reads, (y, saved)."""
+    or "relu".  save: also returns what gated_ffn_backward reads, (y, saved).  act(..) * (..) is rounded to x's type between the
+    products: in float16 above 65504 it is infinite, and so is its row of y, where bfloat16 would hold it."""
     r = _ops.gated_ffn(_handle(dev), dev.device, x, w_gate, w_up, w_down, _activation(activation), save)
     return r if save else r[0]
 
 
 def gated_ffn_backward(dev, dy, x, w_gate, w_up, w_down, saved, activation="silu"):
-    """Gradients (dx, dw_gate, dw_up, dw_down) from that of y, the forward call's inputs and what it saved."""
+    """Gradients (dx, dw_gate, dw_up, dw_down) from that of y, the forward call's inputs and what it saved.  The gradients of
+    both projections are rounded to x's type on the way: in float16 a loss scale has to leave room for them (65504), and what is below 2^-25 is lost."""
     return _ops.gated_ffn_backward(_handle(dev), dev.device, dy, x, w_gate, w_up, w_down, saved, _activation(activation))

@@ -355,7 +355,9 @@ int gn_op_embedding_backward(gn_ctx* ctx, int dtype, int64_t tokens, int64_t voc
  * Wd [dim, ff], dense; all GN_F16 or GN_BF16 (GN_F32: GN_ERR_UNSUPPORTED, TransformerBlock has the 32-bit form).  activation: GN_ACT_SILU,
  * GN_ACT_GELU (tanh form) or GN_ACT_RELU.  dim and ff are multiples of 8, pointers 16-byte aligned, x_stride and y_stride multiples of 8.
  * One kernel forms both projections, the activation and the product; h is rounded to `dtype` between the two kernels (up to 8 tokens without
- * `saved` it is kept with twice its bits).  `saved`: null, or
+ * `saved` it is kept with twice its bits), and so are act'(g) u dh and act(g) dh in the backward pass.  In GN_F16 what is above 65504 there is
+ * infinite and what is below 2^-25 zero: a row whose h does not fit has a y that is not finite, a loss scale has to leave room for those two
+ * products, and wide ranges want GN_BF16.  `saved`: null, or
  * gn_op_gated_ffn_saved bytes that the backward pass reads (both projections with 24 bits in the kernels' own order, and h). */
 int gn_op_gated_ffn_saved(gn_ctx* ctx, int64_t tokens, int dim, int ff, int64_t* bytes);
 int gn_op_gated_ffn_workspace(gn_ctx* ctx, int64_t tokens, int dim, int ff, int backward, int64_t* bytes);
