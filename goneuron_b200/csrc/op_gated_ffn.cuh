@@ -566,7 +566,7 @@ int gn_op_gated_ffn_workspace(gn_ctx* ctx, int64_t tokens, int dim, int ff, int 
 int gn_op_gated_ffn(gn_ctx* ctx, int dtype, int activation, int64_t tokens, int dim, int ff, const void* x, int64_t x_stride, const void* w_gate, const void* w_up, const void* w_down, void* y, int64_t y_stride, void* saved,
                     void* workspace, int64_t workspace_bytes, void* stream) {
   using namespace gn;
-  if (ctx && ctx->alive && dtype == GN_F32) return fail(GN_ERR_UNSUPPORTED, "op_gated_ffn: GN_F32 is not built (TransformerBlock has the 32-bit form)");
+  if (ctx && ctx->alive && dtype == GN_F32) return fail(GN_ERR_UNSUPPORTED, "op_gated_ffn: there is no 32-bit form, GN_F16 or GN_BF16 is needed");
   const char* wrong = check_ffn(dtype, activation, tokens, dim, ff, {x, w_gate, w_up, w_down, y}, {x_stride, y_stride});
   if (!wrong && !aligned_to(saved, 16)) wrong = "saved is not 16-byte aligned";
   GN_OP_BEGIN("op_gated_ffn", wrong);
@@ -580,7 +580,7 @@ int gn_op_gated_ffn(gn_ctx* ctx, int dtype, int activation, int64_t tokens, int 
 int gn_op_gated_ffn_backward(gn_ctx* ctx, int dtype, int activation, int64_t tokens, int dim, int ff, const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, const void* w_gate, const void* w_up, const void* w_down,
                              const void* saved, void* dx, int64_t dx_stride, void* dw_gate, void* dw_up, void* dw_down, void* workspace, int64_t workspace_bytes, void* stream) {
   using namespace gn;
-  if (ctx && ctx->alive && dtype == GN_F32) return fail(GN_ERR_UNSUPPORTED, "op_gated_ffn_backward: GN_F32 is not built (TransformerBlock has the 32-bit form)");
+  if (ctx && ctx->alive && dtype == GN_F32) return fail(GN_ERR_UNSUPPORTED, "op_gated_ffn_backward: there is no 32-bit form, GN_F16 or GN_BF16 is needed");
   const char* wrong = check_ffn(dtype, activation, tokens, dim, ff, {dy, x, w_gate, w_up, w_down, saved}, {dy_stride, x_stride});
   if (!wrong && (!aligned_to(dx, 16) || !aligned_to(dw_gate, 16) || !aligned_to(dw_up, 16) || !aligned_to(dw_down, 16))) wrong = "a pointer is not 16-byte aligned";
   if (!wrong && dx) wrong = check_ffn_strides(tokens, dim, {dx_stride});

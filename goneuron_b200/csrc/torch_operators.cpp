@@ -217,7 +217,7 @@ Tensor embedding_backward(uint64_t handle, int index, const Tensor& dout, const 
 struct Ffn {
   Dev d; Rows x; int dim, ff, dtype;
   Ffn(const Dev& dev, const Tensor& xt, const Tensor& wg, const Tensor& wu, const Tensor& wd) : d(dev), x(rows("x", xt)), dtype(dtype_of("x", xt)) {
-    if (dtype == GN_F32) wrong("x is float32: float16 or bfloat16 is needed (TransformerBlock has the 32-bit form)");
+    if (dtype == GN_F32) wrong("x is float32: float16 or bfloat16 is needed, there is no 32-bit form");
     dense("w_gate", wg, xt.scalar_type(), {-1, x.dim});
     const int64_t f = wg.size(0);
     dense("w_up", wu, xt.scalar_type(), {f, x.dim}); dense("w_down", wd, xt.scalar_type(), {x.dim, f});

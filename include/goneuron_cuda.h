@@ -352,8 +352,8 @@ int gn_op_embedding_backward(gn_ctx* ctx, int dtype, int64_t tokens, int64_t voc
                              const void* ids, int index_type, float* dtable, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Gated feed-forward block: h = act(x Wg^T) * (x Wu^T), y = h Wd^T with x [tokens, dim] (rows x_stride apart), Wg and Wu [ff, dim],
- * Wd [dim, ff], dense; all GN_F16 or GN_BF16 (GN_F32: GN_ERR_UNSUPPORTED, TransformerBlock has the 32-bit form).  activation: GN_ACT_SILU,
- * GN_ACT_GELU (tanh form) or GN_ACT_RELU.  dim and ff are multiples of 8, pointers 16-byte aligned, x_stride and y_stride multiples of 8.
+ * Wd [dim, ff], dense; all GN_F16 or GN_BF16 (GN_F32: GN_ERR_UNSUPPORTED; the float32 block of TransformerBlock with SwiGLU belongs to a
+ * model and has the reference's gradient, not this one).  activation: GN_ACT_SILU, GN_ACT_GELU (tanh form) or GN_ACT_RELU.  dim and ff are multiples of 8, pointers 16-byte aligned, x_stride and y_stride multiples of 8.
  * One kernel forms both projections, the activation and the product; h is rounded to `dtype` between the two kernels (up to 8 tokens without
  * `saved` it is kept with twice its bits), and so are act'(g) u dh and act(g) dh in the backward pass.  In GN_F16 what is above 65504 there is
  * infinite and what is below 2^-25 zero: a row whose h does not fit has a y that is not finite, a loss scale has to leave room for those two
