@@ -32,7 +32,7 @@ def _handle(dev):
 
 def check(dev):
     """Waits for the current stream and raises GoNeuronCudaError for what operators found wrong on the GPU since the last call
-    that did: an id or index out of range, a bounded wait that gave up."""
+    that did, on whatever stream, thread or Device of it: an id or index out of range, a bounded wait that gave up."""
     _ops.status(_handle(dev), dev.device)
 
 

@@ -299,7 +299,8 @@ int gn_op_gemm_nt_static(gn_ctx* ctx, int M, int N, int K, const float* A_dev, c
 typedef enum gn_dtype { GN_F32 = 0, GN_F16 = 1, GN_BF16 = 2 } gn_dtype;
 typedef enum gn_index_type { GN_I32 = 0, GN_I64 = 1 } gn_index_type;
 
-/* Waits for `stream` and returns what the operators found wrong on this GPU since the last call that reported it:
+/* Waits for `stream` and returns what the operators found wrong on this GPU since the last call that reported it, on whatever stream, thread or
+ * context of the process (one word per GPU: whoever asks first gets it, and it is cleared):
  * GN_ERR_INVALID_ARG (a token id or teacher index out of range), GN_ERR_TIMEOUT (a bounded wait gave up), else GN_OK. */
 int gn_op_status(gn_ctx* ctx, void* stream);
 
