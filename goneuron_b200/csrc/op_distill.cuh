@@ -9,7 +9,7 @@
 //
 // Bound by memory: a row is read once and its gradient written once.  A row, or a block's part of it, lies in shared memory; every thread copies there, sums over and writes back its own
 // 16-byte pieces of it, so that the only barrier of a row is the one at which the warps' sums meet, and the copies of a thread's next row are under way as soon as it has written this one.
-// Blocks of an SM (three for rows of 64 KB) overlap each other's phases.  A row of more than 104 KB is spread over a cluster of blocks, whose barrier is then the cluster's.
+// Blocks of an SM (three for rows of 64 KB) overlap each other's phases.  A row of more than 104 KB (distill_plan has the rule) is spread over a cluster of blocks, whose barrier is then the cluster's.
 // One more warp of every block works on the teacher's few entries, a chain of dependent loads, one row ahead of the others (a launch of its own before this one: 58 of 162 us for 4096 rows of
 // 32000 with 64 entries, bf16).  The other warps write q everywhere; that warp writes q - p over it where the teacher has entries, behind the next row's barrier.
 // (Rows held as exponentials in registers, 64 elements a thread, which saves one of an element's two exponentials: 121 us without the teacher's part, 102 this way; the special-function units do not

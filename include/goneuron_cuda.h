@@ -337,7 +337,9 @@ int gn_op_qk_norm_rope_backward(gn_ctx* ctx, int dtype, int64_t tokens, int head
  * (the derivative of loss[r] by logits[r]; an index that occurs twice counts twice).  A row whose weight is 0, or that has no entry of
  * positive probability, has loss 0 and gradient 0 whatever its logits hold.  logits [rows, vocab] and dlogits (null: loss only; may be
  * logits in place) of `dtype`, rows row_stride / drow_stride elements apart; top_ids [rows, top] of index_type, top_logits float32 [rows, top],
- * dense; weight float32 [rows] (null: 1); loss float32 [rows].  top <= 1024.  An index outside [-1, vocab) counts as -1 and sets the status. */
+ * dense; weight float32 [rows] (null: 1); loss float32 [rows].  top <= 1024 (meant for tens to a few hundred: one warp works on
+ * a row's entries, which above that takes longer than all else).  An index outside [-1, vocab) counts as -1 and sets the status; rows
+ * whose weight is 0 are not looked at. */
 int gn_op_distill(gn_ctx* ctx, int dtype, int64_t rows, int64_t vocab, int top, float temperature,
                   const void* logits, int64_t row_stride, const void* top_ids, int index_type, const float* top_logits,
                   const float* weight, float* loss, void* dlogits, int64_t drow_stride, void* stream);
